@@ -212,6 +212,119 @@ IQ_API int iq_rmsnorm_dev(int64_t *d_out, const int64_t *d_x, const int64_t *d_w
 /* softmax (llama_int.c:1060-1072), in place, on `rows` vectors of length n. */
 IQ_API int iq_softmax_dev(int64_t *d_x, int rows, int n, void *stream);
 
+/* -------------------------------------- drafted tokens: rotary, cache, tree
+ *
+ * The calls below are the layer's pieces around the matrix products as
+ * operators on the caller's own buffers (device pointers on the current
+ * device, 8-byte aligned int64, 4-byte aligned int): rotate, write the cache,
+ * attend over it, score. They allocate nothing and never synchronise, so they
+ * can be captured into a CUDA graph (after one call on the device has set the
+ * library up). Index arrays are read on the device: a row whose index lies
+ * outside its range is left out and its outputs stay as they were. A negative
+ * index is the mark of a padding row; any other bad index is also recorded as
+ * IQ_ERR_RANGE in the device status (iq_device_status). */
+
+/* Rotary tables scaled for contexts beyond the trained one. The frequency of
+ * pair i is th_i = fp_exp(fp_mul(-fp_div(2i, rot_dim), ln theta))
+ * (rope_init, llama_int.c:960-986; below -10, where fp_exp leaves its range, the square
+ * of fp_exp of half the exponent), the angle p th_i (mod 2 pi, exact for every
+ * position), cos and sin fp_sincos of it.
+ *   LINEAR: th_i / factor.   NTK: ln theta + fp_log(factor) rot_dim / (rot_dim - 2).
+ *   PARTS:  t = orig_len th_i / (2 pi) turns over the trained context,
+ *           w = clamp((t - low) / (high - low), 0, 1),
+ *           fp_mul(th_i, w) + fp_mul(th_i / factor, 1 - w).
+ * mscale (0 = 1.0) multiplies cos and sin. factor in [1, 1024]. */
+enum { IQ_ROPE_SCALE_NONE = 0, IQ_ROPE_SCALE_LINEAR = 1, IQ_ROPE_SCALE_NTK = 2, IQ_ROPE_SCALE_PARTS = 3 };
+typedef struct iq_rope_scaling {
+    int kind, orig_len;
+    int64_t factor, low, high, mscale;   /* Q16.48 */
+} iq_rope_scaling;
+/* d_cos, d_sin [n_pos][rot_dim / 2] for positions 0 .. n_pos - 1 (n_pos <=
+ * 2^24, rot_dim even and <= 256, theta >= 1). Unscaled tables equal the
+ * model's (rope_init) at every position below 32768; IQ_ERR_RANGE when ln
+ * theta, after NTK, exceeds 20. scaling may be NULL. */
+IQ_API int iq_rope_tables_dev(int64_t *d_cos, int64_t *d_sin, int rot_dim, int n_pos, int theta,
+                              const iq_rope_scaling *scaling, void *stream);
+
+/* Which elements of a head turn together: i and i + rot_dim / 2 (rope_apply,
+ * llama_int.c:997-1008), or 2i and 2i + 1. Elements from rot_dim on are not
+ * rotated. d_pos: the row's position, an index into the tables. */
+enum { IQ_ROPE_HALF = 0, IQ_ROPE_INTERLEAVED = 1 };
+typedef struct iq_rope {
+    const int64_t *d_cos, *d_sin;   /* [n_pos][rot_dim / 2] */
+    const int *d_pos;               /* [rows] */
+    int n_pos, rot_dim, layout;
+} iq_rope;
+/* d_out row r [heads][head_dim] at r * out_stride = d_x row r (at r * x_stride)
+ * rotated: (a, b) -> (fp_mul(a, c) - fp_mul(b, s), fp_mul(b, c) + fp_mul(a, s)).
+ * d_out may be d_x with the same stride; any other overlap is undefined.
+ * head_dim <= 256. Rows at position < 0 or >= n_pos stay as they were. */
+IQ_API int iq_rope_dev(int64_t *d_out, const int64_t *d_x, const iq_rope *rope, int rows, int heads, int head_dim,
+                       int64_t x_stride, int64_t out_stride, void *stream);
+
+/* A KV cache in the caller's memory, in the model's layouts: exact (k_bits =
+ * v_bits = 0) k, v [seqs][max_seq][kv_heads][head_dim], or packed
+ * (--kv-packed KbVb, llama_int.c:1197-1235): K codes of k_bits (1..8) in bytes kq, V codes of
+ * v_bits (1..16) in 16-bit words vq, and a magnitude per vector k_mag, v_mag
+ * [seqs][max_seq][kv_heads]. head_dim <= 256. The unused pointers may be NULL. */
+typedef struct iq_kv_cache {
+    int seqs, max_seq, kv_heads, head_dim, k_bits, v_bits;
+    int64_t *k, *v;
+    uint8_t *kq;
+    uint16_t *vq;
+    int64_t *k_mag, *v_mag;
+} iq_kv_cache;
+/* Writes row r's K and V [kv_heads][head_dim] (at r * k_stride, r * v_stride)
+ * to slot d_slot[r] of sequence d_seq[r] (d_seq NULL: all rows of sequence 0),
+ * K rotated first when rope is given, packed by kv_pack_vector
+ * (llama_int.c:1197-1218) in a packed cache. Rows of one call must name
+ * different slots. Rows outside the cache are left out, a row at a position
+ * outside the rotary tables too. */
+IQ_API int iq_kv_write_dev(const iq_kv_cache *cache, const int64_t *d_k, const int64_t *d_v, const int *d_seq,
+                           const int *d_slot, int rows, int64_t k_stride, int64_t v_stride, const iq_rope *rope,
+                           void *stream);
+/* d_k, d_v [rows][kv_heads][head_dim]: the values attention reads at those
+ * slots (kv_unpack_vector, llama_int.c:1226-1235, in a packed cache). */
+IQ_API int iq_kv_read_dev(int64_t *d_k, int64_t *d_v, const iq_kv_cache *cache, const int *d_seq, const int *d_slot,
+                          int rows, void *stream);
+
+/* Attention of drafted tokens over the cache. Sequence i (of n_seq) reads cache
+ * sequence d_seq[i] (NULL: i): d_len[i] positions before the draft, then its
+ * n_i = d_start[i + 1] - d_start[i] drafted nodes in slots d_len[i] + 0, 1, ...
+ * Rows d_start[i] .. of d_q are the nodes' queries (rotated; [num_heads]
+ * [head_dim] at r * q_stride); d_parent[r] is the node's parent, an earlier node of
+ * the same sequence counted from 0, or -1. A node attends to every position
+ * before the draft, its ancestors and itself, with the model's arithmetic
+ * (llama_int.c:1432-1529): a chain of nodes gives what the same tokens one by one give,
+ * a single node a decode step. d_out [rows][num_heads * head_dim] must not
+ * overlap d_q. A parent that is not an earlier node counts as -1.
+ * max_nodes (<= 256) and max_len (<= max_seq, <= 32767, the range of the
+ * int64 softmax sum) bound n_i and d_len[i] + n_i; rows of a sequence beyond its
+ * bounds, and rows outside d_start, stay as they were.
+ * d_work: iq_attn_tree_work bytes (8-byte aligned) that no other call uses
+ * until this one has run. */
+IQ_API int iq_attn_tree_work(const iq_kv_cache *cache, int num_heads, int n_seq, int rows, int max_nodes, int max_len,
+                             int64_t *bytes);
+IQ_API int iq_attn_tree_dev(int64_t *d_out, const int64_t *d_q, const iq_kv_cache *cache, int num_heads,
+                            const int *d_seq, const int *d_len, const int *d_start, const int *d_parent, int n_seq,
+                            int rows, int max_nodes, int max_len, int64_t q_stride, void *d_work, int64_t work_bytes,
+                            void *stream);
+
+/* Log probabilities of rows of logits (d_logits row r at r * ld; vocab <=
+ * 2^20) in Q16.48 nats. With m = max l, d = m - l, E(d) = e^-d rounded down to
+ * Q16.48 (within 2^-44 relative above 2^-48, no cut-off at 10 as in
+ * fp_safe_exp) and S = sum E(d):
+ *   d_logp[r] = -d_token - ln S for the row's given token (d_tokens NULL: none),
+ *   d_entropy[r] = ln S + (sum fp_mul(E(d), d)) / S (may be NULL),
+ *   d_top_ids, d_top_logp [rows][top]: the `top` (0..32) largest logits in
+ *   falling order, equal ones by rising index, and their log probabilities.
+ * A log probability below INT64_MIN is INT64_MIN. Every step is a whole-number
+ * operation, so results are the same on every run and machine. A token outside
+ * the vocabulary leaves d_logp[r] as it was. */
+IQ_API int iq_logprobs_dev(const int64_t *d_logits, int64_t ld, int rows, int vocab, const int *d_tokens,
+                           int64_t *d_logp, int64_t *d_entropy, int top, int *d_top_ids, int64_t *d_top_logp,
+                           void *stream);
+
 /* ----------------------------------------------------------------- model */
 
 /* llama_config_t (llama_int.c:788-798), same fields and meaning. */

@@ -1,0 +1,235 @@
+// iq_ops.cu -- C ABI of the operators around drafted tokens: rotary tables and
+// rotation, cache rows, tree attention, log probabilities (declared in iq.h).
+#include <climits>
+#include "iq_common.cuh"
+#include "iq_ops.cuh"
+#include "iq_tree.cuh"
+#include "iq_score.cuh"
+
+using namespace iq;
+
+static bool misaligned(const void *p, size_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
+
+// ---- host copies of the fp_math steps that a table's constants need
+
+static int64_t h_mul(int64_t a, int64_t b) { return (int64_t)(((i128)a * b) >> 48); }
+static int64_t h_exp(int64_t x) {   // fp_exp (fp_math.h:714-732)
+    int64_t r = IQ_ONE + ((x < 0 ? -x : x) >> 14);
+    for (int i = 0; i < 14; i++) r = h_mul(r, r);
+    return x >= 0 ? r : r ? (int64_t)(((u128)1 << 96) / (u128)(uint64_t)r) : 0;
+}
+#define IQ_LN2 195103586505167LL
+static int64_t h_log(int64_t x) {   // fp_log (fp_math.h:752-771), x > 0
+    int64_t y = (int64_t)(63 - __builtin_clzll((uint64_t)x) - 48) * IQ_LN2;
+    for (int i = 0; i < 10; i++) {
+        const int64_t ey = h_exp(y);
+        if (ey == 0) break;
+        const int64_t yn = y - IQ_ONE + (int64_t)(((i128)x << 48) / ey);
+        const int64_t d = yn < y ? y - yn : yn - y;
+        if (d < 2) break;
+        y = yn;
+    }
+    return y;
+}
+// ln of a whole number: fp_log below 2^14, where its Newton steps stay in the
+// range of fp_exp; above, of theta / 2^k, plus k ln 2
+static int64_t h_ln_int(int theta) {
+    const int bl = 32 - __builtin_clz((unsigned)theta), k = bl > 14 ? bl - 14 : 0;
+    return h_log((int64_t)(((uint64_t)theta << 48 - k))) + k * IQ_LN2;
+}
+
+// fp_inv_sqrt(fp_from_int(hd)) (fp_math.h:658-707): the score scale (llama_int.c:1433)
+static int64_t h_att_scale(int hd) {
+    const int64_t x = (int64_t)hd << 48;
+    const int k = (63 - __builtin_clzll((uint64_t)x) - 48) >> 1;
+    const int64_t n = x >> (2 * k);
+    int64_t y = 63 - __builtin_clzll((uint64_t)n) == 48 ? IQ_ONE : IQ_ONE >> 1;
+    for (int i = 0; i < 8; i++) y = (int64_t)(((i128)y * (3 * IQ_ONE - h_mul(n, h_mul(y, y)))) >> 49);
+    return y >> k;
+}
+
+static int rope_check(const iq_rope *r, int hd, RopeArgs *a) {
+    if (!r || !r->d_cos || !r->d_sin || !r->d_pos || r->n_pos < 1 || r->rot_dim < 2 || (r->rot_dim & 1) ||
+        r->rot_dim > hd || (r->layout != IQ_ROPE_HALF && r->layout != IQ_ROPE_INTERLEAVED))
+        return IQ_ERR_ARG;
+    if (misaligned(r->d_cos, 8) || misaligned(r->d_sin, 8) || misaligned(r->d_pos, 4)) return IQ_ERR_ARG;
+    *a = RopeArgs{r->d_cos, r->d_sin, r->d_pos, r->n_pos, r->rot_dim, r->layout};
+    return IQ_OK;
+}
+
+static int cache_check(const iq_kv_cache *c, KVArgs *a) {
+    if (!c || c->seqs < 1 || c->max_seq < 1 || c->kv_heads < 1 || c->head_dim < 1 || c->head_dim > 256 ||
+        c->kv_heads > 65536)
+        return IQ_ERR_ARG;
+    const bool packed = c->k_bits || c->v_bits;
+    if (packed) {
+        if (c->k_bits < 1 || c->k_bits > 8 || c->v_bits < 1 || c->v_bits > 16) return IQ_ERR_ARG;
+        if (!c->kq || !c->vq || !c->k_mag || !c->v_mag || misaligned(c->vq, 2) || misaligned(c->k_mag, 8) ||
+            misaligned(c->v_mag, 8))
+            return IQ_ERR_ARG;
+    } else if (!c->k || !c->v || misaligned(c->k, 8) || misaligned(c->v, 8)) {
+        return IQ_ERR_ARG;
+    }
+    *a = KVArgs{c->k, c->v, c->kq, c->vq, c->k_mag, c->v_mag, c->seqs, c->max_seq, c->kv_heads, c->head_dim,
+                c->k_bits, c->v_bits};
+    return IQ_OK;
+}
+
+extern "C" {
+
+IQ_API int iq_rope_tables_dev(int64_t *d_cos, int64_t *d_sin, int rot_dim, int n_pos, int theta,
+                              const iq_rope_scaling *sc, void *stream) {
+    if (!d_cos || !d_sin || misaligned(d_cos, 8) || misaligned(d_sin, 8) || rot_dim < 2 || rot_dim > 256 ||
+        (rot_dim & 1) || n_pos < 1 || n_pos > (1 << 24) || theta < 1)
+        return IQ_ERR_ARG;
+    RopeTab t = {rot_dim / 2, rot_dim, n_pos, IQ_ROPE_SCALE_NONE, 0, h_ln_int(theta), IQ_ONE, 0, IQ_ONE, 0};
+    if (sc) {
+        if (sc->kind < IQ_ROPE_SCALE_NONE || sc->kind > IQ_ROPE_SCALE_PARTS || sc->mscale < 0 ||
+            sc->mscale > 1024 * IQ_ONE)
+            return IQ_ERR_ARG;
+        if (sc->kind != IQ_ROPE_SCALE_NONE && (sc->factor < IQ_ONE || sc->factor > 1024 * IQ_ONE)) return IQ_ERR_ARG;
+        t.kind = sc->kind;
+        t.mscale = sc->mscale == IQ_ONE ? 0 : sc->mscale;
+        if (sc->kind != IQ_ROPE_SCALE_NONE) t.factor = sc->factor;
+        if (sc->kind == IQ_ROPE_SCALE_NTK) {
+            if (rot_dim < 4) return IQ_ERR_ARG;
+            t.ln_theta += h_mul(h_log(sc->factor), (int64_t)(((i128)rot_dim << 48) / (rot_dim - 2)));
+        }
+        if (sc->kind == IQ_ROPE_SCALE_PARTS) {
+            // orig_len <= 2^16 and th <= 1: the turns stay below 2^14
+            if (sc->orig_len < 1 || sc->orig_len > (1 << 16) || sc->low < 0 || sc->high <= sc->low) return IQ_ERR_ARG;
+            t.orig_len = sc->orig_len;
+            t.low = sc->low;
+            t.span = sc->high - sc->low;
+        }
+    }
+    if (t.ln_theta > 20 * IQ_ONE) return IQ_ERR_RANGE;
+    int dev, rc;
+    if ((rc = cur_device(&dev))) return rc;
+    const int64_t n = (int64_t)n_pos * t.half, blocks = (n + 255) / 256, cap = (int64_t)dev_info().sms * 8;
+    k_rope_tables<<<(int)(blocks < cap ? blocks : cap), 256, 0, pick(stream)>>>(d_cos, d_sin, t);
+    IQ_CHECK_LAUNCH();
+    return IQ_OK;
+}
+
+IQ_API int iq_rope_dev(int64_t *d_out, const int64_t *d_x, const iq_rope *rope, int rows, int heads, int head_dim,
+                       int64_t x_stride, int64_t out_stride, void *stream) {
+    RopeArgs r;
+    if (!d_out || !d_x || misaligned(d_out, 8) || misaligned(d_x, 8) || rows < 0 || heads < 1 || heads > 65536 ||
+        head_dim < 1 || head_dim > 256)
+        return IQ_ERR_ARG;
+    const int64_t w = (int64_t)heads * head_dim;
+    if (x_stride < w || out_stride < w || (d_out == d_x && x_stride != out_stride)) return IQ_ERR_ARG;
+    int dev, rc;
+    if ((rc = rope_check(rope, head_dim, &r))) return rc;
+    if (rows == 0) return IQ_OK;
+    if ((rc = cur_device(&dev))) return rc;
+    const int items = heads * ((head_dim + 1) / 2);
+    int tx = 256;
+    while (tx > 32 && tx / 2 >= items) tx /= 2;
+    const dim3 block(tx, 256 / tx), grid((rows + block.y - 1) / block.y, std::min(64, (items + tx - 1) / tx));
+    k_rope<<<grid, block, 0, pick(stream)>>>(d_out, d_x, r, rows, heads, head_dim, x_stride, out_stride);
+    IQ_CHECK_LAUNCH();
+    return IQ_OK;
+}
+
+IQ_API int iq_kv_write_dev(const iq_kv_cache *cache, const int64_t *d_k, const int64_t *d_v, const int *d_seq,
+                           const int *d_slot, int rows, int64_t k_stride, int64_t v_stride, const iq_rope *rope,
+                           void *stream) {
+    KVArgs c;
+    RopeArgs r = {};
+    int dev, rc;
+    if ((rc = cache_check(cache, &c))) return rc;
+    const int64_t w = (int64_t)c.nkv * c.hd;
+    if (!d_k || !d_v || !d_slot || misaligned(d_k, 8) || misaligned(d_v, 8) || misaligned(d_slot, 4) ||
+        misaligned(d_seq, 4) || rows < 0 || k_stride < w || v_stride < w || (int64_t)rows * c.nkv > INT_MAX / 2)
+        return IQ_ERR_ARG;
+    if (rope && (rc = rope_check(rope, c.hd, &r))) return rc;
+    if (rows == 0) return IQ_OK;
+    if ((rc = cur_device(&dev))) return rc;
+    const int blocks = (int)(((int64_t)rows * c.nkv * 2 + 7) / 8);
+    if (c.kbits)
+        k_kv_write<true><<<blocks, 256, 0, pick(stream)>>>(c, d_k, d_v, d_seq, d_slot, rows, k_stride, v_stride, r);
+    else
+        k_kv_write<false><<<blocks, 256, 0, pick(stream)>>>(c, d_k, d_v, d_seq, d_slot, rows, k_stride, v_stride, r);
+    IQ_CHECK_LAUNCH();
+    return IQ_OK;
+}
+
+IQ_API int iq_kv_read_dev(int64_t *d_k, int64_t *d_v, const iq_kv_cache *cache, const int *d_seq, const int *d_slot,
+                          int rows, void *stream) {
+    KVArgs c;
+    int dev, rc;
+    if ((rc = cache_check(cache, &c))) return rc;
+    if (!d_k || !d_v || !d_slot || misaligned(d_k, 8) || misaligned(d_v, 8) || misaligned(d_slot, 4) ||
+        misaligned(d_seq, 4) || rows < 0 || (int64_t)rows * c.nkv > INT_MAX / 2)
+        return IQ_ERR_ARG;
+    if (rows == 0) return IQ_OK;
+    if ((rc = cur_device(&dev))) return rc;
+    const int blocks = (int)(((int64_t)rows * c.nkv * 2 + 7) / 8);
+    k_kv_read<<<blocks, 256, 0, pick(stream)>>>(d_k, d_v, c, d_seq, d_slot, rows);
+    IQ_CHECK_LAUNCH();
+    return IQ_OK;
+}
+
+static int tree_check(const iq_kv_cache *cache, int nh, int n_seq, int rows, int max_nodes, int max_len, KVArgs *c) {
+    int rc;
+    if ((rc = cache_check(cache, c))) return rc;
+    if (nh < 1 || nh > 4096 || nh % c->nkv || n_seq < 1 || n_seq > 65536 || rows < 1 || max_nodes < 1 || max_len < 1) return IQ_ERR_ARG;
+    if (max_nodes > TREE_MAX_NODES || max_len > c->max_seq || max_len > 32767)
+        return IQ_ERR_RANGE;
+    return IQ_OK;
+}
+
+IQ_API int iq_attn_tree_work(const iq_kv_cache *cache, int num_heads, int n_seq, int rows, int max_nodes, int max_len,
+                             int64_t *bytes) {
+    KVArgs c;
+    int rc;
+    if (!bytes) return IQ_ERR_ARG;
+    if ((rc = tree_check(cache, num_heads, n_seq, rows, max_nodes, max_len, &c))) return rc;
+    *bytes = (int64_t)rows * num_heads * max_len * 8;
+    return IQ_OK;
+}
+
+IQ_API int iq_attn_tree_dev(int64_t *d_out, const int64_t *d_q, const iq_kv_cache *cache, int num_heads,
+                            const int *d_seq, const int *d_len, const int *d_start, const int *d_parent, int n_seq,
+                            int rows, int max_nodes, int max_len, int64_t q_stride, void *d_work, int64_t work_bytes,
+                            void *stream) {
+    TreeArgs a = {};
+    int dev, rc;
+    int64_t need;
+    if ((rc = tree_check(cache, num_heads, n_seq, rows, max_nodes, max_len, &a.c))) return rc;
+    if ((rc = iq_attn_tree_work(cache, num_heads, n_seq, rows, max_nodes, max_len, &need))) return rc;
+    if (!d_out || !d_q || !d_len || !d_start || !d_parent || misaligned(d_out, 8) || misaligned(d_q, 8) ||
+        misaligned(d_len, 4) || misaligned(d_start, 4) || misaligned(d_parent, 4) || misaligned(d_seq, 4) ||
+        misaligned(d_work, 8) || d_out == d_q || q_stride < (int64_t)num_heads * a.c.hd || work_bytes < need ||
+        (need && !d_work))
+        return IQ_ERR_ARG;
+    if ((rc = cur_device(&dev))) return rc;
+    a.out = d_out; a.q = d_q; a.seq = d_seq; a.len = d_len; a.start = d_start; a.parent = d_parent;
+    a.n_seq = n_seq; a.rows = rows; a.max_nodes = max_nodes; a.max_len = max_len; a.nh = num_heads;
+    a.qs = q_stride; a.sc = (int64_t *)d_work;
+    a.scale = h_att_scale(a.c.hd);
+    k_tree_simple<<<dim3(n_seq * max_nodes, num_heads), 256, 0, pick(stream)>>>(a);
+    IQ_CHECK_LAUNCH();
+    return IQ_OK;
+}
+
+IQ_API int iq_logprobs_dev(const int64_t *d_logits, int64_t ld, int rows, int vocab, const int *d_tokens,
+                           int64_t *d_logp, int64_t *d_entropy, int top, int *d_top_ids, int64_t *d_top_logp,
+                           void *stream) {
+    if (!d_logits || rows < 0 || vocab < 1 || ld < vocab || !d_tokens != !d_logp || top < 0 || top > vocab ||
+        (top && (!d_top_ids || !d_top_logp)) || misaligned(d_logits, 8) || misaligned(d_tokens, 4) ||
+        misaligned(d_logp, 8) || misaligned(d_entropy, 8) || misaligned(d_top_ids, 4) || misaligned(d_top_logp, 8))
+        return IQ_ERR_ARG;
+    if (vocab > (1 << 20) || top > IQ_LP_MAX_TOP) return IQ_ERR_RANGE;
+    if (rows == 0) return IQ_OK;
+    int dev, rc;
+    if ((rc = cur_device(&dev))) return rc;
+    const LpArgs a = {d_logits, ld, rows, vocab, top, d_tokens, d_logp, d_entropy, d_top_ids, d_top_logp};
+    k_logprobs_simple<<<rows, 1024, 0, pick(stream)>>>(a);
+    IQ_CHECK_LAUNCH();
+    return IQ_OK;
+}
+
+}  // extern "C"

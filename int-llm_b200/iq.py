@@ -59,6 +59,13 @@ SIGNATURES = {
     "iq_fp_dev": (_I, [_I, _P, _P, _P, _I64, _P]),
     "iq_rmsnorm_dev": (_I, [_P, _P, _P, _I, _I, _P]),
     "iq_softmax_dev": (_I, [_P, _I, _I, _P]),
+    "iq_rope_tables_dev": (_I, [_P, _P, _I, _I, _I, _P, _P]),
+    "iq_rope_dev": (_I, [_P, _P, _P, _I, _I, _I, _I64, _I64, _P]),
+    "iq_kv_write_dev": (_I, [_P, _P, _P, _P, _P, _I, _I64, _I64, _P, _P]),
+    "iq_kv_read_dev": (_I, [_P, _P, _P, _P, _P, _I, _P]),
+    "iq_attn_tree_work": (_I, [_P, _I, _I, _I, _I, _I, _P]),
+    "iq_attn_tree_dev": (_I, [_P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I64, _P, _I64, _P]),
+    "iq_logprobs_dev": (_I, [_P, _I64, _I, _I, _P, _P, _P, _I, _P, _P, _P]),
     "iq_model_create": (_I, [_P, _I, _I, _P]),
     "iq_nccl_unique_id": (_I, [_P]),
     "iq_tp_shard_info": (_I, [_P, _I, _I, _P]),
@@ -344,6 +351,111 @@ def rmsnorm_dev(out, x, w, rows, dim, stream=None):
 
 def softmax_dev(x, rows, n, stream=None):
     _call("iq_softmax_dev", _dp(x), rows, n, _sp(stream))
+
+
+# ------------------------- drafted tokens: rotary, cache, tree attention, scores
+
+def _dev_ptr(t, itemsize, name):
+    """Device pointer of t (None: NULL) after checking its element size and that
+    it lies on the device that calls go to (torch's current one)."""
+    if t is None:
+        return None
+    size = t.element_size() if hasattr(t, "element_size") else t.itemsize
+    if size != itemsize:
+        raise ValueError(f"{name}: {itemsize}-byte elements expected, got {size}")
+    d = getattr(t, "device", None)
+    if d is not None and getattr(d, "type", "cuda") != "cuda":
+        raise ValueError(f"{name} must be in device memory, got {d}")
+    if d is not None and getattr(d, "index", None) is not None:
+        import torch
+        if d.index != torch.cuda.current_device():
+            raise ValueError(f"{name} lies on {d}, calls go to cuda:{torch.cuda.current_device()}")
+    return t.data_ptr()
+
+
+ROPE_LAYOUT = dict(half=0, interleaved=1)
+ROPE_SCALE = dict(none=0, linear=1, ntk=2, parts=3)
+
+
+class _RopeScaling(ctypes.Structure):
+    _fields_ = [("kind", _I), ("orig_len", _I), ("factor", _I64), ("low", _I64), ("high", _I64), ("mscale", _I64)]
+
+
+def rope_tables_dev(cos, sin, rot_dim, n_pos, theta, scaling=None, stream=None):
+    """Tables [n_pos][rot_dim / 2]; scaling: dict of kind, factor, orig_len, low, high, mscale (Q16.48 ints)."""
+    sc = None
+    if scaling is not None:
+        f = dict(scaling)
+        f["kind"] = ROPE_SCALE[f.get("kind", "none")]
+        sc = ctypes.byref(_RopeScaling(**f))
+    _call("iq_rope_tables_dev", _dev_ptr(cos, 8, "cos"), _dev_ptr(sin, 8, "sin"), rot_dim, n_pos, theta, sc,
+          _sp(stream))
+
+
+class Rope(ctypes.Structure):
+    """iq_rope: tables, the rows' positions (int32) and the layout ('half' or 'interleaved')."""
+    _fields_ = [("d_cos", _P), ("d_sin", _P), ("d_pos", _P), ("n_pos", _I), ("rot_dim", _I), ("layout", _I)]
+
+    def __init__(self, cos, sin, pos, n_pos, rot_dim, layout="half"):
+        super().__init__(_dev_ptr(cos, 8, "cos"), _dev_ptr(sin, 8, "sin"), _dev_ptr(pos, 4, "pos"), n_pos, rot_dim,
+                         ROPE_LAYOUT[layout])
+        self.keep = (cos, sin, pos)
+
+
+def rope_dev(out, x, rope, rows, heads, head_dim, x_stride=None, out_stride=None, stream=None):
+    w = heads * head_dim
+    _call("iq_rope_dev", _dev_ptr(out, 8, "out"), _dev_ptr(x, 8, "x"), ctypes.byref(rope), rows, heads, head_dim,
+          w if x_stride is None else x_stride, w if out_stride is None else out_stride, _sp(stream))
+
+
+class KVCache(ctypes.Structure):
+    """iq_kv_cache over the caller's tensors: k and v (exact), or kq, vq, k_mag, v_mag with k_bits and v_bits."""
+    _fields_ = [("seqs", _I), ("max_seq", _I), ("kv_heads", _I), ("head_dim", _I), ("k_bits", _I), ("v_bits", _I),
+                ("k", _P), ("v", _P), ("kq", _P), ("vq", _P), ("k_mag", _P), ("v_mag", _P)]
+
+    def __init__(self, seqs, max_seq, kv_heads, head_dim, k=None, v=None, kq=None, vq=None, k_mag=None, v_mag=None,
+                 k_bits=0, v_bits=0):
+        super().__init__(seqs, max_seq, kv_heads, head_dim, k_bits, v_bits, _dev_ptr(k, 8, "k"), _dev_ptr(v, 8, "v"),
+                         _dev_ptr(kq, 1, "kq"), _dev_ptr(vq, 2, "vq"), _dev_ptr(k_mag, 8, "k_mag"),
+                         _dev_ptr(v_mag, 8, "v_mag"))
+        self.keep = (k, v, kq, vq, k_mag, v_mag)
+
+
+def kv_write_dev(cache, k, v, slot, rows, seq=None, rope=None, k_stride=None, v_stride=None, stream=None):
+    w = cache.kv_heads * cache.head_dim
+    _call("iq_kv_write_dev", ctypes.byref(cache), _dev_ptr(k, 8, "k"), _dev_ptr(v, 8, "v"), _dev_ptr(seq, 4, "seq"),
+          _dev_ptr(slot, 4, "slot"), rows, w if k_stride is None else k_stride, w if v_stride is None else v_stride,
+          ctypes.byref(rope) if rope is not None else None, _sp(stream))
+
+
+def kv_read_dev(k, v, cache, slot, rows, seq=None, stream=None):
+    _call("iq_kv_read_dev", _dev_ptr(k, 8, "k"), _dev_ptr(v, 8, "v"), ctypes.byref(cache), _dev_ptr(seq, 4, "seq"),
+          _dev_ptr(slot, 4, "slot"), rows, _sp(stream))
+
+
+def attn_tree_work(cache, num_heads, n_seq, rows, max_nodes, max_len):
+    """Workspace bytes of attn_tree_dev."""
+    n = _I64()
+    _call("iq_attn_tree_work", ctypes.byref(cache), num_heads, n_seq, rows, max_nodes, max_len, ctypes.byref(n))
+    return n.value
+
+
+def attn_tree_dev(out, q, cache, num_heads, lens, starts, parents, n_seq, rows, max_nodes, max_len, work=None,
+                  seqs=None, q_stride=None, stream=None):
+    """Tree attention; work: a device tensor of at least attn_tree_work(...) bytes."""
+    nbytes = 0 if work is None else work.numel() * work.element_size()
+    _call("iq_attn_tree_dev", _dev_ptr(out, 8, "out"), _dev_ptr(q, 8, "q"), ctypes.byref(cache), num_heads,
+          _dev_ptr(seqs, 4, "seqs"), _dev_ptr(lens, 4, "lens"), _dev_ptr(starts, 4, "starts"),
+          _dev_ptr(parents, 4, "parents"), n_seq, rows, max_nodes, max_len,
+          num_heads * cache.head_dim if q_stride is None else q_stride,
+          None if work is None else _dev_ptr(work, work.element_size(), "work"), nbytes, _sp(stream))
+
+
+def logprobs_dev(logits, rows, vocab, tokens=None, logp=None, entropy=None, top=0, top_ids=None, top_logp=None,
+                 ld=None, stream=None):
+    _call("iq_logprobs_dev", _dev_ptr(logits, 8, "logits"), vocab if ld is None else ld, rows, vocab,
+          _dev_ptr(tokens, 4, "tokens"), _dev_ptr(logp, 8, "logp"), _dev_ptr(entropy, 8, "entropy"), top,
+          _dev_ptr(top_ids, 4, "top_ids"), _dev_ptr(top_logp, 8, "top_logp"), _sp(stream))
 
 
 # --------------------------------------------------------- synthetic inputs

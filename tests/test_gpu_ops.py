@@ -1,0 +1,656 @@
+"""GPU tests of the operators around drafted tokens against whole-number
+references (ops_ref): every result is an integer defined exactly, so equality
+is the tolerance."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import configs
+import iq
+import ops_ref as ref
+from helpers import ONE, model_weights
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+RANGE = -6
+KEEP = -7777777          # what outputs hold before a call
+
+
+def dev(a, dtype=None):
+    t = torch.from_numpy(np.ascontiguousarray(a))
+    return (t.to(dtype) if dtype else t).cuda()
+
+
+def i32(a):
+    return dev(np.asarray(a, np.int32))
+
+
+def full(*shape):
+    return torch.full(shape, KEEP, dtype=torch.int64, device="cuda")
+
+
+def rnd(rng, *shape, scale=1.0):
+    return ref.q48(rng.standard_normal(shape) * scale)
+
+
+def wide(rng, *shape):
+    """Values over the whole int64 range, the ends among them."""
+    a = rng.integers(-(1 << 63), (1 << 63) - 1, shape, dtype=np.int64)
+    f = a.reshape(-1)
+    f[: min(4, f.size)] = [ref.I64_MIN, ref.I64_MAX, 0, -1][: min(4, f.size)]
+    return a
+
+
+@pytest.fixture(autouse=True)
+def clean_status():
+    iq.device_status()
+    yield
+    assert iq.device_status() == 0
+
+
+# ------------------------------------------------------------------- rotary
+
+SCALES = [dict(), dict(kind="linear", factor=4 * ONE), dict(kind="ntk", factor=ONE * 5 // 2),
+          dict(kind="parts", factor=8 * ONE, orig_len=2048, low=ONE, high=32 * ONE),
+          dict(kind="parts", factor=3 * ONE, orig_len=100, low=0, high=ONE, mscale=ONE * 9 // 8),
+          dict(kind="none", mscale=ONE // 2), dict(kind="linear", factor=ONE)]
+
+
+@pytest.mark.parametrize("sc", SCALES)
+@pytest.mark.parametrize("rot,theta", [(64, 10000), (4, 16383), (256, 1000000), (30, 1)])
+def test_rope_tables(rot, theta, sc):
+    n = 70000
+    cos, sin = full(n, rot // 2), full(n, rot // 2)
+    iq.rope_tables_dev(cos, sin, rot, n, theta, sc or None)
+    at = [0, 1, 2, 3, 77, 2047, 32767, 32768, 69999]
+    c, s = ref.tables(rot, at, theta, **sc)
+    assert (cos[at].cpu().numpy() == c).all() and (sin[at].cpu().numpy() == s).all()
+    assert int((cos == KEEP).sum()) == 0 and int((sin == KEEP).sum()) == 0
+
+
+def test_rope_tables_far_and_single():
+    n = 1 << 24
+    cos, sin = full(n, 1), full(n, 1)
+    iq.rope_tables_dev(cos, sin, 2, n, 10000)
+    at = [0, n - 1, n // 3]
+    c, s = ref.tables(2, at, 10000)
+    assert (cos[at].cpu().numpy() == c).all() and (sin[at].cpu().numpy() == s).all()
+    one = full(1, 3)
+    iq.rope_tables_dev(one, one.clone(), 6, 1, 10000)
+    assert (one.cpu().numpy() == ref.tables(6, [0], 10000)[0]).all()
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("rows,heads,hd,rot,xs,os", [
+    (1, 36, 64, 64, 0, 0), (5, 3, 128, 96, 1, 3), (7, 1, 2, 2, 0, 0), (3, 2, 33, 32, 0, 5), (2, 5, 255, 14, 1, 0),
+    (130, 4, 256, 256, 2, 2), (9, 2, 6, 4, 0, 0), (2, 3, 20, 20, 1, 1), (2, 70, 40, 8, 4, 2)])
+def test_rope(layout, rows, heads, hd, rot, xs, os):
+    rng = np.random.default_rng(rows * 1000 + hd)
+    w, n = heads * hd, 50
+    x = wide(rng, rows, w + xs) if rows % 2 else rnd(rng, rows, w + xs, scale=3)
+    cos, sin = rnd(rng, n, rot // 2), rnd(rng, n, rot // 2)
+    pos = rng.integers(0, n, rows)
+    pos[rows // 2] = -1 if rows > 2 else pos[rows // 2]
+    out = full(rows, w + os)
+    r = iq.Rope(dev(cos), dev(sin), i32(pos), n, rot, layout)
+    iq.rope_dev(out, dev(x), r, rows, heads, hd, x_stride=w + xs, out_stride=w + os)
+    want = np.full((rows, w + os), KEEP, np.int64)
+    live = pos >= 0
+    want[live, :w] = ref.rotate(x[:, :w].reshape(rows, heads, hd), cos[pos], sin[pos], rot, layout)[live].reshape(-1, w)
+    assert (out.cpu().numpy() == want).all()
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rope_in_place_unaligned_and_bad_position(layout):
+    rng = np.random.default_rng(5)
+    rows, heads, hd, n = 6, 3, 48, 9
+    x, cos, sin = rnd(rng, rows, heads * hd), rnd(rng, n, 12), rnd(rng, n, 12)
+    pos = np.array([0, 8, 9, 3, -1, 1 << 30])
+    buf = torch.empty(rows * heads * hd + 1, dtype=torch.int64, device="cuda")
+    d = buf[1:]                                   # 8-byte aligned only
+    d.copy_(dev(x).flatten())
+    iq.rope_dev(d, d, iq.Rope(dev(cos), dev(sin), i32(pos), n, 24, layout), rows, heads, hd)
+    want = x.copy().reshape(rows, heads, hd)
+    live = (pos >= 0) & (pos < n)
+    want[live] = ref.rotate(want[live], cos[pos[live]], sin[pos[live]], 24, layout)
+    assert (d.cpu().numpy().reshape(want.shape) == want).all()
+    assert iq.device_status() == RANGE
+
+
+# -------------------------------------------------------------------- cache
+
+def new_cache(seqs, max_seq, nkv, hd, kb, vb):
+    """(cache, its tensors), all elements KEEP or a small mark."""
+    if kb:
+        t = dict(kq=torch.full((seqs, max_seq, nkv, hd), 77, dtype=torch.uint8, device="cuda"),
+                 vq=torch.full((seqs, max_seq, nkv, hd), 77, dtype=torch.int16, device="cuda"),
+                 k_mag=full(seqs, max_seq, nkv), v_mag=full(seqs, max_seq, nkv))
+    else:
+        t = dict(k=full(seqs, max_seq, nkv, hd), v=full(seqs, max_seq, nkv, hd))
+    return iq.KVCache(seqs, max_seq, nkv, hd, k_bits=kb, v_bits=vb, **t), t
+
+
+def host_cache(t):
+    h = {n: x.cpu().numpy().copy() for n, x in t.items()}
+    if "vq" in h:
+        h["vq"] = h["vq"].view(np.uint16)
+    return h
+
+
+def write_ref(h, k, v, seq, slot, kb, vb):
+    for r in range(len(slot)):
+        for head in range(k.shape[1]):
+            at = (seq[r], slot[r], head)
+            if kb:
+                h["kq"][at], h["k_mag"][at] = ref.pack(k[r, head], kb)
+                h["vq"][at], h["v_mag"][at] = ref.pack(v[r, head], vb)
+            else:
+                h["k"][at], h["v"][at] = k[r, head], v[r, head]
+
+
+@pytest.mark.parametrize("kb,vb", [(0, 0), (8, 10), (1, 1), (4, 16), (8, 16)])
+@pytest.mark.parametrize("rows,nkv,hd,rot,layout", [
+    (1, 4, 64, 64, "half"), (9, 2, 128, 96, "interleaved"), (3, 3, 1, 0, ""), (5, 1, 255, 128, "half"),
+    (4, 2, 256, 256, "interleaved"), (33, 1, 40, 0, ""), (6, 2, 65, 2, "half")])
+def test_kv_write_and_read(kb, vb, rows, nkv, hd, rot, layout):
+    rng = np.random.default_rng(rows * 100 + hd + kb)
+    seqs, max_seq, n = 3, 17, 30
+    k, v = rnd(rng, rows, nkv, hd), rnd(rng, rows, nkv, hd, scale=40)
+    v[0] = 0                                                        # a vector without magnitude
+    if rows > 3:
+        k[1], v[1] = wide(rng, nkv, hd), wide(rng, nkv, hd)         # wraps as the reference's int64
+        v[2] = rng.integers(-(1 << 62), 1 << 62, (nkv, hd))
+        v[3] = rng.integers(-2, 3, (nkv, hd))
+    at = rng.permutation(seqs * max_seq)[:rows]
+    seq, slot = at // max_seq, at % max_seq
+    pos = rng.integers(0, n, rows)
+    cos, sin = rnd(rng, n, max(1, rot // 2)), rnd(rng, n, max(1, rot // 2))
+    if rows > 5:
+        slot[4], seq[5], pos[3] = -1, -1, -1                        # padding rows
+    w = nkv * hd
+    c, t = new_cache(seqs, max_seq, nkv, hd, kb, vb)
+    buf = np.zeros((rows, 2 * w + 1), np.int64)
+    buf[:, :w], buf[:, w:2 * w] = k.reshape(rows, w), v.reshape(rows, w)
+    d = dev(buf)
+    want = host_cache(t)
+    live = (slot >= 0) & (seq >= 0)
+    r = None
+    if rot:
+        r = iq.Rope(dev(cos), dev(sin), i32(pos), n, rot, layout)
+        live &= pos >= 0
+        k = ref.rotate(k, cos[pos], sin[pos], rot, layout)
+    iq.kv_write_dev(c, d, d[:, w:], i32(slot), rows, seq=i32(seq), rope=r, k_stride=2 * w + 1, v_stride=2 * w + 1)
+    write_ref(want, k[live], v[live], seq[live], slot[live], kb, vb)
+    got = host_cache(t)
+    for name in want:
+        assert (got[name] == want[name]).all(), name
+    # read back: written and padding rows, the same row twice
+    rs, rq = np.r_[slot, slot[:1], -1], np.r_[seq, seq[:1], 0]
+    ko, vo = full(rows + 2, nkv, hd), full(rows + 2, nkv, hd)
+    iq.kv_read_dev(ko, vo, c, i32(rs), rows + 2, seq=i32(rq))
+    for i in range(rows + 2):
+        for h in range(nkv):
+            if rs[i] < 0 or rq[i] < 0:
+                wk = wv = np.full(hd, KEEP)
+            elif kb:
+                a = (rq[i], rs[i], h)
+                wk = ref.unpack(want["kq"][a], want["k_mag"][a], kb)
+                wv = ref.unpack(want["vq"][a], want["v_mag"][a], vb)
+            else:
+                wk, wv = want["k"][rq[i], rs[i], h], want["v"][rq[i], rs[i], h]
+            assert (ko[i, h].cpu().numpy() == wk).all() and (vo[i, h].cpu().numpy() == wv).all()
+
+
+def test_kv_bad_rows_are_left_out_and_recorded():
+    c, t = new_cache(2, 8, 1, 4, 0, 0)
+    x = dev(np.arange(16).reshape(4, 4))
+    iq.kv_write_dev(c, x, x, i32([0, 8, 1, 2]), 4, seq=i32([0, 0, 2, -1]))
+    assert iq.device_status() == RANGE
+    k = t["k"].cpu().numpy()
+    assert (k[0, 0, 0] == [0, 1, 2, 3]).all() and (k.reshape(16, 4)[1:] == KEEP).all()
+    o = full(2, 1, 4)
+    iq.kv_read_dev(o, o.clone(), c, i32([0, 1 << 20]), 2)
+    assert iq.device_status() == RANGE
+    assert (o.cpu().numpy()[:, 0] == [[0, 1, 2, 3], [KEEP] * 4]).all()
+
+
+# --------------------------------------------------------------------- tree
+
+def chain(n):
+    return list(range(-1, n - 1))
+
+
+def bush(rng, n):
+    return [-1 if i == 0 or rng.random() < 0.2 else int(rng.integers(max(0, i - 5), i)) for i in range(n)]
+
+
+def run_tree(q, t, kvb, lens, starts, parents, nh, max_nodes=None, max_len=None, seqs=None, q_stride=None, rows=None,
+             stream=None):
+    kb, vb = kvb
+    shape = t["kq" if kb else "k"].shape
+    cache = iq.KVCache(shape[0], shape[1], shape[2], shape[3], k_bits=kb, v_bits=vb, **t)
+    rows = q.shape[0] if rows is None else rows
+    n = [b - a for a, b in zip(starts, starts[1:])]
+    max_nodes = max_nodes or max(n)
+    max_len = max_len or max(a + b for a, b in zip(lens, n))
+    size = dict(n_seq=len(lens), rows=rows, max_nodes=max_nodes, max_len=max_len)
+    need = iq.attn_tree_work(cache, nh, **size)
+    work = torch.empty((need + 7) // 8 + 1, dtype=torch.int64, device="cuda")
+    out = full(rows, nh * shape[3])
+    iq.attn_tree_dev(out, q, cache, nh, i32(lens), i32(starts), i32(parents), work=work,
+                     seqs=None if seqs is None else i32(seqs), q_stride=q_stride, **size)
+    return out.cpu().numpy()
+
+
+def check_tree(rng, nh, nkv, hd, lens, trees, kvb=(0, 0), q=None, k=None, v=None, pad=0, **kw):
+    """One random case against the reference; trees: parents per sequence."""
+    kb, vb = kvb
+    S, max_seq = len(lens), max(a + len(p) for a, p in zip(lens, trees)) + pad
+    starts = np.r_[0, np.cumsum([len(p) for p in trees])].tolist()
+    parents = [x for p in trees for x in p]
+    rows = starts[-1]
+    q = rnd(rng, rows, nh, hd, scale=1.5) if q is None else q
+    if kb:
+        t = dict(kq=dev(rng.integers(0, 1 << kb, (S, max_seq, nkv, hd)), torch.uint8),
+                 vq=dev(rng.integers(0, 1 << vb, (S, max_seq, nkv, hd)), torch.int16),
+                 k_mag=dev(rng.integers(0, 4 * ONE, (S, max_seq, nkv))),
+                 v_mag=dev(rng.integers(0, 4 * ONE, (S, max_seq, nkv))))
+        h = host_cache(t)
+        k = np.array([ref.unpack(c, m, kb) for c, m in zip(h["kq"].reshape(-1, hd), h["k_mag"].reshape(-1))])
+        v = np.array([ref.unpack(c, m, vb) for c, m in zip(h["vq"].reshape(-1, hd), h["v_mag"].reshape(-1))])
+        k, v = k.reshape(S, max_seq, nkv, hd), v.reshape(S, max_seq, nkv, hd)
+    else:
+        k = rnd(rng, S, max_seq, nkv, hd) if k is None else k
+        v = rnd(rng, S, max_seq, nkv, hd) if v is None else v
+        t = dict(k=dev(k), v=dev(v))
+    got = run_tree(dev(q.reshape(rows, -1)), t, kvb, lens, starts, parents, nh, **kw)
+    want = ref.tree(q, k, v, lens, starts, parents, nh)
+    assert (got == want.reshape(rows, -1)).all()
+
+
+GEOM = [(8, 2, 32), (4, 4, 128), (3, 1, 40), (7, 1, 64), (16, 1, 64), (1, 1, 1), (2, 1, 256), (6, 2, 17), (32, 4, 64),
+        (20, 1, 16), (5, 5, 96)]
+
+
+@pytest.mark.parametrize("kvb", [(0, 0), (8, 10)])
+@pytest.mark.parametrize("nh,nkv,hd", GEOM)
+def test_tree_geometries(nh, nkv, hd, kvb):
+    rng = np.random.default_rng(nh * 100 + hd)
+    check_tree(rng, nh, nkv, hd, [0, 37, 70], [bush(rng, 5), bush(rng, 1), bush(rng, 9)], kvb, pad=3)
+
+
+@pytest.mark.parametrize("ln", [0, 1, 2, 7, 15, 16, 17, 31, 63, 64, 65, 127, 255, 256, 257, 300])
+def test_tree_single_token_lengths(ln):
+    """A decode step: one node over a context of ln positions."""
+    rng = np.random.default_rng(ln)
+    check_tree(rng, 4, 2, 32, [ln, max(0, ln - 1)], [[-1], [-1]])
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 7, 8, 9, 15, 16, 17, 31, 33, 64, 65, 100])
+def test_tree_node_counts(n):
+    rng = np.random.default_rng(n)
+    check_tree(rng, 2, 1, 16, [11, 0], [bush(rng, n), chain(max(1, n // 2))])
+
+
+def test_tree_most_nodes():
+    rng = np.random.default_rng(9)
+    check_tree(rng, 1, 1, 8, [3], [bush(rng, 256)])
+    check_tree(rng, 1, 1, 8, [0], [chain(256)])
+
+
+@pytest.mark.parametrize("kvb", [(0, 0), (1, 1), (5, 16)])
+@pytest.mark.parametrize("ln", [900, 2050, 5000])
+def test_tree_long_contexts(ln, kvb):
+    rng = np.random.default_rng(ln)
+    check_tree(rng, 4, 2, 16, [ln, ln // 3], [bush(rng, 3), bush(rng, 12)], kvb)
+
+
+def test_tree_longest_context():
+    rng = np.random.default_rng(1)
+    check_tree(rng, 2, 1, 4, [32766], [[-1]])
+    check_tree(rng, 1, 1, 4, [32700], [bush(rng, 9)])
+
+
+def test_tree_flat_and_peaked_scores():
+    """All scores equal; one far above the rest (every other probability 0); scores a few units apart."""
+    rng = np.random.default_rng(2)
+    nh, nkv, hd, n, T = 4, 2, 32, 5, 130
+    for s in (0.0, 60.0, 0.2):
+        q = np.full((n, nh, hd), ref.q48(s), np.int64)
+        k = np.full((1, T, nkv, hd), ref.q48(0.01), np.int64)
+        k[0, 77] = ref.q48(1.0)
+        check_tree(rng, nh, nkv, hd, [T - n], [bush(rng, n)], q=q, k=k)
+
+
+@pytest.mark.parametrize("vs", [7.9, 8.1, 100.0, 20000.0])
+def test_tree_large_values(vs):
+    """Values around and beyond the range of the fast sum of products."""
+    rng = np.random.default_rng(3)
+    v = rnd(rng, 2, 150, 2, 32, scale=0.1)
+    v[0, ::7], v[0, 1::7], v[1, 100, 1, 3] = ref.q48(vs), ref.q48(-vs), ref.q48(vs)
+    check_tree(rng, 4, 2, 32, [140, 90], [bush(rng, 6), bush(rng, 8)], v=v, pad=4)
+
+
+def test_tree_whole_int64_range():
+    """Scores and values that wrap: the same integers as the reference, whatever they mean."""
+    rng = np.random.default_rng(4)
+    q, k, v = wide(rng, 7, 4, 32), wide(rng, 2, 60, 2, 32), wide(rng, 2, 60, 2, 32)
+    check_tree(rng, 4, 2, 32, [50, 0], [bush(rng, 4), bush(rng, 3)], q=q, k=k, v=v)
+    q = rng.integers(-(1 << 56), 1 << 56, (7, 4, 32))
+    k = rng.integers(-(1 << 56), 1 << 56, (2, 60, 2, 32))
+    check_tree(rng, 4, 2, 32, [50, 0], [bush(rng, 4), bush(rng, 3)], q=q, k=k, v=v)
+    q = rng.integers(-(1 << 55), 1 << 55, (7, 4, 32))
+    q[0, 0, 0], q[0, 0, 1], k[0, 0, 0, 0], k[0, 1, 0, 0] = -(1 << 55), (1 << 55) - 1, -(1 << 55), (1 << 55) - 1
+    check_tree(rng, 4, 2, 32, [50, 0], [bush(rng, 4), bush(rng, 3)], q=q, k=k >> 2, v=v >> 12)
+
+
+def test_tree_masked_slots_are_not_read_into_results():
+    """Extreme values in slots a node does not see change nothing for it."""
+    rng = np.random.default_rng(6)
+    nh, nkv, hd = 4, 2, 32
+    trees = [[-1, -1, 0, 1, 2, -1]]
+    q, k, v = rnd(rng, 6, nh, hd), rnd(rng, 1, 80, nkv, hd), rnd(rng, 1, 80, nkv, hd)
+    k[0, 41], v[0, 41] = ref.I64_MIN, ref.I64_MAX        # node 1: only nodes 1 and 3 see it
+    k[0, 46:], v[0, 46:] = ref.I64_MAX, ref.I64_MIN      # beyond the draft
+    check_tree(rng, nh, nkv, hd, [40], trees, q=q, k=k, v=v, max_len=60)
+
+
+def test_tree_rows_outside_and_bad_sequences():
+    """Rows behind the last sequence and of a sequence beyond its bounds stay; bad parents count as -1."""
+    rng = np.random.default_rng(7)
+    nh, nkv, hd, S, M = 4, 2, 16, 5, 40
+    k, v = rnd(rng, S, M, nkv, hd), rnd(rng, S, M, nkv, hd)
+    t = dict(k=dev(k), v=dev(v))
+    starts, parents = [1, 3, 3, 5, 8, 9], [-1] * 12
+    lens = [10, 5, 39, 20, -1]                            # the third: 39 + 2 > 40; the last: negative
+    parents[2], parents[6], parents[7] = 0, 5, 0          # node 1 of the fourth names a later node
+    q = rnd(rng, 12, nh, hd)
+    got = run_tree(dev(q.reshape(12, -1)), t, (0, 0), lens, starts, parents, nh, max_nodes=3, max_len=M)
+    assert iq.device_status() == RANGE
+    want = np.full((12, nh, hd), KEEP, np.int64)
+    good = ref.tree(q[:8], [k[0], k[1], k[2][:0], k[3]], [v[0], v[1], v[2][:0], v[3]], [10, 5, 0, 20], [1, 3, 3, 3, 3], parents, nh)
+    want[1:3] = good[1:3]
+    want[5:8] = ref.tree(q[5:8], [k[3]], [v[3]], [20], [0, 3], parents[5:8], nh)
+    assert (got == want.reshape(12, -1)).all()
+    # starts beyond the rows, falling starts, an unknown cache sequence, a padding sequence (-1)
+    for st, sq, want_status in (([0, 13], [0], RANGE), ([2, 1], [0], RANGE), ([0, 1], [5], RANGE), ([0, 1], [-1], 0),
+                                ([-1, 1], [0], RANGE), ([0, 4], [0], RANGE)):
+        got = run_tree(dev(q.reshape(12, -1)), t, (0, 0), [3], st, parents, nh, max_nodes=3, max_len=M, seqs=sq)
+        assert (got == KEEP).all() and iq.device_status() == want_status
+
+
+def test_tree_shared_cache_sequence_and_strided_queries():
+    """Two drafts over the same cache sequence (read only), query rows inside a wider buffer."""
+    rng = np.random.default_rng(8)
+    nh, nkv, hd = 8, 2, 32
+    k, v = rnd(rng, 3, 90, nkv, hd), rnd(rng, 3, 90, nkv, hd)
+    trees = [bush(rng, 4), bush(rng, 6)]
+    starts = [0, 4, 10]
+    q = rnd(rng, 10, nh * hd + 5)
+    got = run_tree(dev(q), dict(k=dev(k), v=dev(v)), (0, 0), [80, 33], starts, trees[0] + trees[1], nh, seqs=[2, 2],
+                   q_stride=nh * hd + 5)
+    want = ref.tree(q[:, : nh * hd].reshape(10, nh, hd).copy(), [k[2], k[2]], [v[2], v[2]], [80, 33], starts,
+                    trees[0] + trees[1], nh)
+    assert (got == want.reshape(10, -1)).all()
+
+
+def test_tree_chain_equals_one_by_one():
+    """A chain of nodes = the same tokens as single-node calls over the growing context."""
+    rng = np.random.default_rng(10)
+    nh, nkv, hd, ln, n = 8, 2, 64, 333, 19
+    t = dict(k=dev(rnd(rng, 1, 400, nkv, hd)), v=dev(rnd(rng, 1, 400, nkv, hd)))
+    q = dev(rnd(rng, n, nh * hd))
+    whole = run_tree(q, t, (0, 0), [ln], [0, n], chain(n), nh)
+    for i in range(n):
+        one = run_tree(q[i:i + 1], t, (0, 0), [ln + i], [0, 1], [-1], nh)
+        assert (one[0] == whole[i]).all()
+
+
+def test_tree_many_rows_batch():
+    """More work than one wave of blocks, checked on a sample of rows."""
+    rng = np.random.default_rng(11)
+    S, nh, nkv, hd, M = 40, 8, 2, 64, 700
+    lens = [int(x) for x in rng.integers(0, 600, S)]
+    trees = [bush(rng, int(x)) for x in rng.integers(1, 64, S)]
+    starts = np.r_[0, np.cumsum([len(p) for p in trees])].tolist()
+    parents = [x for p in trees for x in p]
+    k, v, q = rnd(rng, S, M, nkv, hd), rnd(rng, S, M, nkv, hd), rnd(rng, starts[-1], nh, hd)
+    got = run_tree(dev(q.reshape(starts[-1], -1)), dict(k=dev(k), v=dev(v)), (0, 0), lens, starts, parents, nh)
+    scale = ref.fp(ref.INV_SQRT, hd << 48)
+    for b in range(0, S, 3):
+        paths = ref.ancestors(trees[b])
+        for i in {0, len(trees[b]) - 1}:
+            see = np.r_[np.arange(lens[b]), lens[b] + np.array(paths[i])].astype(int)
+            for h in (0, 5):
+                want = ref.attend(q[starts[b] + i, h], k[b, see, h // 4], v[b, see, h // 4], scale)
+                assert (got[starts[b] + i, h * hd:(h + 1) * hd] == want).all()
+
+
+# ------------------------------------------------------------------- scores
+
+def check_logprobs(l, tokens, top, ld=None):
+    rows, V = l.shape
+    ld = ld or V
+    buf = np.full((rows, ld), ref.I64_MAX, np.int64)
+    buf[:, :V] = l
+    logp, ent = full(rows), full(rows)
+    ids, tl = torch.full((rows, top), -5, dtype=torch.int32, device="cuda"), full(rows, top)
+    iq.logprobs_dev(dev(buf), rows, V, tokens=None if tokens is None else i32(tokens),
+                    logp=None if tokens is None else logp, entropy=ent, top=top, top_ids=ids if top else None,
+                    top_logp=tl if top else None, ld=ld)
+    for r in range(rows):
+        bad = tokens is None or not 0 <= tokens[r] < V
+        lp, h, best, bl = ref.logprobs(l[r], None if bad else tokens[r], top)
+        assert int(logp[r]) == (KEEP if bad else lp)
+        assert int(ent[r]) == h
+        assert ids[r].tolist() == best and tl[r].tolist() == bl
+
+
+@pytest.mark.parametrize("V,top", [(1, 0), (1, 1), (2, 2), (31, 31), (32, 32), (33, 5), (255, 8), (1000, 1),
+                                   (4097, 32), (32000, 5), (32003, 20), (65537, 3), (131072, 32), (300001, 7)])
+def test_logprobs_sizes(V, top):
+    rng = np.random.default_rng(V + top)
+    l = rnd(rng, 3, V, scale=2.5)
+    check_logprobs(l, rng.integers(0, V, 3), top, ld=V + (V % 3))
+
+
+def test_logprobs_many_rows():
+    rng = np.random.default_rng(12)
+    check_logprobs(rnd(rng, 333, 700, scale=4), rng.integers(-1, 700, 333), 6)
+    check_logprobs(rnd(rng, 20, 9000, scale=4), None, 3)
+
+
+def test_logprobs_ties_masks_and_extremes():
+    rng = np.random.default_rng(13)
+    V = 5000
+    l = rnd(rng, 12, V)
+    l[0] = 0                                               # all equal
+    l[1] = ref.I64_MIN                                     # all at the lowest value
+    l[2] = ref.I64_MIN
+    l[2, 17] = ref.I64_MAX                                 # the widest spread: d passes int64
+    l[3, ::2] = ref.I64_MIN                                # half masked
+    l[4] = rng.integers(0, 3, V) * ONE                     # many ties
+    l[5] = np.sort(l[5])
+    l[6] = np.sort(l[6])[::-1]
+    l[7, :] = -34 * ONE
+    l[7, 4999] = 0                                         # all others exactly at the cut-off
+    l[8, :] = -34 * ONE + 1
+    l[8, 0] = 0
+    l[9] = wide(rng, V)
+    l[10] = ref.I64_MAX
+    l[11, 100:150] = l[11].max() + 1                       # more equal maxima than alternatives
+    tokens = [3, 4, 18, 0, 9, 4999, 4999, 0, 4999, 5, 77, 120]
+    for top in (0, 1, 8, 32):
+        check_logprobs(l, tokens, top)
+
+
+def test_logprobs_close_to_real_logarithms():
+    """Against a 64-bit float log-softmax: E is within 2^-44 relative plus 2^-48 a
+    logit, ln within 2^-46, and the 64-bit reference within 1e-13 or so of itself."""
+    rng = np.random.default_rng(14)
+    l = rnd(rng, 4, 32000, scale=6)
+    logp, ent = full(4), full(4)
+    tok = i32([1, 2, 3, 4])
+    iq.logprobs_dev(dev(l), 4, 32000, tokens=tok, logp=logp, entropy=ent)
+    x = torch.log_softmax(dev(l).double() / ONE, -1)
+    tol = 2.0 ** -44 + 32000 * 2.0 ** -48 + 2.0 ** -46 + 1e-12
+    assert (logp.double() / ONE - x.gather(1, tok.long()[:, None])[:, 0]).abs().max().item() < tol
+    # entropy: the same error on ln S, and d <= 34 times it on each probability
+    assert (ent.double() / ONE + (x.exp() * x).sum(-1)).abs().max().item() < 40 * tol
+
+
+# ------------------------------------------------ streams, graphs, together
+
+def test_other_stream_and_two_at_once():
+    rng = np.random.default_rng(15)
+    nh, nkv, hd, n = 8, 2, 32, 12
+    q = [dev(rnd(rng, n, nh * hd)) for _ in range(2)]
+    t = dict(k=dev(rnd(rng, 1, 300, nkv, hd)), v=dev(rnd(rng, 1, 300, nkv, hd)))
+    l = [dev(rnd(rng, 40, 6000, scale=3)) for _ in range(2)]
+    cache = iq.KVCache(1, 300, nkv, hd, **t)
+    size = dict(n_seq=1, rows=n, max_nodes=n, max_len=300)
+    ln, st, par = i32([250]), i32([0, n]), i32(chain(n))
+    need = iq.attn_tree_work(cache, nh, **size) // 8 + 1
+
+    def calls(i, stream, out, lp, work):
+        iq.attn_tree_dev(out, q[i], cache, nh, ln, st, par, work=work, stream=stream, **size)
+        iq.logprobs_dev(l[i], 40, 6000, entropy=lp, stream=stream)
+
+    outs = [(full(n, nh * hd), full(40), torch.empty(need, dtype=torch.int64, device="cuda")) for _ in range(4)]
+    for i in range(2):
+        calls(i, None, *outs[i])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for i in range(2):
+            calls(i, streams[i], *outs[2 + i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(outs[i][0], outs[2 + i][0]) and torch.equal(outs[i][1], outs[2 + i][1])
+
+
+def test_captured_and_replayed():
+    """All calls in one CUDA graph, replayed on changed inputs; two graphs with their own workspaces at once."""
+    rng = np.random.default_rng(16)
+    nh, nkv, hd, n, M, npos = 8, 2, 32, 6, 128, 200
+    cos, sin = full(npos, hd // 2), full(npos, hd // 2)
+    iq.rope_tables_dev(cos, sin, hd, npos, 10000)
+    w = (nh + 2 * nkv) * hd
+
+    def make():
+        s = dict(qkv=dev(rnd(rng, n, w)), q=full(n, nh * hd), out=full(n, nh * hd), pos=i32(range(50, 50 + n)),
+                 slot=i32(range(50, 50 + n)), par=i32(chain(n)), ln=i32([50]), st=i32([0, n]),
+                 k=dev(rnd(rng, 1, M, nkv, hd)), v=dev(rnd(rng, 1, M, nkv, hd)), logp=full(n), tok=i32([3] * n))
+        s["cache"] = iq.KVCache(1, M, nkv, hd, k=s["k"], v=s["v"])
+        s["size"] = dict(n_seq=1, rows=n, max_nodes=n, max_len=M)
+        s["work"] = torch.empty(iq.attn_tree_work(s["cache"], nh, **s["size"]) // 8 + 1, dtype=torch.int64, device="cuda")
+        return s
+
+    def calls(s):
+        rope = iq.Rope(cos, sin, s["pos"], npos, hd)
+        iq.rope_dev(s["q"], s["qkv"], rope, n, nh, hd, x_stride=w)
+        iq.kv_write_dev(s["cache"], s["qkv"][:, nh * hd:], s["qkv"][:, (nh + nkv) * hd:], s["slot"], n, rope=rope,
+                        k_stride=w, v_stride=w)
+        iq.attn_tree_dev(s["out"], s["q"], s["cache"], nh, s["ln"], s["st"], s["par"], work=s["work"], **s["size"])
+        iq.logprobs_dev(s["out"], n, nh * hd, tokens=s["tok"], logp=s["logp"])
+
+    states = [make(), make()]
+    for s in states:
+        calls(s)
+    torch.cuda.synchronize()
+    graphs = []
+    for s in states:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            calls(s)
+        graphs.append(g)
+    for s in states:
+        s["qkv"].copy_(dev(rnd(rng, n, w)))
+    torch.cuda.synchronize()
+    side = [torch.cuda.Stream() for _ in states]
+    for g, st in zip(graphs, side):
+        with torch.cuda.stream(st):
+            for _ in range(3):
+                g.replay()
+    torch.cuda.synchronize()
+    got = [(s["out"].clone(), s["logp"].clone(), s["k"].clone()) for s in states]
+    for s, (o, lp, k) in zip(states, got):
+        calls(s)
+        torch.cuda.synchronize()
+        assert torch.equal(s["out"], o) and torch.equal(s["logp"], lp) and torch.equal(s["k"], k)
+
+
+def _forward(c, w, toks, pos, slot, parents, ln, kvs, tables, kvb):
+    """llama_forward's layers on drafted rows with the library's operators; logits on the device."""
+    n, d, hd, nh, nkv = len(toks), c["dim"], c["head_dim"], c["n_heads"], c["n_kv_heads"]
+    kvd, ml = nkv * hd, c["max_seq"]
+    x = dev(w["embed"][toks])
+    nrm, qkv, q, att = full(n, d), full(n, d + 2 * kvd), full(n, d), full(n, d)
+    rope = iq.Rope(tables[0], tables[1], i32(pos), ml, hd)
+    size = dict(n_seq=1, rows=n, max_nodes=n, max_len=ml)
+    for l, lay in enumerate(w["layers"]):
+        n1, wq, wk, wv, wo, n2, wg, wu, wd = [dev(a) for a in lay]
+        iq.rmsnorm_dev(nrm, x, n1, n, d)
+        wqkv = torch.cat([wq, wk, wv])
+        iq.gemm_dev(qkv, wqkv, nrm, n, d + 2 * kvd, d)
+        iq.rope_dev(q, qkv, rope, n, nh, hd, x_stride=d + 2 * kvd)
+        cache = kvs[l]
+        iq.kv_write_dev(cache, qkv[:, d:], qkv[:, d + kvd:], i32(slot), n, rope=rope, k_stride=d + 2 * kvd,
+                        v_stride=d + 2 * kvd)
+        work = torch.empty(iq.attn_tree_work(cache, nh, **size) // 8 + 1, dtype=torch.int64, device="cuda")
+        iq.attn_tree_dev(att, q, cache, nh, i32([ln]), i32([0, n]), i32(parents), work=work, **size)
+        o = full(n, d)
+        iq.gemm_dev(o, wo, att, n, d, d)
+        x = x + o
+        iq.rmsnorm_dev(nrm, x, n2, n, d)
+        it = c["inter"]
+        g, u, a = full(n, it), full(n, it), full(n, it)
+        iq.gemm_dev(g, wg, nrm, n, it, d)
+        iq.gemm_dev(u, wu, nrm, n, it, d)
+        iq.fp_dev("silu", g, None, a, n * it)
+        iq.fp_dev("mul", a, u, g, n * it)
+        iq.gemm_dev(o, wd, g, n, d, it)
+        x = x + o
+    iq.rmsnorm_dev(nrm, x, dev(w["final_norm"]), n, d)
+    logits = full(n, c["vocab"])
+    iq.gemm_dev(logits, dev(w["lm_head"]), nrm, n, c["vocab"], d)
+    return logits
+
+
+@pytest.mark.parametrize("kvb", [(0, 0), (8, 10)])
+def test_verifying_a_draft_equals_the_model(kvb):
+    """Rotate, write the cache, attend, score: every node's logits equal the model's own
+    forward along the node's path, and its log probabilities the reference's on those logits."""
+    c = configs.TINY_TEST
+    w = model_weights(7, c)
+    rng = np.random.default_rng(17)
+    prompt = [int(x) for x in rng.integers(3, c["vocab"], 9)]
+    draft = [int(x) for x in rng.integers(3, c["vocab"], 7)]
+    parents = [-1, 0, 0, 1, 2, -1, 5]
+    depth = [len(p) - 1 for p in ref.ancestors(parents)]
+    tabs = (full(c["max_seq"], c["head_dim"] // 2), full(c["max_seq"], c["head_dim"] // 2))
+    iq.rope_tables_dev(*tabs, c["head_dim"], c["max_seq"], c["rope_theta"])
+    kvs = [new_cache(1, c["max_seq"], c["n_kv_heads"], c["head_dim"], *kvb)[0] for _ in range(c["n_layers"])]
+    n, P = len(draft), len(prompt)
+    first = _forward(c, w, prompt, range(P), range(P), chain(P), 0, kvs, tabs, kvb)
+    logits = _forward(c, w, draft, [P + x for x in depth], range(P, P + n), parents, P, kvs, tabs, kvb)
+    m = iq.Model(c)
+    m.load(w)
+    if kvb[0]:
+        m.set_kv_packed(*kvb)
+    for i, t in enumerate(prompt):
+        lg = m.forward(t, i)[1]
+        assert (first[i].cpu().numpy() == lg).all()
+    for i, path in enumerate(ref.ancestors(parents)):
+        for j, node in enumerate(path):
+            lg = m.forward(draft[node], P + j)[1]
+        assert (logits[i].cpu().numpy() == lg).all()
+    m.close()
+    tok = [int(x) for x in rng.integers(0, c["vocab"], n)]
+    logp, ids, tl = full(n), torch.zeros(n, 4, dtype=torch.int32, device="cuda"), full(n, 4)
+    iq.logprobs_dev(logits, n, c["vocab"], tokens=i32(tok), logp=logp, top=4, top_ids=ids, top_logp=tl)
+    for i in range(n):
+        lp, _, best, bl = ref.logprobs(logits[i].tolist(), tok[i], 4)
+        assert (int(logp[i]), ids[i].tolist(), tl[i].tolist()) == (lp, best, bl)

@@ -1,0 +1,194 @@
+"""CPU tests of the operators around drafted tokens: their refusals (checked
+before any device work) and the whole-number identities the kernels rest on."""
+import ctypes
+import math
+import random
+from fractions import Fraction
+
+import numpy as np
+import pytest
+
+import iq
+import ops_ref as ref
+import oracle as orc
+from helpers import ONE
+
+ARG, RANGE = -1, -6
+P = 1 << 20          # a non-null address that is never read: every call below is refused
+
+
+def status(name, *args):
+    return getattr(iq.lib(), name)(*args)
+
+
+def rope(**kw):
+    r = iq.Rope.__new__(iq.Rope)
+    ctypes.Structure.__init__(r)
+    for k, v in dict(dict(d_cos=P, d_sin=P, d_pos=P, n_pos=8, rot_dim=16, layout=0), **kw).items():
+        setattr(r, k, v)
+    return ctypes.byref(r)
+
+
+def cache(**kw):
+    c = iq.KVCache.__new__(iq.KVCache)
+    ctypes.Structure.__init__(c)
+    d = dict(seqs=2, max_seq=64, kv_heads=2, head_dim=16, k_bits=0, v_bits=0, k=P, v=P, kq=P, vq=P, k_mag=P, v_mag=P)
+    for k, v in dict(d, **kw).items():
+        setattr(c, k, v)
+    return ctypes.byref(c)
+
+
+def scaling(**kw):
+    return ctypes.byref(iq._RopeScaling(**dict(dict(kind=1, orig_len=64, factor=2 * ONE, low=0, high=ONE), **kw)))
+
+
+@pytest.mark.parametrize("bad,want", [
+    (dict(cos=None), ARG), (dict(sin=P + 4), ARG), (dict(rot=0), ARG), (dict(rot=7), ARG), (dict(rot=258), ARG),
+    (dict(n_pos=0), ARG), (dict(n_pos=(1 << 24) + 1), ARG), (dict(theta=0), ARG),
+    (dict(sc=dict(kind=4)), ARG), (dict(sc=dict(factor=ONE - 1)), ARG), (dict(sc=dict(factor=1025 * ONE)), ARG),
+    (dict(sc=dict(kind=2), rot=2), ARG), (dict(sc=dict(kind=3, orig_len=0)), ARG),
+    (dict(sc=dict(kind=3, low=ONE)), ARG), (dict(sc=dict(mscale=-1)), ARG),
+    (dict(theta=(1 << 31) - 1), RANGE), (dict(theta=400000000, sc=dict(kind=2, factor=1000 * ONE)), RANGE)])
+def test_rope_tables_refusals(bad, want):
+    a = dict(dict(cos=P, sin=P, rot=16, n_pos=8, theta=10000, sc=None), **bad)
+    sc = scaling(**a["sc"]) if a["sc"] is not None else None
+    assert status("iq_rope_tables_dev", a["cos"], a["sin"], a["rot"], a["n_pos"], a["theta"], sc, None) == want
+
+
+@pytest.mark.parametrize("bad", [
+    dict(out=None), dict(x=None), dict(out=P + 4), dict(rows=-1), dict(heads=0), dict(hd=0), dict(hd=257),
+    dict(xs=31), dict(os=31), dict(x=P, out=P, os=40), dict(r=dict(rot_dim=18)), dict(r=dict(rot_dim=3)),
+    dict(r=dict(rot_dim=0)), dict(r=dict(layout=2)), dict(r=dict(d_pos=None)), dict(r=dict(d_cos=P + 2)),
+    dict(r=dict(n_pos=0)), dict(r=None)])
+def test_rope_refusals(bad):
+    a = dict(dict(out=2 * P, x=P, rows=2, heads=2, hd=16, xs=32, os=32, r={}), **bad)
+    r = rope(**a["r"]) if a["r"] is not None else None
+    assert status("iq_rope_dev", a["out"], a["x"], r, a["rows"], a["heads"], a["hd"], a["xs"], a["os"], None) == ARG
+
+
+BAD_CACHE = [dict(seqs=0), dict(max_seq=0), dict(kv_heads=0), dict(head_dim=0), dict(head_dim=257), dict(k=None),
+             dict(v=P + 4), dict(k_bits=8), dict(v_bits=3), dict(k_bits=9, v_bits=8), dict(k_bits=8, v_bits=17),
+             dict(k_bits=8, v_bits=8, kq=None), dict(k_bits=8, v_bits=8, vq=P + 1),
+             dict(k_bits=8, v_bits=8, v_mag=P + 4)]
+
+
+@pytest.mark.parametrize("bad", BAD_CACHE)
+def test_cache_refusals(bad):
+    c = cache(**bad)
+    assert status("iq_kv_write_dev", c, P, P, None, P, 1, 32, 32, None, None) == ARG
+    assert status("iq_kv_read_dev", P, P, c, None, P, 1, None) == ARG
+    n = ctypes.c_int64()
+    assert status("iq_attn_tree_work", c, 4, 1, 1, 1, 1, ctypes.byref(n)) == ARG
+    assert status("iq_attn_tree_dev", P, 2 * P, c, 4, None, P, P, P, 1, 1, 1, 1, 64, P, 1 << 30, None) == ARG
+
+
+def test_kv_row_refusals():
+    c = cache()
+    assert status("iq_kv_write_dev", c, None, P, None, P, 1, 32, 32, None, None) == ARG
+    assert status("iq_kv_write_dev", c, P, P, None, None, 1, 32, 32, None, None) == ARG
+    assert status("iq_kv_write_dev", c, P, P, None, P, -1, 32, 32, None, None) == ARG
+    assert status("iq_kv_write_dev", c, P, P, None, P, 1, 31, 32, None, None) == ARG
+    assert status("iq_kv_write_dev", c, P, P, None, P, 1, 32, 31, None, None) == ARG
+    assert status("iq_kv_write_dev", c, P, P, P + 2, P, 1, 32, 32, None, None) == ARG
+    assert status("iq_kv_write_dev", c, P, P, None, P, 1, 32, 32, rope(rot_dim=18), None) == ARG
+    assert status("iq_kv_write_dev", c, P, P, None, P, 0, 32, 32, None, None) == 0     # no rows: nothing to do
+    assert status("iq_kv_read_dev", None, P, c, None, P, 1, None) == ARG
+    assert status("iq_kv_read_dev", P, P, c, None, P + 1, 1, None) == ARG
+    assert status("iq_kv_read_dev", P, P, c, None, P, 0, None) == 0
+
+
+@pytest.mark.parametrize("bad,want", [
+    (dict(out=None), ARG), (dict(q=None), ARG), (dict(out=P, q=P), ARG), (dict(lens=None), ARG),
+    (dict(starts=None), ARG), (dict(parents=P + 2), ARG), (dict(nh=3), ARG), (dict(nh=0), ARG), (dict(n_seq=0), ARG),
+    (dict(rows=0), ARG), (dict(nodes=0), ARG), (dict(ml=0), ARG), (dict(qs=63), ARG), (dict(work=P + 4), ARG),
+    (dict(wb=-1), ARG), (dict(nodes=257), RANGE), (dict(ml=65), RANGE)])
+def test_tree_refusals(bad, want):
+    a = dict(dict(out=P, q=2 * P, nh=4, seqs=None, lens=P, starts=P, parents=P, n_seq=1, rows=2, nodes=2, ml=64,
+                  qs=64, work=P, wb=1 << 30), **bad)
+    assert status("iq_attn_tree_dev", a["out"], a["q"], cache(), a["nh"], a["seqs"], a["lens"], a["starts"],
+                  a["parents"], a["n_seq"], a["rows"], a["nodes"], a["ml"], a["qs"], a["work"], a["wb"], None) == want
+
+
+def test_tree_context_limit():
+    """Beyond 32767 positions the int64 softmax sum could wrap: refused."""
+    n = ctypes.c_int64()
+    c = cache(max_seq=40000)
+    assert status("iq_attn_tree_work", c, 4, 1, 1, 1, 32767, ctypes.byref(n)) == 0
+    assert status("iq_attn_tree_work", c, 4, 1, 1, 1, 32768, ctypes.byref(n)) == RANGE
+
+
+@pytest.mark.parametrize("bad,want", [
+    (dict(lg=None), ARG), (dict(lg=P + 4), ARG), (dict(ld=99), ARG), (dict(rows=-1), ARG), (dict(V=0), ARG),
+    (dict(tok=None), ARG), (dict(lp=None), ARG), (dict(top=-1), ARG), (dict(top=3, ids=None), ARG),
+    (dict(top=3, tl=None), ARG), (dict(V=20, top=21), ARG), (dict(top=33), RANGE),
+    (dict(V=(1 << 20) + 1, ld=1 << 21), RANGE), (dict(rows=0), 0)])
+def test_logprobs_refusals(bad, want):
+    a = dict(dict(lg=P, ld=100, rows=1, V=100, tok=P, lp=P, ent=P, top=1, ids=P, tl=P), **bad)
+    assert status("iq_logprobs_dev", a["lg"], a["ld"], a["rows"], a["V"], a["tok"], a["lp"], a["ent"], a["top"],
+                  a["ids"], a["tl"], None) == want
+
+
+def test_binding_refuses_host_and_wrong_types():
+    import torch
+    x = torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(ValueError):
+        iq.Rope(x, x, x.int(), 4, 2)
+    with pytest.raises(ValueError):
+        iq.logprobs_dev(x.int(), 1, 4)
+
+
+# ------------------------------------------------------------- identities
+
+def test_reference_tables_equal_rope_init():
+    """The references of the scaled tables reduce to rope_init where nothing is scaled."""
+    for rot, theta in ((32, 10000), (64, 10000), (128, 500)):
+        n = 40
+        c, s = np.empty((n, rot // 2), np.int64), np.empty((n, rot // 2), np.int64)
+        orc.O.iqo_rope_tables(rot, n, theta, orc.p(c), orc.p(s))
+        rc, rs = ref.tables(rot, range(n), theta)
+        assert (c == rc).all() and (s == rs).all()
+
+
+def test_angle_reduction_from_a_double_quotient():
+    """p th mod 2 pi with the quotient from doubles: off by at most one, wrapped remainder exact."""
+    w = 2 * ref.pi()
+    rng = random.Random(1)
+    for _ in range(20000):
+        p = rng.choice([rng.randrange(1 << 24), (1 << 24) - 1 - rng.randrange(9)])
+        th = rng.choice([rng.randrange(1, ONE + 1), ONE, w // rng.randrange(7, 99)])
+        q = int(float(p) * float(th) / float(w))
+        r = ref.wrap(p * th - q * w)
+        r = r + w if r < 0 else r - w if r >= w else r
+        assert r == p * th % w
+
+
+def test_code_and_value_of_a_cache_vector():
+    """kv_code's estimate and remainder, and kv_value's 32-bit halves."""
+    rng = random.Random(2)
+    for _ in range(20000):
+        M = rng.choice([rng.randrange(1, 1 << 61), rng.randrange(1, 1 << 20), (1 << 61) - 1, 1])
+        x = rng.choice([rng.randint(-M, M), M, -M, 0, M - 1])
+        b = rng.randint(1, 16)
+        u, D = x + M, 2 * M
+        q = int(float(u) * (float(1 << b) / float(D)))
+        r = ref.wrap((u << b) - q * D)
+        q = q - 1 if r < 0 else q + 1 if r >= D else q
+        assert q == (u << b) // D
+        code = min(q, (1 << b) - 1)
+        c = 2 * code + 1
+        lo, hi = c * (M & 0xffffffff), c * (M >> 32)
+        assert ref.wrap((hi << (32 - b)) + (lo >> b) - M) == ((2 * code + 1) * M >> b) - M
+
+
+def test_exp_down_and_ln_accuracy():
+    """E(d) within 2^-44 relative plus one unit of 2^-48 of e^-d; ln within 2^-46."""
+    rng = random.Random(3)
+    for _ in range(3000):
+        d = rng.choice([rng.randrange(34 * ONE), rng.randrange(ONE), rng.randrange(1 << 30), 34 * ONE - 1])
+        e, want = ref.exp_down(d), math.exp(-d / ONE) * ONE
+        assert want * (1 - 2.0 ** -44) - 1 <= e <= want * (1 + 2.0 ** -44)
+    assert ref.exp_down(0) == ONE and ref.exp_down(34 * ONE) == 0
+    for _ in range(500):
+        s = rng.randrange(ONE, 1 << rng.randint(49, 68))
+        assert abs(ref.ln_sum(s) / ONE - math.log(s / ONE)) < 2.0 ** -46
+    assert ref.ln_sum(ONE) == 0
