@@ -1,5 +1,6 @@
 // iq_ops.cu -- C ABI of the operators around drafted tokens: rotary tables and
 // rotation, cache rows, tree attention, log probabilities (declared in iq.h).
+#include <atomic>
 #include <climits>
 #include "iq_common.cuh"
 #include "iq_ops.cuh"
@@ -73,6 +74,81 @@ static int cache_check(const iq_kv_cache *c, KVArgs *a) {
     *a = KVArgs{c->k, c->v, c->kq, c->vq, c->k_mag, c->v_mag, c->seqs, c->max_seq, c->kv_heads, c->head_dim,
                 c->k_bits, c->v_bits};
     return IQ_OK;
+}
+
+static int tree_check(const iq_kv_cache *cache, int nh, int n_seq, int rows, int max_nodes, int max_len, KVArgs *c) {
+    int rc;
+    if ((rc = cache_check(cache, c))) return rc;
+    if (nh < 1 || nh > 4096 || nh % c->nkv || n_seq < 1 || n_seq > 65536 || rows < 1 || max_nodes < 1 || max_len < 1) return IQ_ERR_ARG;
+    if (max_nodes > TREE_MAX_NODES || max_len > c->max_seq || max_len > 32767)
+        return IQ_ERR_RANGE;
+    return IQ_OK;
+}
+
+// How a call is cut: columns a cluster (8 NT), CTAs a cluster (they split the
+// positions), score rows in shared memory or in the workspace. Two CTAs an SM
+// (100 KB each beside the static part) as long as 8 columns fit that way, then one.
+struct TreePlan {
+    int nt, cs, blocks, Ts;
+    bool sm;
+    size_t smem;
+    int64_t ctas;
+};
+static TreePlan tree_plan(const KVArgs &c, int nh, int n_seq, int rows, int max_nodes, int max_len) {
+    const int grp = nh / c.nkv, nd = tree_hdp(c.hd) / 64;
+    const int64_t cols = (int64_t)std::min(max_nodes, rows) * grp;
+    TreePlan p = {};
+    auto row = [&](int cs) { return ((max_len + cs - 1) / cs + 15) / 16 * 16 + 2; };
+    auto fits = [&](int nt, int cs, size_t most) {
+        return (size_t)8 * nt * row(cs) * 8 + tree_side(nt, c.hd) <= most;
+    };
+    const size_t two = 100 * 1024, one = 200 * 1024;
+    p.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : nd <= 2 ? 4 : 2;
+    while (p.nt > 1 && !fits(p.nt, 8, two)) p.nt /= 2;
+    p.sm = fits(p.nt, 8, one);
+    const size_t most = fits(p.nt, 8, two) ? two : one;
+    // enough CTAs for two an SM, none with fewer than 64 positions
+    const int64_t clusters = c.nkv * std::max<int64_t>(n_seq, ((int64_t)rows * grp + 8 * p.nt - 1) / (8 * p.nt));
+    for (p.cs = 1; p.cs < 8; p.cs *= 2) {
+        if (p.sm && !fits(p.nt, p.cs, most)) continue;
+        if (!p.sm || (clusters * p.cs < 2 * dev_info().sms && max_len / p.cs > 64)) continue;
+        break;
+    }
+    p.blocks = (int)((cols + 8 * p.nt - 1) / (8 * p.nt));
+    p.Ts = row(p.cs);
+    p.smem = (p.sm ? (size_t)8 * p.nt * p.Ts * 8 : 0) + tree_side(p.nt, c.hd);
+    p.ctas = (int64_t)n_seq * c.nkv * p.blocks * p.cs;
+    return p;
+}
+
+template <int NT, bool PK, bool SM>
+static int launch_tree(const TreeArgs &a, const TreePlan &p, cudaStream_t s) {
+    static std::atomic<uint64_t> set{0};   // devices whose shared-memory limit is raised
+    int dev = 0;
+    IQ_CUDA(cudaGetDevice(&dev));
+    if (!(set.load() >> dev & 1)) {
+        IQ_CUDA(cudaFuncSetAttribute(k_tree<NT, PK, SM>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+        set.fetch_or(1ull << dev);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)p.cs;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)p.ctas);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = p.smem;
+    cfg.stream = s;
+    cfg.attrs = at;
+    cfg.numAttrs = p.cs > 1 ? 1 : 0;
+    IQ_CUDA(cudaLaunchKernelEx(&cfg, k_tree<NT, PK, SM>, a));
+    return IQ_OK;
+}
+template <bool PK>
+static int launch_tree_nt(const TreeArgs &a, const TreePlan &p, cudaStream_t s) {
+    if (!p.sm) return launch_tree<1, PK, false>(a, p, s);
+    return p.nt == 1 ? launch_tree<1, PK, true>(a, p, s) : p.nt == 2 ? launch_tree<2, PK, true>(a, p, s)
+                                                                  : launch_tree<4, PK, true>(a, p, s);
 }
 
 extern "C" {
@@ -172,22 +248,14 @@ IQ_API int iq_kv_read_dev(int64_t *d_k, int64_t *d_v, const iq_kv_cache *cache, 
     return IQ_OK;
 }
 
-static int tree_check(const iq_kv_cache *cache, int nh, int n_seq, int rows, int max_nodes, int max_len, KVArgs *c) {
-    int rc;
-    if ((rc = cache_check(cache, c))) return rc;
-    if (nh < 1 || nh > 4096 || nh % c->nkv || n_seq < 1 || n_seq > 65536 || rows < 1 || max_nodes < 1 || max_len < 1) return IQ_ERR_ARG;
-    if (max_nodes > TREE_MAX_NODES || max_len > c->max_seq || max_len > 32767)
-        return IQ_ERR_RANGE;
-    return IQ_OK;
-}
-
 IQ_API int iq_attn_tree_work(const iq_kv_cache *cache, int num_heads, int n_seq, int rows, int max_nodes, int max_len,
                              int64_t *bytes) {
     KVArgs c;
     int rc;
     if (!bytes) return IQ_ERR_ARG;
     if ((rc = tree_check(cache, num_heads, n_seq, rows, max_nodes, max_len, &c))) return rc;
-    *bytes = (int64_t)rows * num_heads * max_len * 8;
+    const TreePlan p = tree_plan(c, num_heads, n_seq, rows, max_nodes, max_len);
+    *bytes = p.sm ? 0 : p.ctas * 8 * p.nt * p.Ts * 8;
     return IQ_OK;
 }
 
@@ -197,22 +265,26 @@ IQ_API int iq_attn_tree_dev(int64_t *d_out, const int64_t *d_q, const iq_kv_cach
                             void *stream) {
     TreeArgs a = {};
     int dev, rc;
-    int64_t need;
     if ((rc = tree_check(cache, num_heads, n_seq, rows, max_nodes, max_len, &a.c))) return rc;
-    if ((rc = iq_attn_tree_work(cache, num_heads, n_seq, rows, max_nodes, max_len, &need))) return rc;
     if (!d_out || !d_q || !d_len || !d_start || !d_parent || misaligned(d_out, 8) || misaligned(d_q, 8) ||
         misaligned(d_len, 4) || misaligned(d_start, 4) || misaligned(d_parent, 4) || misaligned(d_seq, 4) ||
-        misaligned(d_work, 8) || d_out == d_q || q_stride < (int64_t)num_heads * a.c.hd || work_bytes < need ||
-        (need && !d_work))
+        misaligned(d_work, 8) || d_out == d_q || q_stride < (int64_t)num_heads * a.c.hd || work_bytes < 0)
         return IQ_ERR_ARG;
     if ((rc = cur_device(&dev))) return rc;
+    const TreePlan p = tree_plan(a.c, num_heads, n_seq, rows, max_nodes, max_len);
+    if (p.ctas > INT_MAX) return IQ_ERR_RANGE;
+    const int64_t need = p.sm ? 0 : p.ctas * 8 * p.nt * p.Ts * 8;
+    if (work_bytes < need || (need && !d_work)) return IQ_ERR_ARG;
     a.out = d_out; a.q = d_q; a.seq = d_seq; a.len = d_len; a.start = d_start; a.parent = d_parent;
     a.n_seq = n_seq; a.rows = rows; a.max_nodes = max_nodes; a.max_len = max_len; a.nh = num_heads;
-    a.qs = q_stride; a.sc = (int64_t *)d_work;
+    a.qs = q_stride;
+    a.sc = (int64_t *)d_work;
     a.scale = h_att_scale(a.c.hd);
-    k_tree_simple<<<dim3(n_seq * max_nodes, num_heads), 256, 0, pick(stream)>>>(a);
-    IQ_CHECK_LAUNCH();
-    return IQ_OK;
+    a.cs = p.cs; a.blocks = p.blocks; a.Ts = p.Ts;
+    // 16-byte (exact) or 4-code (packed) loads
+    a.vec = a.c.hd % 4 == 0 && (a.c.kbits ? !misaligned(a.c.kq, 4) && !misaligned(a.c.vq, 8)
+                                          : !misaligned(a.c.k, 16) && !misaligned(a.c.v, 16));
+    return a.c.kbits ? launch_tree_nt<true>(a, p, pick(stream)) : launch_tree_nt<false>(a, p, pick(stream));
 }
 
 IQ_API int iq_logprobs_dev(const int64_t *d_logits, int64_t ld, int rows, int vocab, const int *d_tokens,
