@@ -301,7 +301,7 @@ IQ_API int iq_kv_read_dev(int64_t *d_k, int64_t *d_v, const iq_kv_cache *cache, 
  * max_nodes (<= 256) and max_len (<= max_seq, <= 32767, the range of the
  * int64 softmax sum) bound n_i and d_len[i] + n_i; rows of a sequence beyond its
  * bounds, and rows outside d_start, stay as they were.
- * d_work: iq_attn_tree_work bytes (8-byte aligned) that no other call uses
+ * d_work: iq_attn_tree_work bytes (16-byte aligned) that no other call uses
  * until this one has run. */
 IQ_API int iq_attn_tree_work(const iq_kv_cache *cache, int num_heads, int n_seq, int rows, int max_nodes, int max_len,
                              int64_t *bytes);

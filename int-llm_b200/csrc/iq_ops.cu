@@ -85,70 +85,72 @@ static int tree_check(const iq_kv_cache *cache, int nh, int n_seq, int rows, int
     return IQ_OK;
 }
 
-// How a call is cut: columns a cluster (8 NT), CTAs a cluster (they split the
-// positions), score rows in shared memory or in the workspace. Two CTAs an SM
-// (100 KB each beside the static part) as long as 8 columns fit that way, then one.
-struct TreePlan {
-    int nt, cs, blocks, Ts;
-    bool sm;
-    size_t smem;
-    int64_t ctas;
-};
-static TreePlan tree_plan(const KVArgs &c, int nh, int n_seq, int rows, int max_nodes, int max_len) {
-    const int grp = nh / c.nkv, nd = tree_hdp(c.hd) / 64;
-    const int64_t cols = (int64_t)std::min(max_nodes, rows) * grp;
-    TreePlan p = {};
-    auto row = [&](int cs) { return ((max_len + cs - 1) / cs + 15) / 16 * 16 + 2; };
-    auto fits = [&](int nt, int cs, size_t most) {
-        return (size_t)8 * nt * row(cs) * 8 + tree_side(nt, c.hd) <= most;
-    };
-    const size_t two = 100 * 1024, one = 200 * 1024;
-    p.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : nd <= 2 ? 4 : 2;
-    while (p.nt > 1 && !fits(p.nt, 8, two)) p.nt /= 2;
-    p.sm = fits(p.nt, 8, one);
-    const size_t most = fits(p.nt, 8, two) ? two : one;
-    // enough CTAs for two an SM, none with fewer than 64 positions
-    const int64_t clusters = c.nkv * std::max<int64_t>(n_seq, ((int64_t)rows * grp + 8 * p.nt - 1) / (8 * p.nt));
-    for (p.cs = 1; p.cs < 8; p.cs *= 2) {
-        if (p.sm && !fits(p.nt, p.cs, most)) continue;
-        if (!p.sm || (clusters * p.cs < 2 * dev_info().sms && max_len / p.cs > 64)) continue;
-        break;
-    }
-    p.blocks = (int)((cols + 8 * p.nt - 1) / (8 * p.nt));
-    p.Ts = row(p.cs);
-    p.smem = (p.sm ? (size_t)8 * p.nt * p.Ts * 8 : 0) + tree_side(p.nt, c.hd);
-    p.ctas = (int64_t)n_seq * c.nkv * p.blocks * p.cs;
-    return p;
+// How a call is cut (see k_tree_scores and k_tree_pv).
+static void tree_plan(TreeArgs *a) {
+    const int grp = a->nh / a->c.nkv, sms = dev_info().sms;
+    const int64_t cols = (int64_t)std::min(a->max_nodes, a->rows) * grp;
+    // the row stride keeps every row 16-byte aligned
+    a->Tw = (a->max_len + 3) / 4 * 4;
+    // columns of all sequences, on average over them
+    const int64_t avg = std::max<int64_t>(1, (int64_t)a->rows * grp / a->n_seq);
+    const int nt = cols <= 8 ? 1 : 2, blocks = (int)((cols + 8 * nt - 1) / (8 * nt));
+    a->tiles = (a->max_len + 127) / 128;
+    // up to 8 blocks share the key planes, fewer where that leaves SMs without a CTA
+    const int64_t pairs = (int64_t)a->n_seq * a->c.nkv, have = pairs * a->tiles;
+    a->passes = 8;
+    while (a->passes > 1 && have * ((avg + 8 * nt * a->passes - 1) / (8 * nt * a->passes)) < 4 * sms) a->passes /= 2;
+    a->groups = (blocks + a->passes - 1) / a->passes;
+    a->cg = cols > 16 && a->c.hd <= 128 ? 2 : 1;
+    const int per = cols <= 8 ? 8 : 16 * a->cg;
+    a->cblocks = (int)((cols + per - 1) / per);
+    a->chunk = 1024;
+    const int64_t pv = pairs * ((avg + per - 1) / per);
+    while (a->chunk > 128 && pv * ((a->max_len + a->chunk - 1) / a->chunk) < 4 * sms) a->chunk /= 2;
+    a->chunks = (a->max_len + a->chunk - 1) / a->chunk;
 }
 
-template <int NT, bool PK, bool SM>
-static int launch_tree(const TreeArgs &a, const TreePlan &p, cudaStream_t s) {
+// One kernel; prev: it waits for the one before itself (tree_prev_kernel), so it may start early.
+template <class... P, class... X>
+static int tree_launch(void (*k)(P...), int64_t grid_x, int grid_y, size_t smem, cudaStream_t s, bool prev, X... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)grid_x, (unsigned)grid_y);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = at;
+    cfg.numAttrs = prev ? 1 : 0;
+    IQ_CUDA(cudaLaunchKernelEx(&cfg, k, args...));
+    return IQ_OK;
+}
+
+template <int NT, bool PK>
+static int tree_scores(const TreeArgs &a, cudaStream_t s) {
     static std::atomic<uint64_t> set{0};   // devices whose shared-memory limit is raised
     int dev = 0;
     IQ_CUDA(cudaGetDevice(&dev));
     if (!(set.load() >> dev & 1)) {
-        IQ_CUDA(cudaFuncSetAttribute(k_tree<NT, PK, SM>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+        IQ_CUDA(cudaFuncSetAttribute(k_tree_scores<NT, PK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)tree_scores_smem(NT, 256)));
         set.fetch_or(1ull << dev);
     }
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)p.cs;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)p.ctas);
-    cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = p.smem;
-    cfg.stream = s;
-    cfg.attrs = at;
-    cfg.numAttrs = p.cs > 1 ? 1 : 0;
-    IQ_CUDA(cudaLaunchKernelEx(&cfg, k_tree<NT, PK, SM>, a));
-    return IQ_OK;
+    return tree_launch(k_tree_scores<NT, PK>, (int64_t)a.n_seq * a.c.nkv * a.groups * a.tiles, 1,
+                       tree_scores_smem(NT, a.c.hd), s, false, a);
 }
 template <bool PK>
-static int launch_tree_nt(const TreeArgs &a, const TreePlan &p, cudaStream_t s) {
-    if (!p.sm) return launch_tree<1, PK, false>(a, p, s);
-    return p.nt == 1 ? launch_tree<1, PK, true>(a, p, s) : p.nt == 2 ? launch_tree<2, PK, true>(a, p, s)
-                                                                  : launch_tree<4, PK, true>(a, p, s);
+static int launch_tree(const TreeArgs &a, cudaStream_t s) {
+    const int64_t cols = (int64_t)std::min(a.max_nodes, a.rows) * (a.nh / a.c.nkv);
+    int rc = cols <= 8 ? tree_scores<1, PK>(a, s) : tree_scores<2, PK>(a, s);
+    if (rc) return rc;
+    const int64_t rows = (int64_t)a.n_seq * a.max_nodes;
+    rc = a.max_len <= TREE_SM_T * TREE_SM_E ? tree_launch(k_tree_softmax<PK, false>, rows, a.nh, 0, s, true, a)
+                                            : tree_launch(k_tree_softmax<PK, true>, rows, a.nh, 0, s, true, a);
+    if (rc) return rc;
+    const int64_t pv = (int64_t)a.n_seq * a.c.nkv * a.cblocks * a.chunks;
+    return cols <= 8 ? tree_launch(k_tree_pv<1, PK>, pv, 1, 0, s, true, a)
+                     : tree_launch(k_tree_pv<2, PK>, pv, 1, 0, s, true, a);
 }
 
 extern "C" {
@@ -254,8 +256,7 @@ IQ_API int iq_attn_tree_work(const iq_kv_cache *cache, int num_heads, int n_seq,
     int rc;
     if (!bytes) return IQ_ERR_ARG;
     if ((rc = tree_check(cache, num_heads, n_seq, rows, max_nodes, max_len, &c))) return rc;
-    const TreePlan p = tree_plan(c, num_heads, n_seq, rows, max_nodes, max_len);
-    *bytes = p.sm ? 0 : p.ctas * 8 * p.nt * p.Ts * 8;
+    *bytes = (int64_t)rows * num_heads * ((max_len + 3) / 4 * 4) * 8;
     return IQ_OK;
 }
 
@@ -268,23 +269,24 @@ IQ_API int iq_attn_tree_dev(int64_t *d_out, const int64_t *d_q, const iq_kv_cach
     if ((rc = tree_check(cache, num_heads, n_seq, rows, max_nodes, max_len, &a.c))) return rc;
     if (!d_out || !d_q || !d_len || !d_start || !d_parent || misaligned(d_out, 8) || misaligned(d_q, 8) ||
         misaligned(d_len, 4) || misaligned(d_start, 4) || misaligned(d_parent, 4) || misaligned(d_seq, 4) ||
-        misaligned(d_work, 8) || d_out == d_q || q_stride < (int64_t)num_heads * a.c.hd || work_bytes < 0)
+        misaligned(d_work, 16) || d_out == d_q || q_stride < (int64_t)num_heads * a.c.hd || !d_work ||
+        work_bytes < (int64_t)rows * num_heads * ((max_len + 3) / 4 * 4) * 8)
         return IQ_ERR_ARG;
     if ((rc = cur_device(&dev))) return rc;
-    const TreePlan p = tree_plan(a.c, num_heads, n_seq, rows, max_nodes, max_len);
-    if (p.ctas > INT_MAX) return IQ_ERR_RANGE;
-    const int64_t need = p.sm ? 0 : p.ctas * 8 * p.nt * p.Ts * 8;
-    if (work_bytes < need || (need && !d_work)) return IQ_ERR_ARG;
     a.out = d_out; a.q = d_q; a.seq = d_seq; a.len = d_len; a.start = d_start; a.parent = d_parent;
     a.n_seq = n_seq; a.rows = rows; a.max_nodes = max_nodes; a.max_len = max_len; a.nh = num_heads;
     a.qs = q_stride;
     a.sc = (int64_t *)d_work;
     a.scale = h_att_scale(a.c.hd);
-    a.cs = p.cs; a.blocks = p.blocks; a.Ts = p.Ts;
-    // 16-byte (exact) or 4-code (packed) loads
-    a.vec = a.c.hd % 4 == 0 && (a.c.kbits ? !misaligned(a.c.kq, 4) && !misaligned(a.c.vq, 8)
-                                          : !misaligned(a.c.k, 16) && !misaligned(a.c.v, 16));
-    return a.c.kbits ? launch_tree_nt<true>(a, p, pick(stream)) : launch_tree_nt<false>(a, p, pick(stream));
+    tree_plan(&a);
+    const int64_t most = std::max({(int64_t)n_seq * a.c.nkv * a.groups * a.tiles,
+                                   (int64_t)n_seq * a.c.nkv * a.cblocks * a.chunks, (int64_t)n_seq * max_nodes});
+    if (most > INT_MAX) return IQ_ERR_RANGE;
+    // whole 32-wide steps in aligned pieces: 16 bytes of exact vectors, 16 key and 2 value codes of packed ones
+    a.vec = a.c.hd % 32 == 0 && (a.c.kbits ? !misaligned(a.c.kq, 16) && !misaligned(a.c.vq, 4)
+                                           : !misaligned(a.c.k, 16) && !misaligned(a.c.v, 16));
+    a.vecq = a.c.hd % 32 == 0 && !misaligned(d_q, 16) && q_stride % 2 == 0;
+    return a.c.kbits ? launch_tree<true>(a, pick(stream)) : launch_tree<false>(a, pick(stream));
 }
 
 IQ_API int iq_logprobs_dev(const int64_t *d_logits, int64_t ld, int rows, int vocab, const int *d_tokens,

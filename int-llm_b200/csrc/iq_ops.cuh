@@ -150,9 +150,9 @@ __device__ __forceinline__ int kv_code(int64_t x, int64_t M, int bits, double in
 // ((2q + 1) M >> b) - M (kv_unpack_vector, llama_int.c:1226-1235) from 32-bit halves of M:
 // c M = c Mh 2^32 + c Ml with c < 2^17, and 2^32 is a multiple of 2^b.
 __device__ __forceinline__ int64_t kv_value(int q, int64_t M, int bits) {
-    const int64_t c = 2 * q + 1;
+    const uint32_t c = 2 * q + 1;
     const uint64_t lo = (uint64_t)c * (uint32_t)M;
-    const int64_t hi = c * (M >> 32);
+    const int64_t hi = (int64_t)(int)c * (int)(M >> 32);
     return (int64_t)(((uint64_t)hi << (32 - bits)) + (lo >> bits) - (uint64_t)M);
 }
 

@@ -4,31 +4,35 @@
 //   s_t = fp_mul((int64)(sum_d (i128)q[d] k_t[d] >> 48), fp_inv_sqrt(hd))
 //   m = max s;  e_t = fp_safe_exp(s_t - m);  S = sum e;  p_t = S > 0 ? fp_div(e_t, S) : e_t
 //   out[d] = sum_t fp_mul(p_t, v_t[d])   (wrapping int64)
+// The columns of a (sequence, kv head) are its (node, query head) pairs. Three
+// kernels over scores in the workspace: p needs S, and S the maximum of the whole
+// row, and each step has its own best shape. Every reduction is of whole
+// numbers, so neither tiles nor splits change a result.
 //
-// One cluster of CTAs takes NC = 8 NT columns (node, query head of one kv head)
-// of a sequence; its CTAs split the positions, so K and V are read once for all
-// the columns and the scores stay in shared memory (in the workspace when they
-// do not fit). Maxima, sums and partial outputs meet over distributed shared
-// memory; all of them are whole numbers, so the split changes nothing.
-//
-// 1. Scores on the int8 tensor cores: byte planes of K (A: 16 positions x 32 d)
-//    and Q (B: 32 d x 8 columns), the pairs of each diagonal i + j in one s32
-//    (see k_attn_scores_tc). Where every |x| < 2^55 (128.0) on both sides
-//    plane 6 is the signed top and 49 of the 63 products remain.
-// 2. fp_safe_exp and fp_div in doubles with directed rounding. With r = 2^48 + f,
-//    floor(r^2 / 2^48) = 2^48 + 2f + floor(f^2 / 2^48), and as long as the result is below
-//    2^52 an fma that rounds down at M = 2^52 (one unit = one ulp) gives the
-//    floor: g = M + f -> fma.rd(f 2^-24, f 2^-24, M + 2f). 12 of the 14 squarings
-//    fit (r <= e^2.5); the last two take 32-bit pieces.
-// 3. sum_t floor(p_t v_t / 2^48) as one chain of fma.rd per output at 1.5 2^52: with p
-//    and v exact in doubles and the running sum within 2^51, each step adds
-//    exactly floor(p v 2^-48). As sum p <= 2^48 that holds for |v| <= 2^51 - 2^16
-//    (8.0). Up to |v| < 2^54 (64.0), v = n 2^51 + f with |f| <= 2^50 and
-//    floor(p v / 2^48) = 8 p n + floor(p f / 2^48): a second, exact chain. Larger values take
-//    fp_mul term by term. One DFMA a term against six integer instructions of
-//    the remainder form (k_attn_pv_tc).
+// 1. k_tree_scores, on the tensor cores (tcgen05 kind::i8). With x_u = x + 2^63 in 8
+//    unsigned bytes, q.k = sum_(i,j) 2^(8(i+j)) sum_d q_j k_i - 2^63 (sum q_u + sum k_u) +
+//    hd 2^126, and (q.k >> 48) mod 2^64 needs the diagonals i + j <= 13 and, of the rest,
+//    only -2^15 (sum q + sum k). A: 128 positions x 32 d of one key plane; B: the 8
+//    planes of NC queries (N = 8 NC rows, plane-major). Plane i accumulates into
+//    TMEM from column i NC on, so that all pairs of a diagonal land on the same
+//    NC columns: 8 instructions a step for the 64 pairs, 15 NC columns of s32
+//    (each below 8 pairs x hd x 255^2 < 2^28). The epilogue reads 14 diagonals.
+// 2. k_tree_softmax, a CTA a row and head: fp_safe_exp and fp_div in doubles with
+//    directed rounding. With r / 2^24 exact in a double and M = 2^52 (one unit = one
+//    ulp up to 2^53), fma.rd(r 2^-24, r 2^-24, M) = M + floor(r^2 / 2^48) while that floor is
+//    below 2^52. 12 of the 14 squarings fit (r <= e^2.5 < 16); the last two
+//    take 32-bit pieces.
+// 3. k_tree_pv: sum_t floor(p_t v_t / 2^48) as one chain of fma.rd per output at
+//    1.5 2^52: with p and v exact in doubles and the running sum within 2^51, each
+//    step adds exactly floor(p v 2^-48). As sum p <= 2^48 that holds for
+//    |v| <= 2^51 - 2^32 (8.0). Beyond, v = n 2^51 + f with |f| <= 2^50 and floor(p v / 2^48) =
+//    8 p n + floor(p f / 2^48): f takes the chain, 8 p n (mod 2^64) whole numbers beside it.
+//    The chain runs on the FP64 tensor cores (m8n8k4, .rm: every product is
+//    added and rounded down in its turn), 256 terms an instruction; plain fma.rd
+//    would wait for its operands (a load returns 16 doubles a clock, the pipe
+//    takes 64 terms). Six integer instructions a term is what the remainder form
+//    of k_attn_pv_tc costs.
 #pragma once
-#include <cooperative_groups.h>
 #include "iq_ops.cuh"
 
 namespace iq {
@@ -42,8 +46,10 @@ struct TreeArgs {
     const int *seq, *len, *start, *parent;
     int n_seq, rows, max_nodes, max_len, nh;
     int64_t qs, scale;
-    int64_t *sc;   // [CTA][NC][Ts] scores where they do not fit shared memory, else null
-    int cs, blocks, Ts, vec;   // CTAs a cluster, column blocks a kv head, row stride of the scores, wide loads
+    int64_t *sc;    // workspace [rows][nh][Tw]: scores, then p 2^-48 as doubles
+    int Tw, vec, vecq;
+    int tiles, groups, passes;   // k_tree_scores: position tiles, groups of column blocks, blocks a group
+    int chunk, chunks, cg, cblocks;   // k_tree_pv: positions a CTA, their number, groups of 8 CB columns a block, blocks
 };
 
 struct TreeSeq { int row0, n, len, sq; };
@@ -61,54 +67,185 @@ __device__ __forceinline__ bool tree_seq(const TreeArgs &a, int b, TreeSeq &s) {
     return ok;
 }
 
-// ---- exponentials and quotients
-
-#define TREE_M 4503599627370496.0            // 2^52
-#define TREE_MB 0x4330000000000000ull        // its bits
-#define TREE_A 6755399441055744.0            // 1.5 2^52
-#define TREE_AB 0x4338000000000000ull
-
-__device__ __forceinline__ double tree_u52(uint64_t x) {   // exact for x < 2^52
-    return __longlong_as_double((long long)(x | TREE_MB)) - TREE_M;
+// The d (of a 32-wide step) of element e of a half h. Any order serves as long as keys
+// and queries share it: exact keys take 16-byte pieces in turn, so that the two
+// halves read full sectors, packed ones 16 codes in a row.
+template <bool PK>
+__device__ __forceinline__ int tree_d(int h, int e) {
+    return PK ? h * 16 + e : (e >> 1) * 4 + 2 * h + (e & 1);
 }
-// floor(r^2 / 2^48) for r < 2^56
-__device__ __forceinline__ uint64_t tree_sqr(uint64_t r) {
-    const uint32_t l = (uint32_t)r, h = (uint32_t)(r >> 32);
-    return (((uint64_t)h * h) << 16) + ((((uint64_t)h * l << 1) + __umulhi(l, l)) >> 16);
+
+// The K or V vectors of one (sequence, kv head) from a first position on. The
+// loads never branch: a position or d beyond the end is clamped into the
+// vectors (such keys meet a query plane of zeros or a score that no row sees,
+// such values a probability of zero or an output column that is not kept).
+// wide: aligned pieces; else element by element.
+struct TreeRows {
+    const char *x;         // exact elements or codes
+    const int64_t *mag;    // packed
+    uint32_t rs, ms;       // bytes of a position, magnitudes of a position
+    int T, hd, bits;
+    bool wide;
+};
+template <bool PK>
+__device__ __forceinline__ TreeRows tree_rows(const TreeArgs &a, bool val, size_t vec0, int T) {
+    const KVArgs &c = a.c;
+    const size_t e = vec0 * c.hd;
+    TreeRows r;
+    const int es = !PK ? 8 : val ? 2 : 1;
+    r.x = (!PK ? (const char *)(val ? c.v : c.k) : val ? (const char *)c.vq : (const char *)c.kq) + e * es;
+    r.mag = PK ? (val ? c.vmag : c.kmag) + vec0 : nullptr;
+    r.rs = (uint32_t)c.nkv * c.hd * es;
+    r.ms = c.nkv;
+    r.T = T;
+    r.hd = c.hd;
+    r.bits = val ? c.vbits : c.kbits;
+    r.wide = a.vec;
+    return r;
 }
-// fp_exp(-d) (fp_math.h:714-732) for 0 <= d <= 10
-__device__ __forceinline__ int64_t tree_exp(uint64_t d) {
-    double g = __longlong_as_double((long long)((d >> 14) | TREE_MB));
+// Half h of one position's 32-wide key step from d0 on, as loaded.
+template <bool PK> struct TreeKeys;
+template <> struct TreeKeys<false> {
+    longlong2 x[8];
+    __device__ __forceinline__ void load(const TreeRows &r, int t, int d0, int h) {
+        const int64_t *p = reinterpret_cast<const int64_t *>(r.x + (size_t)(uint32_t)min(t, r.T - 1) * r.rs);
+        if (r.wide) {
+            const longlong2 *q = reinterpret_cast<const longlong2 *>(p + d0 + 2 * h);
 #pragma unroll
-    for (int i = 0; i < 12; i++) {
-        const double u = __fma_rn(g, 0x1p-24, -TREE_M * 0x1p-24);
-        g = __fma_rd(u, u, __fma_rn(g, 2.0, -TREE_M));
+            for (int j = 0; j < 8; j++) x[j] = __ldg(q + 2 * j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                x[j] = make_longlong2(__ldg(p + min(d0 + tree_d<false>(h, 2 * j), r.hd - 1)),
+                                      __ldg(p + min(d0 + tree_d<false>(h, 2 * j + 1), r.hd - 1)));
+        }
     }
-    const uint64_t r12 = IQ_ONE + ((uint64_t)__double_as_longlong(g) & 0xFFFFFFFFFFFFFull);
-    const uint64_t r = tree_sqr(tree_sqr(r12));   // 2^48 <= r < 2^62.5
-    // floor(2^96 / r): reciprocal by two Newton steps (relative error below
-    // 2^-51, so the quotient, at most 2^48, is off by less than 1/8), floored,
-    // then one exact remainder (2^96 = 0 mod 2^64)
-    const double rd = (__longlong_as_double((long long)((r >> 32) | 0x4530000000000000ull)) - 19342813118337666422669312.0) +
-                      __longlong_as_double((long long)((r & 0xFFFFFFFFull) | TREE_MB));
-    double y;
-    asm("rcp.approx.ftz.f64 %0, %1;" : "=d"(y) : "d"(rd));
-    y = __fma_rn(y, __fma_rn(-rd, y, 1.0), y);
-    y = __fma_rn(y, __fma_rn(-rd, y, 1.0), y);
-    uint64_t q = (uint64_t)__double_as_longlong(__fma_rd(y, 0x1p96, TREE_M)) & 0xFFFFFFFFFFFFFull;
-    const int64_t rem = (int64_t)(0 - q * r);
-    if (rem < 0) q--;
-    else if ((uint64_t)rem >= r) q++;
-    return (int64_t)q;
+    // elements 4w .. 4w + 3
+    __device__ __forceinline__ void get(const TreeRows &, int w, int64_t (&o)[4]) const {
+        o[0] = x[2 * w].x; o[1] = x[2 * w].y; o[2] = x[2 * w + 1].x; o[3] = x[2 * w + 1].y;
+    }
+};
+template <> struct TreeKeys<true> {
+    uint32_t q[4];
+    int64_t m;
+    __device__ __forceinline__ void load(const TreeRows &r, int t, int d0, int h) {
+        t = min(t, r.T - 1);
+        const uint8_t *p = reinterpret_cast<const uint8_t *>(r.x) + (size_t)(uint32_t)t * r.rs;
+        m = __ldg(r.mag + (size_t)(uint32_t)t * r.ms);
+        if (r.wide) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p + d0 + h * 16));
+            q[0] = u.x; q[1] = u.y; q[2] = u.z; q[3] = u.w;
+        } else {
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                q[w] = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) q[w] |= (uint32_t)__ldg(p + min(d0 + h * 16 + 4 * w + i, r.hd - 1)) << (8 * i);
+            }
+        }
+    }
+    __device__ __forceinline__ void get(const TreeRows &r, int w, int64_t (&o)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = kv_value((q[w] >> (8 * i)) & 0xFF, m, r.bits);
+    }
+};
+// A lane's values of one position: pairs at d0 + 16 k + 2 gq, k < 4, as loaded.
+template <bool PK> struct TreeVals;
+template <> struct TreeVals<false> {
+    longlong2 x[4];
+    __device__ __forceinline__ void load(const TreeRows &r, int t, const int (&d)[4]) {
+        const char *p = r.x + (size_t)(uint32_t)min(t, r.T - 1) * r.rs;
+        if (r.wide) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) x[k] = *reinterpret_cast<const longlong2 *>(p + d[k] * 8);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int64_t *e = reinterpret_cast<const int64_t *>(p) + d[k];
+                x[k] = make_longlong2(e[0], e[d[k] + 1 < r.hd]);
+            }
+        }
+    }
+    __device__ __forceinline__ longlong2 get(const TreeRows &, int k) const { return x[k]; }
+};
+template <> struct TreeVals<true> {
+    ushort2 q[4];
+    int64_t m;
+    __device__ __forceinline__ void load(const TreeRows &r, int t, const int (&d)[4]) {
+        t = min(t, r.T - 1);
+        const char *p = r.x + (size_t)(uint32_t)t * r.rs;
+        m = __ldg(r.mag + (size_t)(uint32_t)t * r.ms);
+        if (r.wide) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) q[k] = *reinterpret_cast<const ushort2 *>(p + d[k] * 2);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint16_t *e = reinterpret_cast<const uint16_t *>(p) + d[k];
+                q[k] = make_ushort2(e[0], e[d[k] + 1 < r.hd]);
+            }
+        }
+    }
+    __device__ __forceinline__ longlong2 get(const TreeRows &r, int k) const {
+        return make_longlong2(kv_value(q[k].x, m, r.bits), kv_value(q[k].y, m, r.bits));
+    }
+};
+// key or value d < hd of position t < T
+template <bool PK>
+__device__ __forceinline__ int64_t tree_key(const TreeRows &r, int t, int d) {
+    const char *p = r.x + (size_t)(uint32_t)t * r.rs;
+    return PK ? kv_value(reinterpret_cast<const uint8_t *>(p)[d], r.mag[(size_t)(uint32_t)t * r.ms], r.bits)
+              : reinterpret_cast<const int64_t *>(p)[d];
 }
-// fp_div(e, S) for 0 <= e <= 2^48 <= S < 2^63, e <= S, inv = 2^48 / S
-__device__ __forceinline__ uint64_t tree_prob(int64_t e, int64_t S, double inv) {
-    uint64_t q = (uint64_t)__double_as_longlong(__fma_rd(tree_u52((uint64_t)e), inv, TREE_M)) & 0xFFFFFFFFFFFFFull;
-    const int64_t rem = (int64_t)(((uint64_t)e << 48) - q * (uint64_t)S);
-    if (rem < 0) q--;
-    else if (rem >= S) q++;
-    return q;
+template <bool PK>
+__device__ __forceinline__ int64_t tree_val(const TreeRows &r, int t, int d) {
+    const char *p = r.x + (size_t)(uint32_t)t * r.rs;
+    return PK ? kv_value(reinterpret_cast<const uint16_t *>(p)[d], r.mag[(size_t)(uint32_t)t * r.ms], r.bits)
+              : reinterpret_cast<const int64_t *>(p)[d];
 }
+
+// c0, c1 of an 8 x 8 tile += A (8 x 4, row) B (4 x 8, col), each product added and
+// rounded down in its turn
+__device__ __forceinline__ void dmma_rd(double &c0, double &c1, double x, double y) {
+    asm volatile("wmma.mma.sync.aligned.row.col.m8n8k4.rm.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
+                 : "+d"(c0), "+d"(c1) : "d"(x), "d"(y));
+}
+
+// 16 consecutive bytes of each of the 8 planes of 16 elements (offset binary)
+__device__ __forceinline__ void tree_planes(const int64_t (&x)[16], uint32_t (&o)[4][8]) {
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        const int64_t e[4] = {x[4 * w], x[4 * w + 1], x[4 * w + 2], x[4 * w + 3]};
+        byte_planes4(e, o[w]);
+        o[w][7] ^= 0x80808080u;
+    }
+}
+// byte offset of 16-byte piece c of row r in a tile of 128-byte rows with the 128-byte swizzle
+__device__ __forceinline__ uint32_t tree_sw(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
+
+// 4 TMEM columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t (&v)[4]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_zero4(uint32_t taddr) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %1, %1, %1};" :: "r"(taddr), "r"(0) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// this thread's shared-memory writes before the tensor cores' reads
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void madu(uint64_t &acc, uint32_t x, uint32_t y) {
+    asm("mad.wide.u32 %0, %1, %2, %0;" : "+l"(acc) : "r"(x), "r"(y));
+}
+
+// Range check from the high words, gathered with a maximum: hi + b as unsigned stays
+// below 2b exactly when -b <= hi < b.
+__device__ __forceinline__ void tree_hi(uint32_t &m, int64_t x, uint32_t b) { m = max(m, (uint32_t)(x >> 32) + b); }
+#define TREE_V1 ((1u << 19) - 1)    // |x| <= 2^51 - 2^32: one chain
+
+// Work that the kernel launched before this one may still be doing is waited for here.
+__device__ __forceinline__ void tree_prev_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // fp_mul(s, c) for 0 <= c <= 2^48 (the score scale)
 __device__ __forceinline__ int64_t tree_scale(int64_t s, uint64_t c) {
     const uint32_t sl = (uint32_t)s, cl = (uint32_t)c, ch = (uint32_t)(c >> 32);
@@ -117,394 +254,476 @@ __device__ __forceinline__ int64_t tree_scale(int64_t s, uint64_t c) {
     return (int64_t)((uint64_t)(sh * (int64_t)ch) << 16) + (t >> 16) + (u >> 16) + (((t & 0xFFFF) + (u & 0xFFFF)) >> 16);
 }
 
-// ---- the kernel
+// ---------------------------------------------------------------- 1. scores
 
-#define TREE_V 4096   // doubles of a staged value tile
+#define TREE_A_BYTES 65536   // key planes: two steps of (128 positions x 4 planes x 32 d) x 2
+__host__ __device__ constexpr size_t tree_b_bytes(int NT, int hd) { return (size_t)((hd + 127) / 128) * 64 * NT * 128; }
+__host__ __device__ constexpr size_t tree_scores_smem(int NT, int hd) { return 1024 + TREE_A_BYTES + tree_b_bytes(NT, hd); }
 
-template <bool PK>
-__device__ __forceinline__ int64_t tree_at(const KVArgs &c, bool val, size_t vec, int d) {
-    const size_t e = vec * c.hd + d;
-    if (!PK) return (val ? c.v : c.k)[e];
-    return val ? kv_value(c.vq[e], c.vmag[vec], c.vbits) : kv_value(c.kq[e], c.kmag[vec], c.kbits);
-}
-// elements d .. d + 3 of a vector, zero from hd on
-template <bool PK>
-__device__ __forceinline__ void tree_at4(const TreeArgs &a, bool val, size_t vec, int d, int64_t (&x)[4]) {
-    const KVArgs &c = a.c;
-    if (a.vec && d < c.hd) {   // hd a multiple of 4, aligned bases
-        const size_t e = vec * c.hd + d;
-        if (!PK) {
-            const longlong2 *p = reinterpret_cast<const longlong2 *>((val ? c.v : c.k) + e);
-            const longlong2 u = __ldg(p), w = __ldg(p + 1);
-            x[0] = u.x; x[1] = u.y; x[2] = w.x; x[3] = w.y;
-        } else if (val) {
-            const ushort4 q = __ldg(reinterpret_cast<const ushort4 *>(c.vq + e));
-            const int64_t M = __ldg(c.vmag + vec);
-            x[0] = kv_value(q.x, M, c.vbits); x[1] = kv_value(q.y, M, c.vbits);
-            x[2] = kv_value(q.z, M, c.vbits); x[3] = kv_value(q.w, M, c.vbits);
-        } else {
-            const uchar4 q = __ldg(reinterpret_cast<const uchar4 *>(c.kq + e));
-            const int64_t M = __ldg(c.kmag + vec);
-            x[0] = kv_value(q.x, M, c.kbits); x[1] = kv_value(q.y, M, c.kbits);
-            x[2] = kv_value(q.z, M, c.kbits); x[3] = kv_value(q.w, M, c.kbits);
+// A CTA takes 128 positions of one (sequence, kv head) and up to a.passes blocks of
+// NC = 8 NT columns. With hd <= 64 the key planes are made once for all its blocks.
+// Two CTAs an SM (three with 8 columns) overlap one another's loads, products
+// and epilogues; TMEM holds 128 NT columns a CTA.
+template <int NT, bool PK>
+__global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __grid_constant__ TreeArgs a) {
+    extern __shared__ __align__(16) char tree_smem[];
+    constexpr int NC = 8 * NT, HC = NC / 2;
+    __shared__ int64_t ksum[128];              // sum of a position's key
+    __shared__ unsigned long long qsum[NC];
+    __shared__ __align__(8) uint64_t mbar[2];  // the products of a step's key planes are done
+    __shared__ uint32_t tmem_s;
+    const int tile = blockIdx.x % a.tiles, rest = blockIdx.x / a.tiles;
+    const int group = rest % a.groups, g = rest / a.groups % a.c.nkv, b = rest / a.groups / a.c.nkv;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int grp = a.nh / a.c.nkv, hd = a.c.hd, KS = (hd + 31) / 32;
+    TreeSeq s;
+    if (!tree_seq(a, b, s)) return;
+    const int cols = s.n * grp, T = s.len + s.n, tb = tile * 128, Tl = min(128, T - tb);
+    const int p0 = group * a.passes, p1 = min(p0 + a.passes, (cols + NC - 1) / NC);   // column blocks
+    if (Tl <= 0 || p0 >= p1) return;
+    char *const sA = tree_smem + ((1024 - (smem_u32(tree_smem) & 1023)) & 1023), *const sB = sA + TREE_A_BYTES;
+
+    // conversion: two threads a position; eight lanes in a row take positions whose
+    // swizzles differ, so that their 16-byte stores meet no bank twice
+    const int cq = lane >> 1, ch = lane & 1, cp = warp * 16 + ((cq & 8) | ((cq & 3) << 1) | ((cq >> 2) & 1));
+    const TreeRows kr = tree_rows<PK>(a, false, ((size_t)s.sq * a.c.max_seq + tb) * a.c.nkv + g, Tl);
+    TreeKeys<PK> kx;
+    if (cp < Tl) kx.load(kr, cp, 0, ch);
+    if (warp == 0) tmem_alloc(&tmem_s, 128 * NT);
+    if (tid == 0) {
+        mbar_init(&mbar[0], 1);
+        mbar_init(&mbar[1], 1);
+        fence_mbar_init();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    // epilogue: TMEM lane quadrant warp & 3, half of the columns warp >> 2
+    const uint32_t tmem = tmem_s, tlane = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (warp >> 2) * HC;
+    const int ep = (warp & 3) * 32 + lane;
+    int batch = 0;   // steps issued; step n uses half n & 1 of the key planes
+    unsigned long long sum = 0;
+    for (int pass = p0; pass < p1; pass++) {
+        // the diagonals that plane 0 does not start
+#pragma unroll
+        for (int sd = 8; sd < 14; sd++)
+#pragma unroll
+            for (int c = 0; c < HC; c += 4) tmem_zero4(tlane + sd * NC + c);
+        tmem_st_wait();
+        // query planes of the block
+        const int c0 = pass * NC, nc = min(NC, cols - c0);
+        if (tid < NC) qsum[tid] = 0;
+        __syncthreads();
+        for (int e = tid; e < NC * KS * 2; e += 256) {   // (column, step, half)
+            const int h = e & 1, col = (e >> 1) % NC, ks = (e >> 1) / NC, cc = c0 + min(col, nc - 1);
+            const int64_t *q = a.q + (int64_t)(s.row0 + cc / grp) * a.qs + (int64_t)(g * grp + cc % grp) * hd;
+            int64_t x[16];
+            if (a.vecq) {   // whole steps, aligned pairs
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const longlong2 u = __ldg(reinterpret_cast<const longlong2 *>(q + ks * 32 + tree_d<PK>(h, i)));
+                    x[i] = u.x;
+                    x[i + 1] = u.y;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int d = ks * 32 + tree_d<PK>(h, i);
+                    x[i] = d < hd ? q[d] : 0;
+                }
+            }
+            unsigned long long qs = 0;
+#pragma unroll
+            for (int i = 0; i < 16; i++) qs += (unsigned long long)x[i];
+            uint32_t o[4][8];
+            tree_planes(x, o);
+            if (!a.vecq)   // beyond hd x_u is 0, not 2^63: nothing meets whatever the keys hold there
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (ks * 32 + tree_d<PK>(h, i) >= hd) o[i >> 2][7] &= ~(0xFFu << (8 * (i & 3)));
+            char *tile_b = sB + (size_t)(ks >> 2) * 64 * NT * 128;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                *reinterpret_cast<uint4 *>(tile_b + tree_sw(j * NC + col, (ks & 3) * 2 + h)) =
+                    make_uint4(o[0][j], o[1][j], o[2][j], o[3][j]);
+            atomicAdd(&qsum[col], qs);
         }
+        const bool made = KS <= 2 && pass > p0;   // the key planes stand
+        for (int ks = 0; ks < KS; ks++, batch++) {
+            char *const A = sA + (size_t)(batch & 1) * 32768;
+            if (!made) {
+                if (batch >= 2) mbar_wait(&mbar[batch & 1], (uint32_t)((batch >> 1) - 1) & 1u);
+                if (cp < Tl) {
+                    int64_t x[16];
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        int64_t e[4];
+                        kx.get(kr, w, e);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) x[4 * w + i] = e[i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (kr.wide || ks * 32 + tree_d<PK>(ch, i) < hd) sum += (unsigned long long)x[i];
+                    // the next step's keys are on their way meanwhile
+                    if (ks + 1 < KS || (KS > 2 && pass + 1 < p1)) kx.load(kr, cp, ks + 1 < KS ? (ks + 1) * 32 : 0, ch);
+                    uint32_t o[4][8];
+                    tree_planes(x, o);
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        *reinterpret_cast<uint4 *>(A + (j >> 2) * 16384 + tree_sw(cp, (j & 3) * 2 + ch)) =
+                            make_uint4(o[0][j], o[1][j], o[2][j], o[3][j]);
+                }
+                if (ks == KS - 1 && pass == p0) {
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    if (ch == 0) ksum[cp] = (int64_t)sum;
+                }
+            }
+            if (!made || ks == 0) {
+                fence_async_smem();
+                tc_fence_before();
+                __syncthreads();
+            }
+            if (tid == 0) {
+                tc_fence_after();
+                const char *Am = made && KS == 1 ? sA : A;
+                const uint64_t bd = smem_desc_sw128(sB + (size_t)(ks >> 2) * 64 * NT * 128) + 2 * (ks & 3);
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    tc_mma_i8(tmem + i * NC, smem_desc_sw128(Am + (i >> 2) * 16384) + 2 * (i & 3), bd,
+                              idesc_i8(false, false, 128, 8 * NC), ks > 0 || i > 0);
+                tc_commit(&mbar[batch & 1]);
+            }
+        }
+        // (a wait that runs out has recorded IQ_ERR_TIMEOUT; the outputs then mean nothing)
+        mbar_wait(&mbar[(batch - 1) & 1], (uint32_t)((batch - 1) >> 1) & 1u);
+        tc_fence_after();
+        const unsigned long long kp = (unsigned long long)ksum[ep];
+#pragma unroll
+        for (int c = 0; c < HC; c += 4) {
+            uint32_t v[14][4];
+#pragma unroll
+            for (int sd = 0; sd < 14; sd++) tmem_ld4(tlane + sd * NC + c, v[sd]);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint64_t G[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    G[k] = v[4 * k][i];
+#pragma unroll
+                    for (int m = 1; m < 4; m++)
+                        if (4 * k + m < 14) madu(G[k], v[4 * k + m][i], 1u << (8 * m));
+                }
+                // (G0 + G1 2^32 + G2 2^64 + G3 2^96) >> 48, nested floors, less 2^15 (sum q + sum k)
+                const int col = (warp >> 2) * HC + c + i, cc = c0 + col;
+                const uint64_t dot = (((G[0] >> 32) + G[1]) >> 16) + (G[2] << 16) + (G[3] << 48) - ((qsum[col] + kp) << 15);
+                if (ep < Tl && col < nc)
+                    a.sc[((size_t)(s.row0 + cc / grp) * a.nh + g * grp + cc % grp) * a.Tw + tb + ep] =
+                        tree_scale((int64_t)dot, (uint64_t)a.scale);
+            }
+        }
+        tc_fence_before();
+        __syncthreads();   // qsum, TMEM and the query planes are free
+        tc_fence_after();
+    }
+    if (warp == 0) tmem_dealloc(tmem, 128 * NT);
+}
+
+// --------------------------------------------------------------- 2. softmax
+
+#define TREE_M 4503599627370496.0            // 2^52
+#define TREE_MB 0x4330000000000000ull        // its bits
+#define TREE_A 6755399441055744.0            // 1.5 2^52
+#define TREE_AB 0x4338000000000000ull
+#define TREE_MASK 0xFFFFFFFFFFFFFull
+
+__device__ __forceinline__ double tree_u52(uint64_t x) {   // exact for x < 2^52
+    return __longlong_as_double((long long)(x | TREE_MB)) - TREE_M;
+}
+// floor(r^2 / 2^48) for r < 2^56, r = h 2^32 + l: h^2 2^16 + (2 h l + (l^2 >> 32) >> 16)
+__device__ __forceinline__ uint64_t tree_sqr(uint64_t r) {
+    const uint32_t l = (uint32_t)r, h = (uint32_t)(r >> 32);
+    uint64_t x = __umulhi(l, l);
+    madu(x, 2 * h, l);
+    x >>= 16;
+    madu(x, h << 8, h << 8);
+    return x;
+}
+// fp_exp(-d) (fp_math.h:714-732) for 0 <= d <= 10
+__device__ __forceinline__ int64_t tree_exp(uint64_t d) {
+    double g = __longlong_as_double((long long)(((d >> 14) + IQ_ONE) | TREE_MB));   // M + r
+#pragma unroll
+    for (int i = 0; i < 12; i++) {
+        const double u = __fma_rn(g, 0x1p-24, -TREE_M * 0x1p-24);
+        g = __fma_rd(u, u, TREE_M);
+    }
+    const uint64_t r = tree_sqr(tree_sqr((uint64_t)__double_as_longlong(g) & TREE_MASK));   // 2^48 <= r < 2^62.5
+    // floor(2^96 / r), at most 2^48: reciprocal by two Newton steps (relative error
+    // below 2^-51), lowered by 2^-50 so that its floor is q or q - 1; the remainder
+    // (2^96 = 0 mod 2^64) tells which
+    const double rd = (__longlong_as_double((long long)((r >> 32) | 0x4530000000000000ull)) - 19342813118337666422669312.0) +
+                      __longlong_as_double((long long)((r & 0xFFFFFFFFull) | TREE_MB));
+    double y;
+    asm("rcp.approx.ftz.f64 %0, %1;" : "=d"(y) : "d"(rd));
+    y = __fma_rn(y, __fma_rn(-rd, y, 1.0), y);
+    y = __fma_rn(y, __fma_rn(-rd, y, 1.0), y);
+    const uint64_t q = (uint64_t)__double_as_longlong(__fma_rd(y, 0x1p96 - 0x1p46, TREE_M)) & TREE_MASK;
+    return (int64_t)(q + (0 - q * r >= r));
+}
+// 2^48 / S, lowered likewise for tree_prob
+__device__ __forceinline__ double tree_inv(int64_t S) {
+    return __dmul_rn(281474976710656.0 / (double)S, 1.0 - 0x1p-50);
+}
+// fp_div(e, S) 2^-48 as a double for 0 <= e <= S, 2^48 <= S < 2^63, e <= 2^48
+__device__ __forceinline__ double tree_prob(int64_t e, int64_t S, double inv) {
+    uint64_t q = (uint64_t)__double_as_longlong(__fma_rd(tree_u52((uint64_t)e), inv, TREE_M)) & TREE_MASK;
+    q += ((uint64_t)e << 48) - q * (uint64_t)S >= (uint64_t)S;
+    return tree_u52(q) * 0x1p-48;
+}
+
+// A row in which a score difference wraps: fp_safe_exp of the wrapped difference, the
+// int64 sum, fp_div and fp_mul term by term. p goes through the row of the
+// workspace, which is then zero. The scores are made again.
+template <bool PK, class Sees>
+__device__ __noinline__ void tree_wrapped(const TreeArgs &a, const TreeSeq &s, int r, int h, int T, int64_t m, int64_t *row,
+                                          int64_t *out, uint64_t *red, const Sees &sees) {
+    const int hd = a.c.hd, g = h / (a.nh / a.c.nkv);
+    const size_t vec0 = (size_t)s.sq * a.c.max_seq * a.c.nkv + g;
+    const TreeRows kr = tree_rows<PK>(a, false, vec0, T), vr = tree_rows<PK>(a, true, vec0, T);
+    const int64_t *q = a.q + (int64_t)r * a.qs + (int64_t)h * hd;
+    uint64_t sum = 0;
+    for (int t = threadIdx.x; t < T; t += blockDim.x) {
+        int64_t e = 0;
+        if (sees(t)) {
+            i128 dot = 0;
+            for (int d = 0; d < hd; d++) dot += d_mul128(q[d], tree_key<PK>(kr, t, d));
+            e = d_safe_exp((int64_t)((uint64_t)d_mul((int64_t)(dot >> 48), a.scale) - (uint64_t)m));
+        }
+        row[t] = e;
+        sum += (uint64_t)e;
+    }
+    const int64_t S = (int64_t)(uint64_t)cta_sum_i128((i128)(u128)sum, red);
+    for (int t = threadIdx.x; t < T; t += blockDim.x)
+        if (S > 0) row[t] = d_div(row[t], S);
+    __syncthreads();
+    for (int d = threadIdx.x; d < hd; d += blockDim.x) {
+        uint64_t acc = 0;
+        for (int t = 0; t < T; t++) acc += (uint64_t)d_mul(row[t], tree_val<PK>(vr, t, d));
+        out[d] = (int64_t)acc;
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t < min(a.Tw, (s.len + s.n + 3) & ~3); t += blockDim.x) row[t] = 0;
+}
+
+// A CTA a (node row, head). E scores a thread stay in registers; longer rows go
+// through the workspace three times (LONG). A row whose score differences
+// wrap (the reference's int64 then gives other numbers, reproduced here) is
+// finished here term by term and leaves zeros to k_tree_pv.
+#define TREE_SM_T 256
+#define TREE_SM_E 8
+template <bool PK, bool LONG>
+__global__ void __launch_bounds__(TREE_SM_T) k_tree_softmax(const __grid_constant__ TreeArgs a) {
+    __shared__ uint64_t red[64];
+    __shared__ int up[TREE_MAX_NODES];
+    __shared__ uint32_t anc[TREE_MAX_NODES / 32];
+    const int b = blockIdx.x / a.max_nodes, node = blockIdx.x % a.max_nodes, h = blockIdx.y, tid = threadIdx.x;
+    TreeSeq s;
+    if (!tree_seq(a, b, s) || node >= s.n) return;
+    const int r = s.row0 + node, hd = a.c.hd, T = s.len + node + 1;   // no later node is seen
+    // ancestors of the node
+    for (int i = tid; i < node; i += TREE_SM_T) up[i] = a.parent[s.row0 + i];
+    if (tid < TREE_MAX_NODES / 32) anc[tid] = 0;
+    if (tid == TREE_SM_T - 1) up[node] = a.parent[r];
+    __syncthreads();
+    if (tid == 0)
+        for (int j = node;;) {
+            anc[j >> 5] |= 1u << (j & 31);
+            const int p = up[j];
+            if (p < 0 || p >= j) break;
+            j = p;
+        }
+    tree_prev_kernel();
+    __syncthreads();
+    int64_t *row = a.sc + ((size_t)r * a.nh + h) * a.Tw;
+    auto sees = [&](int t) {
+        const int j = t - s.len;
+        return j < 0 || (t < T && (anc[j >> 5] >> (j & 31) & 1));
+    };
+    int64_t x[TREE_SM_E], m = INT64_MIN;
+    for (int t0 = 0; t0 < (LONG ? T : 1); t0 += TREE_SM_T * TREE_SM_E) {
+#pragma unroll
+        for (int k = 0; k < TREE_SM_E; k++) {
+            const int t = t0 + k * TREE_SM_T + tid;
+            x[k] = t < T ? row[t] : INT64_MIN;
+            if (sees(t)) m = max(m, x[k]);
+        }
+    }
+    m = cta_max_i64(m, (int64_t *)red);
+    uint64_t sum = 0;
+    int wraps = 0;
+    for (int t0 = 0; t0 < (LONG ? T : 1); t0 += TREE_SM_T * TREE_SM_E) {
+#pragma unroll
+        for (int k = 0; k < TREE_SM_E; k++) {
+            const int t = t0 + k * TREE_SM_T + tid;
+            if (k && t0 + k * TREE_SM_T >= T) break;
+            if (LONG) x[k] = t < T ? row[t] : INT64_MIN;
+            const uint64_t d = (uint64_t)m - (uint64_t)x[k];
+            const bool in = sees(t);
+            wraps |= in && (int64_t)d < 0;
+            const int64_t e = tree_exp(d <= 10 * (uint64_t)IQ_ONE ? d : 0);
+            x[k] = in && d <= 10 * (uint64_t)IQ_ONE ? e : 0;
+            sum += (uint64_t)x[k];
+            if (LONG && t < T) row[t] = x[k];
+        }
+    }
+    int64_t *out = a.out + ((size_t)r * a.nh + h) * hd;
+    if (__syncthreads_or(wraps)) {
+        tree_wrapped<PK>(a, s, r, h, T, m, row, out, red, sees);
         return;
     }
+    const int64_t S = (int64_t)(uint64_t)cta_sum_i128((i128)(u128)sum, red);
+    const double inv = tree_inv(S);
+    double *p = reinterpret_cast<double *>(row);
+    const int end = min(a.Tw, (s.len + s.n + 3) & ~3);   // k_tree_pv reads fours up to here
+    for (int t0 = 0; t0 < (LONG ? end : 1); t0 += TREE_SM_T * TREE_SM_E) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = d + i < c.hd ? tree_at<PK>(c, val, vec, d + i) : 0;
-}
-
-// All plane pairs of one 16 x 8 x 32 step into the diagonals; P planes, the last signed.
-template <int P>
-__device__ __forceinline__ void tree_mma(int (&acc)[14][4], const uint32_t (&A)[4][8], const uint2 *B, int lane) {
-#pragma unroll
-    for (int j = 0; j < P; j++) {
-        const uint2 b = B[j * 32 + lane];
-#pragma unroll
-        for (int i = 0; i < P; i++) {
-            if (i + j > 13) continue;
-            if (i == P - 1 && j == P - 1) mma_s32<true, true>(acc[i + j], A[0][i], A[1][i], A[2][i], A[3][i], b.x, b.y);
-            else if (i == P - 1) mma_s32<true, false>(acc[i + j], A[0][i], A[1][i], A[2][i], A[3][i], b.x, b.y);
-            else if (j == P - 1) mma_s32<false, true>(acc[i + j], A[0][i], A[1][i], A[2][i], A[3][i], b.x, b.y);
-            else mma_s32<false, false>(acc[i + j], A[0][i], A[1][i], A[2][i], A[3][i], b.x, b.y);
+        for (int k = 0; k < TREE_SM_E; k++) {
+            const int t = t0 + k * TREE_SM_T + tid;
+            if (t0 + k * TREE_SM_T >= end) break;
+            const int64_t e = LONG ? (t < T ? row[t] : 0) : t < T ? x[k] : 0;
+            if (t < end) p[t] = tree_prob(e, S, inv);
         }
     }
+    for (int d = tid; d < hd; d += TREE_SM_T) out[d] = 0;   // k_tree_pv adds
 }
 
-__device__ __forceinline__ bool tree_big(int64_t x) { return (uint64_t)(x + (1ll << 55)) >= (1ull << 56); }
+// ---------------------------------------------------- 3. probabilities x values
 
-__host__ __device__ constexpr int tree_hdp(int hd) { return (hd + 63) / 64 * 64; }
-// bytes of shared memory beside the scores: query planes, or value tile and partial outputs
-__host__ __device__ constexpr size_t tree_side(int NT, int hd) {
-    const size_t q = (size_t)NT * ((hd + 31) / 32) * 8 * 32 * 8;
-    const size_t v = (size_t)TREE_V * 8 + (size_t)8 * NT * tree_hdp(hd) * 8;
-    return q > v ? q : v;
-}
+#define TREE_RED 4096   // whole numbers of the buffer in which partial outputs meet
 
-template <int NT, bool PK, bool SM>
-__global__ void __launch_bounds__(256, 2) k_tree(const __grid_constant__ TreeArgs a) {
-    namespace cg = cooperative_groups;
-    extern __shared__ __align__(16) char tree_smem[];
-    constexpr int NC = 8 * NT;
-    __shared__ int64_t cmax[NC], csum[NC], gmax[NC], gsum[NC];
-    __shared__ double ginv[NC];
-    __shared__ uint32_t anc[TREE_MAX_NODES][TREE_MAX_NODES / 32];   // nodes that a node sees
-    __shared__ int up[TREE_MAX_NODES];
-    __shared__ int weird_s;
-    const int rank = blockIdx.x % a.cs, rest = blockIdx.x / a.cs;
-    const int blk = rest % a.blocks, g = rest / a.blocks % a.c.nkv, b = rest / a.blocks / a.c.nkv;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+// A CTA takes a.chunk positions of CG x 8 CB columns of one (sequence, kv head); a
+// warp 64 d of 8 CB columns and every tg_n-th four positions. A lane holds V of
+// position lane & 3 at d = 16 k + 2 (lane >> 2) + {0, 1}, k < 4, i.e. column lane >> 2 of
+// the 8-wide tiles 2k and 2k + 1, and of each tile's output the columns
+// 2 (lane & 3) + {0, 1}. Values come straight from global memory: nothing is
+// staged and no barrier runs inside the loop.
+template <int CB, bool PK>
+__global__ void __launch_bounds__(256, 2) k_tree_pv(const __grid_constant__ TreeArgs a) {
+    __shared__ __align__(16) unsigned long long red[TREE_RED];
+    constexpr int CW = 8 * CB;
+    const int chunk = blockIdx.x % a.chunks, rest = blockIdx.x / a.chunks;
+    const int blk = rest % a.cblocks, g = rest / a.cblocks % a.c.nkv, b = rest / a.cblocks / a.c.nkv;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
+    const int grp = a.nh / a.c.nkv, hd = a.c.hd, hdp = (hd + 63) / 64 * 64, nd = hdp >> 6;
     TreeSeq s;
-    const int grp = a.nh / a.c.nkv, hd = a.c.hd;
-    // uniform over the cluster: every CTA of it leaves here or none
-    if (!tree_seq(a, b, s) || blk * NC >= s.n * grp) return;
-    const int cols = min(NC, s.n * grp - blk * NC), c0 = blk * NC, T = s.len + s.n;
-    const int per = ((T + a.cs - 1) / a.cs + 15) & ~15;
-    const int tb = min(T, rank * per), Tl = min(per, T - tb), Tp = (Tl + 15) & ~15;   // this CTA's positions
-    const size_t v0 = (size_t)s.sq * a.c.max_seq + tb;
-    int64_t *sc = SM ? reinterpret_cast<int64_t *>(tree_smem) : a.sc + (size_t)blockIdx.x * NC * a.Ts;
-    char *side = SM ? tree_smem + (size_t)NC * a.Ts * 8 : tree_smem;
-    uint2 *qp = reinterpret_cast<uint2 *>(side);   // [NT][KS][8][32]
-    const int KS = (hd + 31) / 32;
-
-    // ---- query planes in B-fragment order, node masks
-    int qbig = 0;
-    for (int e = tid; e < NT * KS * 64; e += 256) {   // (nt, ks, fragment half, lane)
-        const int ln = e & 31, f = (e >> 5) & 1, ks = (e >> 6) % KS, nt = (e >> 6) / KS;
-        const int col = nt * 8 + (ln >> 2), d = ks * 32 + (ln & 3) * 4 + f * 16;
-        int64_t x[4] = {0, 0, 0, 0};
-        if (col < cols) {
-            const int64_t *q = a.q + (int64_t)(s.row0 + (c0 + col) / grp) * a.qs + (int64_t)(g * grp + (c0 + col) % grp) * hd;
+    if (!tree_seq(a, b, s)) return;
+    const int CG = a.cg, NC = CG * CW;   // NC hdp <= TREE_RED
+    const int cols = min(NC, s.n * grp - blk * NC), c0 = blk * NC, tb = chunk * a.chunk;
+    const int Tl = min(a.chunk, s.len + s.n - tb);
+    if (Tl <= 0 || cols <= 0) return;
+    const int units = CG * nd, tg_n = 8 / units;   // units <= 8; warps from units * tg_n on idle
+    const int unit = warp % units, tg = warp / units, pc = unit / nd * CW, db = unit % nd * 64;
+    const bool on = tg < tg_n && pc < cols;
+    for (int e = tid; e < NC * hdp; e += 256) red[e] = 0;
+    const TreeRows vr = tree_rows<PK>(a, true, ((size_t)s.sq * a.c.max_seq + tb) * a.c.nkv + g, Tl);
+    int vd[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                x[i] = d + i < hd ? q[d + i] : 0;
-                qbig |= tree_big(x[i]);
-            }
-        }
-        uint32_t o[8];
-        byte_planes4(x, o);
-        uint32_t *dst = reinterpret_cast<uint32_t *>(qp + (size_t)(nt * KS + ks) * 256 + ln) + f;
+    for (int k = 0; k < 4; k++) vd[k] = db + 16 * k + 2 * gq < hd ? db + 16 * k + 2 * gq : 0;
+    const double *pp[CB];   // this lane's columns (a missing one: the last, not kept)
 #pragma unroll
-        for (int j = 0; j < 8; j++) dst[j * 64] = o[j];
+    for (int cb = 0; cb < CB; cb++) {
+        const int cc = c0 + min(pc + cb * 8 + gq, cols - 1);
+        pp[cb] = reinterpret_cast<const double *>(a.sc) +
+                 ((size_t)(s.row0 + cc / grp) * a.nh + g * grp + cc % grp) * a.Tw + tb;
     }
-    // ancestors by pointer doubling: after k rounds a node knows 2^k of its path
-    constexpr int AW = TREE_MAX_NODES / 32;
-    const int nw = (s.n + 31) >> 5;
-    if (tid < s.n) {
-        for (int i = 0; i < nw; i++) anc[tid][i] = i == tid >> 5 ? 1u << (tid & 31) : 0;
-        const int p = a.parent[s.row0 + tid];
-        up[tid] = p < tid ? p : -1;
-    }
+    double f[CB][8][2];
+#pragma unroll
+    for (int cb = 0; cb < CB; cb++)
+#pragma unroll
+        for (int k = 0; k < 8; k++) f[cb][k][0] = f[cb][k][1] = TREE_A;
+    TreeVals<PK> vx;
+    if (on) vx.load(vr, tg * 4 + tq, vd);
+    tree_prev_kernel();
     __syncthreads();
-    for (int k = 1; k < s.n; k <<= 1) {
-        uint32_t m[AW];
-        int nu = -1;
-        const int p = tid < s.n ? up[tid] : -1;
-        if (p >= 0) {
-            for (int i = 0; i < AW; i++) m[i] = i < nw ? anc[p][i] : 0;
-            nu = up[p];
-        }
-        if (!__syncthreads_or(p >= 0)) break;
-        if (p >= 0) {
-            for (int i = 0; i < AW; i++)
-                if (i < nw) anc[tid][i] |= m[i];
-            up[tid] = nu;
-        }
-        __syncthreads();
-    }
-    if (tid == 0) weird_s = 0;
-    qbig = __syncthreads_or(qbig);
-
-    // ---- 1. scores
-    const int gq = lane >> 2, tq = lane & 3;
-    for (int u = warp; u < (Tp >> 4) * NT; u += 8) {
-        const int nt = u % NT, t0 = u / NT * 16;
-        if (nt * 8 >= cols) continue;
-        int acc[14][4];
+    if (on) {
+        double pn[CB];
 #pragma unroll
-        for (int k = 0; k < 14; k++) acc[k][0] = acc[k][1] = acc[k][2] = acc[k][3] = 0;
-        for (int ks = 0; ks < KS; ks++) {
-            uint32_t A[4][8];
-            int big = qbig;
-            int64_t x[4][4];
-#pragma unroll
-            for (int f = 0; f < 4; f++) {   // rows gq (+8), columns tq*4 (+16)
-                const int t = t0 + gq + (f & 1) * 8, d = ks * 32 + tq * 4 + (f >> 1) * 16;
-                x[f][0] = x[f][1] = x[f][2] = x[f][3] = 0;
-                if (t < Tl) tree_at4<PK>(a, false, (v0 + t) * a.c.nkv + g, d, x[f]);
-            }
-#pragma unroll
-            for (int f = 0; f < 4; f++) {
-                big |= tree_big(x[f][0]) | tree_big(x[f][1]) | tree_big(x[f][2]) | tree_big(x[f][3]);
-                byte_planes4(x[f], A[f]);
-            }
-            const uint2 *B = qp + (size_t)(nt * KS + ks) * 256;
-            if (__any_sync(0xffffffffu, big)) tree_mma<8>(acc, A, B, lane);
-            else tree_mma<7>(acc, A, B, lane);
-        }
-#pragma unroll
-        for (int c = 0; c < 4; c++) {   // positions t0 + gq (+8), columns 2 tq + {0, 1}
-            int64_t G[4];
+        for (int cb = 0; cb < CB; cb++) pn[cb] = tg * 4 < Tl ? pp[cb][tg * 4 + tq] : 0;
+        for (int t0 = tg * 4; t0 < Tl; t0 += tg_n * 4) {
+            longlong2 nx[4];
+            double p[CB];
+            uint32_t vm = 0;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                G[k] = acc[4 * k][c];
-#pragma unroll
-                for (int m = 1; m < 4; m++)
-                    if (4 * k + m < 14) madw(G[k], acc[4 * k + m][c], 1 << (8 * m));
+                nx[k] = vx.get(vr, k);
+                tree_hi(vm, nx[k].x, TREE_V1);
+                tree_hi(vm, nx[k].y, TREE_V1);
             }
-            // (G0 + G1 2^32 + G2 2^64 + G3 2^96) >> 48, nested floors
-            const int64_t lo = (G[0] >> 32) + G[1];
-            const int64_t dot = (int64_t)((uint64_t)(lo >> 16) + ((uint64_t)G[2] << 16) + ((uint64_t)G[3] << 48));
-            const int t = t0 + gq + (c < 2 ? 0 : 8), col = nt * 8 + 2 * tq + (c & 1);
-            sc[(size_t)col * a.Ts + t] = tree_scale(dot, (uint64_t)a.scale);
+            const int t1 = t0 + tg_n * 4;   // the next four are on their way meanwhile
+            vx.load(vr, t1 + tq, vd);
+#pragma unroll
+            for (int cb = 0; cb < CB; cb++) {
+                p[cb] = pn[cb];
+                pn[cb] = pp[cb][min(t1, (Tl - 1) & ~3) + tq];
+            }
+            if (__any_sync(0xffffffffu, vm >= 2 * TREE_V1)) {   // 8 p n for values beyond the chain
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int64_t n0 = (nx[k].x >> 51) + (nx[k].x >> 50 & 1), n1 = (nx[k].y >> 51) + (nx[k].y >> 50 & 1);
+                    nx[k].x = (int64_t)((uint64_t)nx[k].x << 13) >> 13;
+                    nx[k].y = (int64_t)((uint64_t)nx[k].y << 13) >> 13;
+                    // the other lanes' columns of this position too: p from the lane that holds it
+#pragma unroll
+                    for (int cb = 0; cb < CB; cb++)
+                        for (int i = 0; i < 8; i++) {
+                            const uint64_t p8 = (uint64_t)(__shfl_sync(0xffffffffu, p[cb], i * 4 + tq) * 0x1p51);
+                            unsigned long long *dst = red + (pc + cb * 8 + i) * hdp + db + 16 * k + 2 * gq;
+                            if (n0 && t0 + tq < Tl) atomicAdd(dst, (unsigned long long)(p8 * (uint64_t)n0));
+                            if (n1 && t0 + tq < Tl) atomicAdd(dst + 1, (unsigned long long)(p8 * (uint64_t)n1));
+                        }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const double v0 = __longlong_as_double((long long)((uint64_t)nx[k].x + TREE_AB)) - TREE_A;
+                const double v1 = __longlong_as_double((long long)((uint64_t)nx[k].y + TREE_AB)) - TREE_A;
+#pragma unroll
+                for (int cb = 0; cb < CB; cb++) {
+                    dmma_rd(f[cb][2 * k][0], f[cb][2 * k][1], p[cb], v0);
+                    dmma_rd(f[cb][2 * k + 1][0], f[cb][2 * k + 1][1], p[cb], v1);
+                }
+            }
         }
+    }
+    // partial outputs of the tg_n position groups meet in shared memory, group after group
+    const int od = db + 4 * tq;   // tile k, output j: + 16 (k >> 1) + (k & 1) + 2 j
+    for (int turn = 0; turn < tg_n; turn++) {
+        __syncthreads();
+        if (on && tg == turn)
+#pragma unroll
+            for (int cb = 0; cb < CB; cb++) {
+                unsigned long long *dst = red + (pc + cb * 8 + gq) * hdp + od;
+#pragma unroll
+                for (int k = 0; k < 8; k += 2) {   // tiles k, k + 1: four outputs in a row
+                    ulonglong2 *q = reinterpret_cast<ulonglong2 *>(dst + 8 * k);
+                    ulonglong2 u = q[0], w = q[1];
+                    u.x += (unsigned long long)__double_as_longlong(f[cb][k][0]) - TREE_AB;
+                    u.y += (unsigned long long)__double_as_longlong(f[cb][k + 1][0]) - TREE_AB;
+                    w.x += (unsigned long long)__double_as_longlong(f[cb][k][1]) - TREE_AB;
+                    w.y += (unsigned long long)__double_as_longlong(f[cb][k + 1][1]) - TREE_AB;
+                    q[0] = u;
+                    q[1] = w;
+                }
+            }
     }
     __syncthreads();
-
-    // ---- 2. maxima, exponentials, sums: a warp a column
-    auto sees = [&](int node, int t) {   // local position t
-        const int j = tb + t - s.len;
-        return t < Tl && (j < 0 || (anc[node][j >> 5] >> (j & 31) & 1));
-    };
-    auto cluster_wait = [&]() {
-        if (a.cs > 1) cg::this_cluster().sync();
-        else __syncthreads();
-    };
-    for (int col = warp; col < cols; col += 8) {
-        const int node = (c0 + col) / grp;
-        int64_t m = INT64_MIN;
-        for (int t = lane; t < Tl; t += 32)
-            if (sees(node, t)) m = max(m, sc[(size_t)col * a.Ts + t]);
-        for (int k = 16; k >= 1; k >>= 1) m = max(m, (int64_t)__shfl_xor_sync(0xffffffffu, m, k));
-        if (lane == 0) cmax[col] = m;
+    for (int e = tid; e < cols * hdp; e += 256) {
+        const int col = e / hdp, d = e - col * hdp, cc = c0 + col;
+        if (d < hd && red[e])
+            atomicAdd(reinterpret_cast<unsigned long long *>(a.out) +
+                          ((size_t)(s.row0 + cc / grp) * a.nh + g * grp + cc % grp) * hd + d, red[e]);
     }
-    cluster_wait();
-    if (tid < cols) {
-        int64_t m = cmax[tid];
-        for (int r = 0; r < a.cs && a.cs > 1; r++)
-            m = max(m, cg::this_cluster().map_shared_rank(cmax, r)[tid]);
-        gmax[tid] = m;
-    }
-    __syncthreads();
-    int weird = 0;
-    for (int col = warp; col < cols; col += 8) {
-        const int64_t m = gmax[col];
-        int64_t *row = sc + (size_t)col * a.Ts;
-        const int node = (c0 + col) / grp;
-        uint64_t sum = 0;
-        for (int t = lane; t < Tp; t += 32) {
-            int64_t e = 0;
-            if (sees(node, t)) {
-                const uint64_t d = (uint64_t)m - (uint64_t)row[t];
-                if ((int64_t)d < 0) {   // the difference wraps: the reference's value all the same
-                    weird = 1;
-                    e = d_safe_exp((int64_t)(0 - d));
-                } else if (d <= 10 * (uint64_t)IQ_ONE) {
-                    e = tree_exp(d);
-                }
-            }
-            row[t] = e;
-            sum += (uint64_t)e;
-        }
-        for (int k = 16; k >= 1; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-        if (lane == 0) csum[col] = (int64_t)sum;
-    }
-    if (weird) weird_s = 1;
-    cluster_wait();
-    weird = weird_s;
-    for (int r = 0; r < a.cs && a.cs > 1; r++) weird |= *cg::this_cluster().map_shared_rank(&weird_s, r);
-    if (tid < cols) {
-        uint64_t S = (uint64_t)csum[tid];
-        if (a.cs > 1) {
-            S = 0;
-            for (int r = 0; r < a.cs; r++) S += (uint64_t)cg::this_cluster().map_shared_rank(csum, r)[tid];
-        }
-        gsum[tid] = (int64_t)S;
-        ginv[tid] = 281474976710656.0 / (double)(int64_t)S;
-    }
-    __syncthreads();
-    for (int col = warp; col < NC; col += 8) {
-        int64_t *row = sc + (size_t)col * a.Ts;
-        if (col >= cols) {
-            for (int t = lane; t < Tp; t += 32) row[t] = 0;
-            continue;
-        }
-        const int64_t S = gsum[col];
-        const double inv = ginv[col];
-        for (int t = lane; t < Tp; t += 32) {
-            const int64_t e = row[t];
-            if (weird) row[t] = S > 0 ? d_div(e, S) : e;
-            else row[t] = __double_as_longlong(tree_u52(e ? tree_prob(e, S, inv) : 0));
-        }
-    }
-
-    // ---- 3. probabilities times values
-    const int hdp = tree_hdp(hd), TV = TREE_V / hdp, nd = hdp >> 6;
-    double *vt = reinterpret_cast<double *>(side);                                    // [TV][hdp]
-    unsigned long long *part = reinterpret_cast<unsigned long long *>(side + TREE_V * 8);   // [NC][hdp]
-    for (int e = tid; e < NC * hdp; e += 256) part[e] = 0;
-    const int units = NT * nd, tg_n = 8 / units;      // units <= 8
-    const int unit = warp % units, tg = warp / units;   // warps beyond units * tg_n idle
-    const int pc = (unit / nd) * 8 + (lane >> 4) * 4, pd = (unit % nd) * 64 + (lane & 15) * 2;
-    const int per_t = (TV + tg_n - 1) / tg_n;
-    double o[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = TREE_A;
-    const bool on = tg < tg_n && (unit / nd) * 8 < cols;
-    for (int st = 0; st < Tl; st += TV) {
-        int64_t x[4][4];
-        int big = 0;   // 1: beyond the single chain, 2: beyond both
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int e = (k * 256 + tid) * 4, t = e / hdp, d = e - t * hdp;
-            x[k][0] = x[k][1] = x[k][2] = x[k][3] = 0;
-            if (st + t < Tl) tree_at4<PK>(a, true, (v0 + st + t) * a.c.nkv + g, d, x[k]);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int64_t lim = (1ll << 51) - (1 << 16);
-                if ((uint64_t)(x[k][i] + lim) > (uint64_t)(2 * lim)) big |= 1;
-                if ((uint64_t)(x[k][i] + (1ll << 54)) >= (1ull << 55)) big |= 2;
-            }
-        }
-        // the previous tile is consumed
-        big = __syncthreads_or(big & 2) ? 2 : __syncthreads_or(big) ? 1 : 0;
-        const int n = min(TV, Tl - st);
-        if (big == 2 || weird) {   // term by term
-            int64_t *vi = reinterpret_cast<int64_t *>(vt);
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) vi[(k * 256 + tid) * 4 + i] = x[k][i];
-            __syncthreads();
-            for (int e = tid; e < cols * hdp; e += 256) {
-                const int col = e / hdp, d = e - col * hdp;
-                uint64_t acc = 0;
-                for (int t = 0; t < n; t++) {
-                    const int64_t pv = sc[(size_t)col * a.Ts + st + t];
-                    const int64_t p = weird ? pv : (int64_t)((uint64_t)__double_as_longlong(
-                                                        __longlong_as_double(pv) + TREE_M) & 0xFFFFFFFFFFFFFull);
-                    acc += (uint64_t)d_mul(p, vi[t * hdp + d]);
-                }
-                atomicAdd(&part[e], (unsigned long long)acc);
-            }
-            continue;
-        }
-        for (int half = 0; half <= big; half++) {   // v, or its low part f, then n = (v - f) / 2^51
-            if (half) __syncthreads();
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    int64_t v = x[k][i];
-                    if (big) {
-                        const int64_t f = (int64_t)((uint64_t)v << 13) >> 13;
-                        v = half ? (v - f) >> 51 : f;
-                    }
-                    const double w = __longlong_as_double((long long)((uint64_t)v + TREE_AB)) - TREE_A;
-                    vt[(k * 256 + tid) * 4 + i] = half ? w : w * 0x1p-48;
-                }
-            __syncthreads();
-            if (!on) continue;
-            const int te = min(n, (tg + 1) * per_t);
-            const double *pp = reinterpret_cast<const double *>(sc) + (size_t)pc * a.Ts + st;
-            if (!half) {
-#pragma unroll 2
-                for (int t = tg * per_t; t < te; t++) {
-                    const double2 va = *reinterpret_cast<const double2 *>(vt + t * hdp + pd);
-                    const double2 vb = *reinterpret_cast<const double2 *>(vt + t * hdp + pd + 32);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const double p = pp[(size_t)i * a.Ts + t];
-                        o[i][0] = __fma_rd(p, va.x, o[i][0]);
-                        o[i][1] = __fma_rd(p, va.y, o[i][1]);
-                        o[i][2] = __fma_rd(p, vb.x, o[i][2]);
-                        o[i][3] = __fma_rd(p, vb.y, o[i][3]);
-                    }
-                }
-            } else {   // 8 sum p n, exact: below 2^48 2^3
-                double m[4][4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) m[i][0] = m[i][1] = m[i][2] = m[i][3] = TREE_A;
-                for (int t = tg * per_t; t < te; t++) {
-                    const double2 va = *reinterpret_cast<const double2 *>(vt + t * hdp + pd);
-                    const double2 vb = *reinterpret_cast<const double2 *>(vt + t * hdp + pd + 32);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const double p = pp[(size_t)i * a.Ts + t];
-                        m[i][0] = __fma_rn(p, va.x, m[i][0]);
-                        m[i][1] = __fma_rn(p, va.y, m[i][1]);
-                        m[i][2] = __fma_rn(p, vb.x, m[i][2]);
-                        m[i][3] = __fma_rn(p, vb.y, m[i][3]);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        atomicAdd(&part[(pc + i) * hdp + pd + (k & 1) + (k >> 1) * 32],
-                                  ((unsigned long long)__double_as_longlong(m[i][k]) - TREE_AB) << 3);
-            }
-        }
-    }
-    __syncthreads();
-    if (on)
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                atomicAdd(&part[(pc + i) * hdp + pd + (k & 1) + (k >> 1) * 32],
-                          (unsigned long long)__double_as_longlong(o[i][k]) - TREE_AB);
-    cluster_wait();
-    for (int e = rank * 256 + tid; e < cols * hdp; e += 256 * a.cs) {
-        const int col = e / hdp, d = e - col * hdp;
-        if (d >= hd) continue;
-        uint64_t t = 0;
-        if (a.cs == 1) t = part[e];
-        else
-            for (int r = 0; r < a.cs; r++) t += cg::this_cluster().map_shared_rank(part, r)[e];
-        a.out[((size_t)(s.row0 + (c0 + col) / grp) * a.nh + g * grp + (c0 + col) % grp) * hd + d] = (int64_t)t;
-    }
-    if (a.cs > 1) cg::this_cluster().sync();   // the others may still read this CTA's part
 }
 
 }  // namespace iq
