@@ -94,11 +94,15 @@ static void tree_plan(TreeArgs *a) {
     // columns of all sequences, on average over them
     const int64_t avg = std::max<int64_t>(1, (int64_t)a->rows * grp / a->n_seq);
     const int nt = cols <= 8 ? 1 : 2, blocks = (int)((cols + 8 * nt - 1) / (8 * nt));
-    a->tiles = (a->max_len + 127) / 128;
-    // up to 8 blocks share the key planes, fewer where that leaves SMs without a CTA
-    const int64_t pairs = (int64_t)a->n_seq * a->c.nkv, have = pairs * a->tiles;
+    // up to 8 blocks share the key planes, fewer where that leaves SMs without a CTA;
+    // a single block's CTA walks over up to 8 tiles on the same terms
+    const int tiles = (a->max_len + 127) / 128;
+    const int64_t pairs = (int64_t)a->n_seq * a->c.nkv;
     a->passes = 8;
-    while (a->passes > 1 && have * ((avg + 8 * nt * a->passes - 1) / (8 * nt * a->passes)) < 4 * sms) a->passes /= 2;
+    while (a->passes > 1 && pairs * tiles * ((avg + 8 * nt * a->passes - 1) / (8 * nt * a->passes)) < 4 * sms) a->passes /= 2;
+    a->tpc = blocks == 1 ? 8 : 1;
+    while (a->tpc > 1 && pairs * ((tiles + a->tpc - 1) / a->tpc) < 6 * sms) a->tpc /= 2;
+    a->tiles = (tiles + a->tpc - 1) / a->tpc;
     a->groups = (blocks + a->passes - 1) / a->passes;
     a->cg = cols > 16 && a->c.hd <= 128 ? 2 : 1;
     const int per = cols <= 8 ? 8 : 16 * a->cg;

@@ -33,6 +33,7 @@
 //    takes 64 terms). Six integer instructions a term is what the remainder form
 //    of k_attn_pv_tc costs.
 #pragma once
+#include <type_traits>
 #include "iq_ops.cuh"
 
 namespace iq {
@@ -48,7 +49,7 @@ struct TreeArgs {
     int64_t qs, scale;
     int64_t *sc;    // workspace [rows][nh][Tw]: scores, then p 2^-48 as doubles
     int Tw, vec, vecq;
-    int tiles, groups, passes;   // k_tree_scores: position tiles, groups of column blocks, blocks a group
+    int tiles, tpc, groups, passes;   // k_tree_scores: CTAs along the positions, tiles each, groups of column blocks, blocks a group
     int chunk, chunks, cg, cblocks;   // k_tree_pv: positions a CTA, their number, groups of 8 CB columns a block, blocks
 };
 
@@ -149,21 +150,22 @@ template <> struct TreeKeys<true> {
         for (int i = 0; i < 4; i++) o[i] = kv_value((q[w] >> (8 * i)) & 0xFF, m, r.bits);
     }
 };
-// A lane's values of one position: pairs at d0 + 16 k + 2 gq, k < 4, as loaded.
+// A lane's values of one position, as loaded: pairs at d + 16 k, k < 4 (d in the
+// 64-wide block from db on; beyond hd anything).
 template <bool PK> struct TreeVals;
 template <> struct TreeVals<false> {
     longlong2 x[4];
-    __device__ __forceinline__ void load(const TreeRows &r, int t, const int (&d)[4]) {
-        const char *p = r.x + (size_t)(uint32_t)min(t, r.T - 1) * r.rs;
-        if (r.wide) {
-#pragma unroll
-            for (int k = 0; k < 4; k++) x[k] = *reinterpret_cast<const longlong2 *>(p + d[k] * 8);
+    __device__ __forceinline__ void load(const TreeRows &r, int t, int d, int db) {
+        const int64_t *p = reinterpret_cast<const int64_t *>(r.x + (size_t)(uint32_t)min(t, r.T - 1) * r.rs) + d;
+        if (r.wide) {   // hd a multiple of 32: a block is whole or half
+            const longlong2 *q = reinterpret_cast<const longlong2 *>(p), *q2 = r.hd - db >= 64 ? q + 16 : q;
+            x[0] = q[0];
+            x[1] = q[8];
+            x[2] = q2[0];
+            x[3] = q2[8];
         } else {
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int64_t *e = reinterpret_cast<const int64_t *>(p) + d[k];
-                x[k] = make_longlong2(e[0], e[d[k] + 1 < r.hd]);
-            }
+            for (int k = 0; k < 4; k++) x[k] = make_longlong2(p[min(16 * k, r.hd - 1 - d)], p[min(16 * k + 1, r.hd - 1 - d)]);
         }
     }
     __device__ __forceinline__ longlong2 get(const TreeRows &, int k) const { return x[k]; }
@@ -171,19 +173,19 @@ template <> struct TreeVals<false> {
 template <> struct TreeVals<true> {
     ushort2 q[4];
     int64_t m;
-    __device__ __forceinline__ void load(const TreeRows &r, int t, const int (&d)[4]) {
+    __device__ __forceinline__ void load(const TreeRows &r, int t, int d, int db) {
         t = min(t, r.T - 1);
-        const char *p = r.x + (size_t)(uint32_t)t * r.rs;
+        const uint16_t *p = reinterpret_cast<const uint16_t *>(r.x + (size_t)(uint32_t)t * r.rs) + d;
         m = __ldg(r.mag + (size_t)(uint32_t)t * r.ms);
         if (r.wide) {
-#pragma unroll
-            for (int k = 0; k < 4; k++) q[k] = *reinterpret_cast<const ushort2 *>(p + d[k] * 2);
+            const ushort2 *u = reinterpret_cast<const ushort2 *>(p), *u2 = r.hd - db >= 64 ? u + 16 : u;
+            q[0] = u[0];
+            q[1] = u[8];
+            q[2] = u2[0];
+            q[3] = u2[8];
         } else {
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const uint16_t *e = reinterpret_cast<const uint16_t *>(p) + d[k];
-                q[k] = make_ushort2(e[0], e[d[k] + 1 < r.hd]);
-            }
+            for (int k = 0; k < 4; k++) q[k] = make_ushort2(p[min(16 * k, r.hd - 1 - d)], p[min(16 * k + 1, r.hd - 1 - d)]);
         }
     }
     __device__ __forceinline__ longlong2 get(const TreeRows &r, int k) const {
@@ -211,14 +213,14 @@ __device__ __forceinline__ void dmma_rd(double &c0, double &c1, double x, double
                  : "+d"(c0), "+d"(c1) : "d"(x), "d"(y));
 }
 
-// 16 consecutive bytes of each of the 8 planes of 16 elements (offset binary)
-__device__ __forceinline__ void tree_planes(const int64_t (&x)[16], uint32_t (&o)[4][8]) {
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-        const int64_t e[4] = {x[4 * w], x[4 * w + 1], x[4 * w + 2], x[4 * w + 3]};
-        byte_planes4(e, o[w]);
-        o[w][7] ^= 0x80808080u;
-    }
+// Byte planes of four elements' words w: o[i] holds byte i of w[0] .. w[3].
+__device__ __forceinline__ void tree_bytes4(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t (&o)[4]) {
+    const uint32_t x01 = __byte_perm(w0, w1, 0x5140), x23 = __byte_perm(w2, w3, 0x5140);
+    const uint32_t y01 = __byte_perm(w0, w1, 0x7362), y23 = __byte_perm(w2, w3, 0x7362);
+    o[0] = __byte_perm(x01, x23, 0x5410);
+    o[1] = __byte_perm(x01, x23, 0x7632);
+    o[2] = __byte_perm(y01, y23, 0x5410);
+    o[3] = __byte_perm(y01, y23, 0x7632);
 }
 // byte offset of 16-byte piece c of row r in a tile of 128-byte rows with the 128-byte swizzle
 __device__ __forceinline__ uint32_t tree_sw(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
@@ -246,12 +248,29 @@ __device__ __forceinline__ void tree_hi(uint32_t &m, int64_t x, uint32_t b) { m 
 // Work that the kernel launched before this one may still be doing is waited for here.
 __device__ __forceinline__ void tree_prev_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// fp_mul(s, c) for 0 <= c <= 2^48 (the score scale)
-__device__ __forceinline__ int64_t tree_scale(int64_t s, uint64_t c) {
-    const uint32_t sl = (uint32_t)s, cl = (uint32_t)c, ch = (uint32_t)(c >> 32);
-    const int64_t sh = s >> 32;
-    const int64_t t = (int64_t)((uint64_t)sl * ch + __umulhi(sl, cl)), u = sh * (int64_t)cl;
-    return (int64_t)((uint64_t)(sh * (int64_t)ch) << 16) + (t >> 16) + (u >> 16) + (((t & 0xFFFF) + (u & 0xFFFF)) >> 16);
+// fp_mul(s, c) for 0 <= c <= 2^48 (the score scale). With s = sh 2^32 + sl and c = ch 2^32 + cl =
+// ch' 2^32 + cl', cl' signed (so that |sh cl'| <= 2^62):
+// floor(s c / 2^48) = sh ch' 2^16 + floor((sh cl' + floor(sl c / 2^32)) / 2^16).
+struct TreeScale {
+    uint32_t ch, cl;
+    int hs, ls;   // ch', cl'
+};
+__device__ __forceinline__ TreeScale tree_scale_of(int64_t c) {
+    TreeScale r;
+    r.ch = (uint32_t)((uint64_t)c >> 32);
+    r.cl = (uint32_t)c;
+    r.ls = (int)r.cl;
+    r.hs = (int)r.ch + (r.ls < 0);
+    return r;
+}
+__device__ __forceinline__ int64_t tree_scale(int64_t s, const TreeScale &c) {
+    const uint32_t sl = (uint32_t)s;
+    const int sh = (int)(s >> 32);
+    uint64_t t = __umulhi(sl, c.cl);
+    madu(t, sl, c.ch);
+    int64_t u = (int64_t)t;
+    madw(u, sh, c.ls);
+    return (u >> 16) + (int64_t)((uint64_t)((int64_t)sh * c.hs) << 16);
 }
 
 // ---------------------------------------------------------------- 1. scores
@@ -260,8 +279,9 @@ __device__ __forceinline__ int64_t tree_scale(int64_t s, uint64_t c) {
 __host__ __device__ constexpr size_t tree_b_bytes(int NT, int hd) { return (size_t)((hd + 127) / 128) * 64 * NT * 128; }
 __host__ __device__ constexpr size_t tree_scores_smem(int NT, int hd) { return 1024 + TREE_A_BYTES + tree_b_bytes(NT, hd); }
 
-// A CTA takes 128 positions of one (sequence, kv head) and up to a.passes blocks of
-// NC = 8 NT columns. With hd <= 64 the key planes are made once for all its blocks.
+// A CTA takes a.tpc tiles of 128 positions of one (sequence, kv head) and up to
+// a.passes blocks of NC = 8 NT columns. With hd <= 64 the key planes of a tile are made
+// once for all its blocks, with one block the query planes once for all its tiles.
 // Two CTAs an SM (three with 8 columns) overlap one another's loads, products
 // and epilogues; TMEM holds 128 NT columns a CTA.
 template <int NT, bool PK>
@@ -269,7 +289,8 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __gr
     extern __shared__ __align__(16) char tree_smem[];
     constexpr int NC = 8 * NT, HC = NC / 2;
     __shared__ int64_t ksum[128];              // sum of a position's key
-    __shared__ unsigned long long qsum[NC];
+    __shared__ unsigned long long qsum[NC];    // 2^15 times the sum of a column's query
+    __shared__ int64_t *scol[NC];              // a column's row of scores
     __shared__ __align__(8) uint64_t mbar[2];  // the products of a step's key planes are done
     __shared__ uint32_t tmem_s;
     const int tile = blockIdx.x % a.tiles, rest = blockIdx.x / a.tiles;
@@ -278,17 +299,17 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __gr
     const int grp = a.nh / a.c.nkv, hd = a.c.hd, KS = (hd + 31) / 32;
     TreeSeq s;
     if (!tree_seq(a, b, s)) return;
-    const int cols = s.n * grp, T = s.len + s.n, tb = tile * 128, Tl = min(128, T - tb);
+    const int cols = s.n * grp, T = s.len + s.n, tb0 = tile * a.tpc * 128, te = min(T, tb0 + a.tpc * 128);
     const int p0 = group * a.passes, p1 = min(p0 + a.passes, (cols + NC - 1) / NC);   // column blocks
-    if (Tl <= 0 || p0 >= p1) return;
+    if (tb0 >= te || p0 >= p1) return;
     char *const sA = tree_smem + ((1024 - (smem_u32(tree_smem) & 1023)) & 1023), *const sB = sA + TREE_A_BYTES;
 
     // conversion: two threads a position; eight lanes in a row take positions whose
     // swizzles differ, so that their 16-byte stores meet no bank twice
     const int cq = lane >> 1, ch = lane & 1, cp = warp * 16 + ((cq & 8) | ((cq & 3) << 1) | ((cq >> 2) & 1));
-    const TreeRows kr = tree_rows<PK>(a, false, ((size_t)s.sq * a.c.max_seq + tb) * a.c.nkv + g, Tl);
+    const TreeRows kr = tree_rows<PK>(a, false, (size_t)s.sq * a.c.max_seq * a.c.nkv + g, T);
     TreeKeys<PK> kx;
-    if (cp < Tl) kx.load(kr, cp, 0, ch);
+    if (tb0 + cp < te) kx.load(kr, tb0 + cp, 0, ch);
     if (warp == 0) tmem_alloc(&tmem_s, 128 * NT);
     if (tid == 0) {
         mbar_init(&mbar[0], 1);
@@ -301,7 +322,10 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __gr
     // epilogue: TMEM lane quadrant warp & 3, half of the columns warp >> 2
     const uint32_t tmem = tmem_s, tlane = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (warp >> 2) * HC;
     const int ep = (warp & 3) * 32 + lane;
-    int batch = 0;   // steps issued; step n uses half n & 1 of the key planes
+    const TreeScale scale = tree_scale_of(a.scale);
+    int batch = 0, made_at = 0;   // steps issued; half of the key planes that a tile's first step went to
+    for (int tb = tb0; tb < te; tb += 128) {
+    const int Tl = min(128, te - tb);
     unsigned long long sum = 0;
     for (int pass = p0; pass < p1; pass++) {
         // the diagonals that plane 0 does not start
@@ -310,48 +334,52 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __gr
 #pragma unroll
             for (int c = 0; c < HC; c += 4) tmem_zero4(tlane + sd * NC + c);
         tmem_st_wait();
-        // query planes of the block
         const int c0 = pass * NC, nc = min(NC, cols - c0);
-        if (tid < NC) qsum[tid] = 0;
-        __syncthreads();
-        for (int e = tid; e < NC * KS * 2; e += 256) {   // (column, step, half)
-            const int h = e & 1, col = (e >> 1) % NC, ks = (e >> 1) / NC, cc = c0 + min(col, nc - 1);
-            const int64_t *q = a.q + (int64_t)(s.row0 + cc / grp) * a.qs + (int64_t)(g * grp + cc % grp) * hd;
-            int64_t x[16];
-            if (a.vecq) {   // whole steps, aligned pairs
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const longlong2 u = __ldg(reinterpret_cast<const longlong2 *>(q + ks * 32 + tree_d<PK>(h, i)));
-                    x[i] = u.x;
-                    x[i + 1] = u.y;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int d = ks * 32 + tree_d<PK>(h, i);
-                    x[i] = d < hd ? q[d] : 0;
-                }
+        if (p1 - p0 > 1 || tb == tb0) {   // query planes of the block: a thread four d of one 16-byte piece
+            if (tid < NC) {
+                const int cc = c0 + min(tid, nc - 1), nd = cc / grp;
+                scol[tid] = a.sc + ((size_t)(s.row0 + nd) * a.nh + g * grp + cc - nd * grp) * a.Tw;
             }
-            unsigned long long qs = 0;
+            for (int e = tid; e < NC * KS * 8; e += 256) {   // (column, step, half, quad): a column's 8 KS threads in a row
+                const int w = e & 3, h = (e >> 2) & 1, ks = (e >> 3) % KS, col = (e >> 3) / KS;
+                const int cc = c0 + min(col, nc - 1), nd = cc / grp;
+                const int64_t *q = a.q + (int64_t)(s.row0 + nd) * a.qs + (int64_t)(g * grp + cc - nd * grp) * hd + ks * 32;
+                int64_t x[4];
+                if (a.vecq) {   // whole steps, aligned pairs
+                    const longlong2 u = __ldg(reinterpret_cast<const longlong2 *>(q + tree_d<PK>(h, 4 * w)));
+                    const longlong2 v = __ldg(reinterpret_cast<const longlong2 *>(q + tree_d<PK>(h, 4 * w + 2)));
+                    x[0] = u.x; x[1] = u.y; x[2] = v.x; x[3] = v.y;
+                } else {
 #pragma unroll
-            for (int i = 0; i < 16; i++) qs += (unsigned long long)x[i];
-            uint32_t o[4][8];
-            tree_planes(x, o);
-            if (!a.vecq)   // beyond hd x_u is 0, not 2^63: nothing meets whatever the keys hold there
+                    for (int i = 0; i < 4; i++) x[i] = ks * 32 + tree_d<PK>(h, 4 * w + i) < hd ? q[tree_d<PK>(h, 4 * w + i)] : 0;
+                }
+                uint32_t o[8];
+                byte_planes4(x, o);
+                o[7] ^= 0x80808080u;
+                if (!a.vecq)   // beyond hd x_u is 0, not 2^63: nothing meets whatever the keys hold there
 #pragma unroll
-                for (int i = 0; i < 16; i++)
-                    if (ks * 32 + tree_d<PK>(h, i) >= hd) o[i >> 2][7] &= ~(0xFFu << (8 * (i & 3)));
-            char *tile_b = sB + (size_t)(ks >> 2) * 64 * NT * 128;
+                    for (int i = 0; i < 4; i++)
+                        if (ks * 32 + tree_d<PK>(h, 4 * w + i) >= hd) o[7] &= ~(0xFFu << (8 * i));
+                char *dst = sB + (size_t)(ks >> 2) * 64 * NT * 128 + w * 4;
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                *reinterpret_cast<uint4 *>(tile_b + tree_sw(j * NC + col, (ks & 3) * 2 + h)) =
-                    make_uint4(o[0][j], o[1][j], o[2][j], o[3][j]);
-            atomicAdd(&qsum[col], qs);
+                for (int j = 0; j < 8; j++)
+                    *reinterpret_cast<uint32_t *>(dst + tree_sw(j * NC + col, (ks & 3) * 2 + h)) = o[j];
+            }
+            for (int col = warp; col < NC; col += 8) {   // a warp a column's sum
+                const int cc = c0 + min(col, nc - 1), nd = cc / grp;
+                const int64_t *q = a.q + (int64_t)(s.row0 + nd) * a.qs + (int64_t)(g * grp + cc - nd * grp) * hd;
+                unsigned long long qs = 0;
+                for (int d = lane; d < hd; d += 32) qs += (unsigned long long)__ldg(q + d);
+                for (int m = 16; m >= 1; m >>= 1) qs += __shfl_xor_sync(0xffffffffu, qs, m);
+                if (lane == 0) qsum[col] = qs << 15;
+            }
         }
         const bool made = KS <= 2 && pass > p0;   // the key planes stand
         for (int ks = 0; ks < KS; ks++, batch++) {
-            char *const A = sA + (size_t)(batch & 1) * 32768;
+            // the half that this step's planes are in: batch & 1, or, when they stand, where they were made
+            const int half = made ? (made_at + ks) & 1 : batch & 1;
             if (!made) {
+                if (ks == 0) made_at = half;
                 if (batch >= 2) mbar_wait(&mbar[batch & 1], (uint32_t)((batch >> 1) - 1) & 1u);
                 if (cp < Tl) {
                     int64_t x[16];
@@ -362,17 +390,34 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __gr
 #pragma unroll
                         for (int i = 0; i < 4; i++) x[4 * w + i] = e[i];
                     }
+                    if (pass == p0)
 #pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (kr.wide || ks * 32 + tree_d<PK>(ch, i) < hd) sum += (unsigned long long)x[i];
-                    // the next step's keys are on their way meanwhile
-                    if (ks + 1 < KS || (KS > 2 && pass + 1 < p1)) kx.load(kr, cp, ks + 1 < KS ? (ks + 1) * 32 : 0, ch);
-                    uint32_t o[4][8];
-                    tree_planes(x, o);
+                        for (int i = 0; i < 16; i++)
+                            if (kr.wide || ks * 32 + tree_d<PK>(ch, i) < hd) sum += (unsigned long long)x[i];
+                    char *const A = sA + (size_t)half * 32768;
 #pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        *reinterpret_cast<uint4 *>(A + (j >> 2) * 16384 + tree_sw(cp, (j & 3) * 2 + ch)) =
-                            make_uint4(o[0][j], o[1][j], o[2][j], o[3][j]);
+                    for (int hw = 0; hw < 2; hw++) {   // planes 0-3 from the low words, 4-7 from the high ones
+                        uint32_t o[4][4];
+#pragma unroll
+                        for (int w = 0; w < 4; w++) {
+                            tree_bytes4((uint32_t)((uint64_t)x[4 * w] >> (32 * hw)), (uint32_t)((uint64_t)x[4 * w + 1] >> (32 * hw)),
+                                        (uint32_t)((uint64_t)x[4 * w + 2] >> (32 * hw)),
+                                        (uint32_t)((uint64_t)x[4 * w + 3] >> (32 * hw)), o[w]);
+                            if (hw) o[w][3] ^= 0x80808080u;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            *reinterpret_cast<uint4 *>(A + hw * 16384 + tree_sw(cp, j * 2 + ch)) =
+                                make_uint4(o[0][j], o[1][j], o[2][j], o[3][j]);
+                    }
+                }
+                // the next step's keys are on their way meanwhile
+                if (ks + 1 < KS) {
+                    if (cp < Tl) kx.load(kr, tb + cp, (ks + 1) * 32, ch);
+                } else if (KS > 2 && pass + 1 < p1) {
+                    if (cp < Tl) kx.load(kr, tb + cp, 0, ch);
+                } else if (tb + 128 + cp < te) {
+                    kx.load(kr, tb + 128 + cp, 0, ch);
                 }
                 if (ks == KS - 1 && pass == p0) {
                     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
@@ -386,11 +431,11 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __gr
             }
             if (tid == 0) {
                 tc_fence_after();
-                const char *Am = made && KS == 1 ? sA : A;
+                const char *A = sA + (size_t)half * 32768;
                 const uint64_t bd = smem_desc_sw128(sB + (size_t)(ks >> 2) * 64 * NT * 128) + 2 * (ks & 3);
 #pragma unroll
                 for (int i = 0; i < 8; i++)
-                    tc_mma_i8(tmem + i * NC, smem_desc_sw128(Am + (i >> 2) * 16384) + 2 * (i & 3), bd,
+                    tc_mma_i8(tmem + i * NC, smem_desc_sw128(A + (i >> 2) * 16384) + 2 * (i & 3), bd,
                               idesc_i8(false, false, 128, 8 * NC), ks > 0 || i > 0);
                 tc_commit(&mbar[batch & 1]);
             }
@@ -398,7 +443,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __gr
         // (a wait that runs out has recorded IQ_ERR_TIMEOUT; the outputs then mean nothing)
         mbar_wait(&mbar[(batch - 1) & 1], (uint32_t)((batch - 1) >> 1) & 1u);
         tc_fence_after();
-        const unsigned long long kp = (unsigned long long)ksum[ep];
+        const unsigned long long kp = 0 - ((unsigned long long)ksum[ep] << 15);
 #pragma unroll
         for (int c = 0; c < HC; c += 4) {
             uint32_t v[14][4];
@@ -407,25 +452,25 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __gr
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                uint64_t G[4];
+                // bits 48 .. 111 of sum_s v_s 2^(8s): below 2^48 a chain of floors leaves the
+                // carry; above, 2^32 v_10 and on need their low words only
+                uint32_t lo = v[0][i];
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    G[k] = v[4 * k][i];
-#pragma unroll
-                    for (int m = 1; m < 4; m++)
-                        if (4 * k + m < 14) madu(G[k], v[4 * k + m][i], 1u << (8 * m));
-                }
-                // (G0 + G1 2^32 + G2 2^64 + G3 2^96) >> 48, nested floors, less 2^15 (sum q + sum k)
-                const int col = (warp >> 2) * HC + c + i, cc = c0 + col;
-                const uint64_t dot = (((G[0] >> 32) + G[1]) >> 16) + (G[2] << 16) + (G[3] << 48) - ((qsum[col] + kp) << 15);
-                if (ep < Tl && col < nc)
-                    a.sc[((size_t)(s.row0 + cc / grp) * a.nh + g * grp + cc % grp) * a.Tw + tb + ep] =
-                        tree_scale((int64_t)dot, (uint64_t)a.scale);
+                for (int k = 1; k < 6; k++) lo = (lo >> 8) + v[k][i];
+                const uint32_t hi = v[10][i] + (v[11][i] << 8) + (v[12][i] << 16) + (v[13][i] << 24);
+                const int col = (warp >> 2) * HC + c + i;
+                uint64_t dot = kp - qsum[col] + ((uint64_t)hi << 32) + (lo >> 8);
+                madu(dot, v[6][i], 1);
+                madu(dot, v[7][i], 1 << 8);
+                madu(dot, v[8][i], 1 << 16);
+                madu(dot, v[9][i], 1 << 24);
+                if (ep < Tl && col < nc) scol[col][tb + ep] = tree_scale((int64_t)dot, scale);
             }
         }
         tc_fence_before();
-        __syncthreads();   // qsum, TMEM and the query planes are free
+        __syncthreads();   // sums, TMEM and the query planes are free
         tc_fence_after();
+    }
     }
     if (warp == 0) tmem_dealloc(tmem, 128 * NT);
 }
@@ -450,6 +495,12 @@ __device__ __forceinline__ uint64_t tree_sqr(uint64_t r) {
     madu(x, h << 8, h << 8);
     return x;
 }
+// 1 where q r + c < 0 (mod 2^64, as a signed number), else 0
+__device__ __forceinline__ uint32_t tree_more(uint64_t q, uint64_t r, uint64_t c) {
+    madu(c, (uint32_t)q, (uint32_t)r);
+    const uint32_t h = (uint32_t)(c >> 32) + (uint32_t)q * (uint32_t)(r >> 32) + (uint32_t)(q >> 32) * (uint32_t)r;
+    return h >> 31;
+}
 // fp_exp(-d) (fp_math.h:714-732) for 0 <= d <= 10
 __device__ __forceinline__ int64_t tree_exp(uint64_t d) {
     double g = __longlong_as_double((long long)(((d >> 14) + IQ_ONE) | TREE_MB));   // M + r
@@ -460,8 +511,8 @@ __device__ __forceinline__ int64_t tree_exp(uint64_t d) {
     }
     const uint64_t r = tree_sqr(tree_sqr((uint64_t)__double_as_longlong(g) & TREE_MASK));   // 2^48 <= r < 2^62.5
     // floor(2^96 / r), at most 2^48: reciprocal by two Newton steps (relative error
-    // below 2^-51), lowered by 2^-50 so that its floor is q or q - 1; the remainder
-    // (2^96 = 0 mod 2^64) tells which
+    // below 2^-51), lowered by 2^-50 so that its floor is q or q - 1; the sign of
+    // (q + 1) r - 2^96 - 1 (2^96 = 0 mod 2^64) tells which
     const double rd = (__longlong_as_double((long long)((r >> 32) | 0x4530000000000000ull)) - 19342813118337666422669312.0) +
                       __longlong_as_double((long long)((r & 0xFFFFFFFFull) | TREE_MB));
     double y;
@@ -469,7 +520,7 @@ __device__ __forceinline__ int64_t tree_exp(uint64_t d) {
     y = __fma_rn(y, __fma_rn(-rd, y, 1.0), y);
     y = __fma_rn(y, __fma_rn(-rd, y, 1.0), y);
     const uint64_t q = (uint64_t)__double_as_longlong(__fma_rd(y, 0x1p96 - 0x1p46, TREE_M)) & TREE_MASK;
-    return (int64_t)(q + (0 - q * r >= r));
+    return (int64_t)(q + tree_more(q, r, r - 1));
 }
 // 2^48 / S, lowered likewise for tree_prob
 __device__ __forceinline__ double tree_inv(int64_t S) {
@@ -477,9 +528,8 @@ __device__ __forceinline__ double tree_inv(int64_t S) {
 }
 // fp_div(e, S) 2^-48 as a double for 0 <= e <= S, 2^48 <= S < 2^63, e <= 2^48
 __device__ __forceinline__ double tree_prob(int64_t e, int64_t S, double inv) {
-    uint64_t q = (uint64_t)__double_as_longlong(__fma_rd(tree_u52((uint64_t)e), inv, TREE_M)) & TREE_MASK;
-    q += ((uint64_t)e << 48) - q * (uint64_t)S >= (uint64_t)S;
-    return tree_u52(q) * 0x1p-48;
+    const uint64_t q = (uint64_t)__double_as_longlong(__fma_rd(tree_u52((uint64_t)e), inv, TREE_M)) & TREE_MASK;
+    return tree_u52(q + tree_more(q, (uint64_t)S, (uint64_t)S - 1 - ((uint64_t)e << 48))) * 0x1p-48;
 }
 
 // A row in which a score difference wraps: fp_safe_exp of the wrapped difference, the
@@ -554,31 +604,43 @@ __global__ void __launch_bounds__(TREE_SM_T) k_tree_softmax(const __grid_constan
     for (int t0 = 0; t0 < (LONG ? T : 1); t0 += TREE_SM_T * TREE_SM_E) {
 #pragma unroll
         for (int k = 0; k < TREE_SM_E; k++) {
-            const int t = t0 + k * TREE_SM_T + tid;
-            x[k] = t < T ? row[t] : INT64_MIN;
-            if (sees(t)) m = max(m, x[k]);
+            const int tk = t0 + k * TREE_SM_T, t = tk + tid;
+            x[k] = INT64_MIN;
+            if (tk + TREE_SM_T <= s.len) {   // all before the draft
+                x[k] = row[t];
+                m = max(m, x[k]);
+            } else if (tk < T) {
+                if (t < T) x[k] = row[t];
+                if (sees(t)) m = max(m, x[k]);
+            }
         }
     }
     m = cta_max_i64(m, (int64_t *)red);
     uint64_t sum = 0;
-    int wraps = 0;
+    int wraps = 0;   // sign: a seen difference of 2^63 or more
     for (int t0 = 0; t0 < (LONG ? T : 1); t0 += TREE_SM_T * TREE_SM_E) {
 #pragma unroll
         for (int k = 0; k < TREE_SM_E; k++) {
-            const int t = t0 + k * TREE_SM_T + tid;
-            if (k && t0 + k * TREE_SM_T >= T) break;
+            const int tk = t0 + k * TREE_SM_T, t = tk + tid;
+            if (tk >= T) break;
             if (LONG) x[k] = t < T ? row[t] : INT64_MIN;
             const uint64_t d = (uint64_t)m - (uint64_t)x[k];
-            const bool in = sees(t);
-            wraps |= in && (int64_t)d < 0;
-            const int64_t e = tree_exp(d <= 10 * (uint64_t)IQ_ONE ? d : 0);
-            x[k] = in && d <= 10 * (uint64_t)IQ_ONE ? e : 0;
+            int64_t e = tree_exp(d);   // (anything where d is beyond 10)
+            bool in = d <= 10 * (uint64_t)IQ_ONE;
+            if (tk + TREE_SM_T <= s.len) {
+                wraps |= (int)(d >> 32);
+            } else if (sees(t)) {
+                wraps |= (int)(d >> 32);
+            } else {
+                in = false;
+            }
+            x[k] = in ? e : 0;
             sum += (uint64_t)x[k];
             if (LONG && t < T) row[t] = x[k];
         }
     }
     int64_t *out = a.out + ((size_t)r * a.nh + h) * hd;
-    if (__syncthreads_or(wraps)) {
+    if (__syncthreads_or(wraps < 0)) {
         tree_wrapped<PK>(a, s, r, h, T, m, row, out, red, sees);
         return;
     }
@@ -627,9 +689,6 @@ __global__ void __launch_bounds__(256, 2) k_tree_pv(const __grid_constant__ Tree
     const bool on = tg < tg_n && pc < cols;
     for (int e = tid; e < NC * hdp; e += 256) red[e] = 0;
     const TreeRows vr = tree_rows<PK>(a, true, ((size_t)s.sq * a.c.max_seq + tb) * a.c.nkv + g, Tl);
-    int vd[4];
-#pragma unroll
-    for (int k = 0; k < 4; k++) vd[k] = db + 16 * k + 2 * gq < hd ? db + 16 * k + 2 * gq : 0;
     const double *pp[CB];   // this lane's columns (a missing one: the last, not kept)
 #pragma unroll
     for (int cb = 0; cb < CB; cb++) {
@@ -638,63 +697,64 @@ __global__ void __launch_bounds__(256, 2) k_tree_pv(const __grid_constant__ Tree
                  ((size_t)(s.row0 + cc / grp) * a.nh + g * grp + cc % grp) * a.Tw + tb;
     }
     double f[CB][8][2];
+    uint32_t vm = 0;
+    // SPLIT: values beyond the chain as n 2^51 + f, 8 p n added in shared memory
+    auto sum = [&](auto split) {
+        constexpr bool SPLIT = decltype(split)::value;
 #pragma unroll
-    for (int cb = 0; cb < CB; cb++)
+        for (int cb = 0; cb < CB; cb++)
 #pragma unroll
-        for (int k = 0; k < 8; k++) f[cb][k][0] = f[cb][k][1] = TREE_A;
-    TreeVals<PK> vx;
-    if (on) vx.load(vr, tg * 4 + tq, vd);
+            for (int k = 0; k < 8; k++) f[cb][k][0] = f[cb][k][1] = TREE_A;
+        TreeVals<PK> vx;
+        double pn[CB];
+        vx.load(vr, tg * 4 + tq, db + 2 * gq, db);
+#pragma unroll
+        for (int cb = 0; cb < CB; cb++) pn[cb] = tg * 4 < Tl ? pp[cb][tg * 4 + tq] : 0;
+#pragma unroll 1
+        for (int t0 = tg * 4; t0 < Tl; t0 += tg_n * 4) {
+            double p[CB], v[8];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const longlong2 u = vx.get(vr, k);
+                int64_t w[2] = {u.x, u.y};
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    if (!SPLIT) tree_hi(vm, w[j], TREE_V1);
+                    else w[j] = (int64_t)((uint64_t)w[j] << 13) >> 13;
+                    v[2 * k + j] = __hiloint2double((int)(w[j] >> 32) + 0x43380000, (int)w[j]) - TREE_A;
+                }
+            }
+#pragma unroll
+            for (int cb = 0; cb < CB; cb++) p[cb] = pn[cb];
+            if (SPLIT)
+                for (int k = 0; k < 4; k++) {
+                    const longlong2 u = vx.get(vr, k);
+                    const int64_t n0 = (u.x >> 51) + (u.x >> 50 & 1), n1 = (u.y >> 51) + (u.y >> 50 & 1);
+                    // the other lanes' columns of this position too: p from the lane that holds it
+                    for (int i = 0; i < CW; i++) {
+                        const double pi = __shfl_sync(0xffffffffu, CB == 1 || i < 8 ? p[0] : p[CB - 1], (i & 7) * 4 + tq);
+                        const uint64_t p8 = (uint64_t)(pi * 0x1p51);
+                        unsigned long long *dst = red + (pc + i) * hdp + db + 16 * k + 2 * gq;
+                        if (n0 && t0 + tq < Tl) atomicAdd(dst, (unsigned long long)(p8 * (uint64_t)n0));
+                        if (n1 && t0 + tq < Tl) atomicAdd(dst + 1, (unsigned long long)(p8 * (uint64_t)n1));
+                    }
+                }
+            // the next four are on their way meanwhile (the last once more at the end)
+            const int t1 = min(t0 + tg_n * 4, (Tl - 1) & ~3);
+            vx.load(vr, t1 + tq, db + 2 * gq, db);
+#pragma unroll
+            for (int cb = 0; cb < CB; cb++) pn[cb] = pp[cb][t1 + tq];
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+#pragma unroll
+                for (int cb = 0; cb < CB; cb++) dmma_rd(f[cb][k][0], f[cb][k][1], p[cb], v[k]);
+        }
+    };
     tree_prev_kernel();
     __syncthreads();
     if (on) {
-        double pn[CB];
-#pragma unroll
-        for (int cb = 0; cb < CB; cb++) pn[cb] = tg * 4 < Tl ? pp[cb][tg * 4 + tq] : 0;
-        for (int t0 = tg * 4; t0 < Tl; t0 += tg_n * 4) {
-            longlong2 nx[4];
-            double p[CB];
-            uint32_t vm = 0;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                nx[k] = vx.get(vr, k);
-                tree_hi(vm, nx[k].x, TREE_V1);
-                tree_hi(vm, nx[k].y, TREE_V1);
-            }
-            const int t1 = t0 + tg_n * 4;   // the next four are on their way meanwhile
-            vx.load(vr, t1 + tq, vd);
-#pragma unroll
-            for (int cb = 0; cb < CB; cb++) {
-                p[cb] = pn[cb];
-                pn[cb] = pp[cb][min(t1, (Tl - 1) & ~3) + tq];
-            }
-            if (__any_sync(0xffffffffu, vm >= 2 * TREE_V1)) {   // 8 p n for values beyond the chain
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int64_t n0 = (nx[k].x >> 51) + (nx[k].x >> 50 & 1), n1 = (nx[k].y >> 51) + (nx[k].y >> 50 & 1);
-                    nx[k].x = (int64_t)((uint64_t)nx[k].x << 13) >> 13;
-                    nx[k].y = (int64_t)((uint64_t)nx[k].y << 13) >> 13;
-                    // the other lanes' columns of this position too: p from the lane that holds it
-#pragma unroll
-                    for (int cb = 0; cb < CB; cb++)
-                        for (int i = 0; i < 8; i++) {
-                            const uint64_t p8 = (uint64_t)(__shfl_sync(0xffffffffu, p[cb], i * 4 + tq) * 0x1p51);
-                            unsigned long long *dst = red + (pc + cb * 8 + i) * hdp + db + 16 * k + 2 * gq;
-                            if (n0 && t0 + tq < Tl) atomicAdd(dst, (unsigned long long)(p8 * (uint64_t)n0));
-                            if (n1 && t0 + tq < Tl) atomicAdd(dst + 1, (unsigned long long)(p8 * (uint64_t)n1));
-                        }
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const double v0 = __longlong_as_double((long long)((uint64_t)nx[k].x + TREE_AB)) - TREE_A;
-                const double v1 = __longlong_as_double((long long)((uint64_t)nx[k].y + TREE_AB)) - TREE_A;
-#pragma unroll
-                for (int cb = 0; cb < CB; cb++) {
-                    dmma_rd(f[cb][2 * k][0], f[cb][2 * k][1], p[cb], v0);
-                    dmma_rd(f[cb][2 * k + 1][0], f[cb][2 * k + 1][1], p[cb], v1);
-                }
-            }
-        }
+        sum(std::false_type{});
+        if (__any_sync(0xffffffffu, vm >= 2 * TREE_V1)) sum(std::true_type{});   // a value beyond the chain: once more
     }
     // partial outputs of the tg_n position groups meet in shared memory, group after group
     const int od = db + 4 * tq;   // tile k, output j: + 16 (k >> 1) + (k & 1) + 2 j
