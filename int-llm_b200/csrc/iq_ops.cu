@@ -104,7 +104,9 @@ static void tree_plan(TreeArgs *a) {
     while (a->tpc > 1 && pairs * ((tiles + a->tpc - 1) / a->tpc) < 6 * sms) a->tpc /= 2;
     a->tiles = (tiles + a->tpc - 1) / a->tpc;
     a->groups = (blocks + a->passes - 1) / a->passes;
-    a->cg = cols > 16 && a->c.hd <= 128 ? 2 : 1;
+    a->cg = cols > 32 && a->c.hd <= 64 ? 4 : cols > 16 && a->c.hd <= 128 ? 2 : 1;
+    a->heads = 1;
+    while (a->heads < 8 && (int64_t)a->rows * a->nh > (int64_t)a->heads * 32 * sms) a->heads *= 2;
     const int per = cols <= 8 ? 8 : 16 * a->cg;
     a->cblocks = (int)((cols + per - 1) / per);
     a->chunk = 1024;
@@ -115,13 +117,13 @@ static void tree_plan(TreeArgs *a) {
 
 // One kernel; prev: it waits for the one before itself (tree_prev_kernel), so it may start early.
 template <class... P, class... X>
-static int tree_launch(void (*k)(P...), int64_t grid_x, int grid_y, size_t smem, cudaStream_t s, bool prev, X... args) {
+static int tree_launch(void (*k)(P...), int64_t grid_x, int grid_y, int threads, size_t smem, cudaStream_t s, bool prev, X... args) {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3((unsigned)grid_x, (unsigned)grid_y);
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = at;
@@ -140,7 +142,7 @@ static int tree_scores(const TreeArgs &a, cudaStream_t s) {
                                      (int)tree_scores_smem(NT, 256)));
         set.fetch_or(1ull << dev);
     }
-    return tree_launch(k_tree_scores<NT, PK>, (int64_t)a.n_seq * a.c.nkv * a.groups * a.tiles, 1,
+    return tree_launch(k_tree_scores<NT, PK>, (int64_t)a.n_seq * a.c.nkv * a.groups * a.tiles, 1, 256,
                        tree_scores_smem(NT, a.c.hd), s, false, a);
 }
 template <bool PK>
@@ -149,12 +151,13 @@ static int launch_tree(const TreeArgs &a, cudaStream_t s) {
     int rc = cols <= 8 ? tree_scores<1, PK>(a, s) : tree_scores<2, PK>(a, s);
     if (rc) return rc;
     const int64_t rows = (int64_t)a.n_seq * a.max_nodes;
-    rc = a.max_len <= TREE_SM_T * TREE_SM_E ? tree_launch(k_tree_softmax<PK, false>, rows, a.nh, 0, s, true, a)
-                                            : tree_launch(k_tree_softmax<PK, true>, rows, a.nh, 0, s, true, a);
+    const int hb = (a.nh + a.heads - 1) / a.heads;
+    rc = a.max_len <= TREE_SM_T * TREE_SM_E ? tree_launch(k_tree_softmax<PK, false>, rows, hb, TREE_SM_T, 0, s, true, a)
+                                            : tree_launch(k_tree_softmax<PK, true>, rows, hb, TREE_SM_T, 0, s, true, a);
     if (rc) return rc;
     const int64_t pv = (int64_t)a.n_seq * a.c.nkv * a.cblocks * a.chunks;
-    return cols <= 8 ? tree_launch(k_tree_pv<1, PK>, pv, 1, 0, s, true, a)
-                     : tree_launch(k_tree_pv<2, PK>, pv, 1, 0, s, true, a);
+    return cols <= 8 ? tree_launch(k_tree_pv<1, PK>, pv, 1, 256, 0, s, true, a)
+                     : tree_launch(k_tree_pv<2, PK>, pv, 1, 256, 0, s, true, a);
 }
 
 extern "C" {

@@ -50,6 +50,7 @@ struct TreeArgs {
     int64_t *sc;    // workspace [rows][nh][Tw]: scores, then p 2^-48 as doubles
     int Tw, vec, vecq;
     int tiles, tpc, groups, passes;   // k_tree_scores: CTAs along the positions, tiles each, groups of column blocks, blocks a group
+    int heads;                        // k_tree_softmax: heads a CTA
     int chunk, chunks, cg, cblocks;   // k_tree_pv: positions a CTA, their number, groups of 8 CB columns a block, blocks
 };
 
@@ -495,6 +496,18 @@ __device__ __forceinline__ uint64_t tree_sqr(uint64_t r) {
     madu(x, h << 8, h << 8);
     return x;
 }
+// 1 / x by two Newton steps, relative error below 2^-51
+__device__ __forceinline__ double tree_rcp(double x) {
+    double y;
+    asm("rcp.approx.ftz.f64 %0, %1;" : "=d"(y) : "d"(x));
+    y = __fma_rn(y, __fma_rn(-x, y, 1.0), y);
+    return __fma_rn(y, __fma_rn(-x, y, 1.0), y);
+}
+// the positive 64-bit x as a double (one rounding)
+__device__ __forceinline__ double tree_u64(uint64_t x) {
+    return (__longlong_as_double((long long)((x >> 32) | 0x4530000000000000ull)) - 19342813118337666422669312.0) +
+           __longlong_as_double((long long)((x & 0xFFFFFFFFull) | TREE_MB));
+}
 // 1 where q r + c < 0 (mod 2^64, as a signed number), else 0
 __device__ __forceinline__ uint32_t tree_more(uint64_t q, uint64_t r, uint64_t c) {
     madu(c, (uint32_t)q, (uint32_t)r);
@@ -513,20 +526,12 @@ __device__ __forceinline__ int64_t tree_exp(uint64_t d) {
     // floor(2^96 / r), at most 2^48: reciprocal by two Newton steps (relative error
     // below 2^-51), lowered by 2^-50 so that its floor is q or q - 1; the sign of
     // (q + 1) r - 2^96 - 1 (2^96 = 0 mod 2^64) tells which
-    const double rd = (__longlong_as_double((long long)((r >> 32) | 0x4530000000000000ull)) - 19342813118337666422669312.0) +
-                      __longlong_as_double((long long)((r & 0xFFFFFFFFull) | TREE_MB));
-    double y;
-    asm("rcp.approx.ftz.f64 %0, %1;" : "=d"(y) : "d"(rd));
-    y = __fma_rn(y, __fma_rn(-rd, y, 1.0), y);
-    y = __fma_rn(y, __fma_rn(-rd, y, 1.0), y);
+    const double y = tree_rcp(tree_u64(r));
     const uint64_t q = (uint64_t)__double_as_longlong(__fma_rd(y, 0x1p96 - 0x1p46, TREE_M)) & TREE_MASK;
     return (int64_t)(q + tree_more(q, r, r - 1));
 }
-// 2^48 / S, lowered likewise for tree_prob
-__device__ __forceinline__ double tree_inv(int64_t S) {
-    return __dmul_rn(281474976710656.0 / (double)S, 1.0 - 0x1p-50);
-}
-// fp_div(e, S) 2^-48 as a double for 0 <= e <= S, 2^48 <= S < 2^63, e <= 2^48
+// fp_div(e, S) 2^-48 as a double for 0 <= e <= S, 2^48 <= S < 2^63, e <= 2^48,
+// inv = tree_rcp(S) 2^48 lowered like the quotient of tree_exp
 __device__ __forceinline__ double tree_prob(int64_t e, int64_t S, double inv) {
     const uint64_t q = (uint64_t)__double_as_longlong(__fma_rd(tree_u52((uint64_t)e), inv, TREE_M)) & TREE_MASK;
     return tree_u52(q + tree_more(q, (uint64_t)S, (uint64_t)S - 1 - ((uint64_t)e << 48))) * 0x1p-48;
@@ -566,25 +571,26 @@ __device__ __noinline__ void tree_wrapped(const TreeArgs &a, const TreeSeq &s, i
     for (int t = threadIdx.x; t < min(a.Tw, (s.len + s.n + 3) & ~3); t += blockDim.x) row[t] = 0;
 }
 
-// A CTA a (node row, head). E scores a thread stay in registers; longer rows go
+// A CTA a node row and a.heads of its heads. E scores a thread stay in registers; longer rows go
 // through the workspace three times (LONG). A row whose score differences
 // wrap (the reference's int64 then gives other numbers, reproduced here) is
 // finished here term by term and leaves zeros to k_tree_pv.
-#define TREE_SM_T 256
-#define TREE_SM_E 8
+#define TREE_SM_T 128
+#define TREE_SM_E 16
 template <bool PK, bool LONG>
 __global__ void __launch_bounds__(TREE_SM_T) k_tree_softmax(const __grid_constant__ TreeArgs a) {
     __shared__ uint64_t red[64];
+    __shared__ int64_t wmax[2][TREE_SM_T / 32];
+    __shared__ uint64_t wsum[2][TREE_SM_T / 32];
     __shared__ int up[TREE_MAX_NODES];
     __shared__ uint32_t anc[TREE_MAX_NODES / 32];
-    const int b = blockIdx.x / a.max_nodes, node = blockIdx.x % a.max_nodes, h = blockIdx.y, tid = threadIdx.x;
+    const int b = blockIdx.x / a.max_nodes, node = blockIdx.x - b * a.max_nodes, tid = threadIdx.x;
     TreeSeq s;
     if (!tree_seq(a, b, s) || node >= s.n) return;
     const int r = s.row0 + node, hd = a.c.hd, T = s.len + node + 1;   // no later node is seen
     // ancestors of the node
-    for (int i = tid; i < node; i += TREE_SM_T) up[i] = a.parent[s.row0 + i];
+    for (int i = tid; i <= node; i += TREE_SM_T) up[i] = a.parent[s.row0 + i];
     if (tid < TREE_MAX_NODES / 32) anc[tid] = 0;
-    if (tid == TREE_SM_T - 1) up[node] = a.parent[r];
     __syncthreads();
     if (tid == 0)
         for (int j = node;;) {
@@ -595,69 +601,82 @@ __global__ void __launch_bounds__(TREE_SM_T) k_tree_softmax(const __grid_constan
         }
     tree_prev_kernel();
     __syncthreads();
-    int64_t *row = a.sc + ((size_t)r * a.nh + h) * a.Tw;
     auto sees = [&](int t) {
         const int j = t - s.len;
         return j < 0 || (t < T && (anc[j >> 5] >> (j & 31) & 1));
     };
-    int64_t x[TREE_SM_E], m = INT64_MIN;
-    for (int t0 = 0; t0 < (LONG ? T : 1); t0 += TREE_SM_T * TREE_SM_E) {
-#pragma unroll
-        for (int k = 0; k < TREE_SM_E; k++) {
-            const int tk = t0 + k * TREE_SM_T, t = tk + tid;
-            x[k] = INT64_MIN;
-            if (tk + TREE_SM_T <= s.len) {   // all before the draft
-                x[k] = row[t];
-                m = max(m, x[k]);
-            } else if (tk < T) {
-                if (t < T) x[k] = row[t];
-                if (sees(t)) m = max(m, x[k]);
-            }
-        }
-    }
-    m = cta_max_i64(m, (int64_t *)red);
-    uint64_t sum = 0;
-    int wraps = 0;   // sign: a seen difference of 2^63 or more
-    for (int t0 = 0; t0 < (LONG ? T : 1); t0 += TREE_SM_T * TREE_SM_E) {
-#pragma unroll
-        for (int k = 0; k < TREE_SM_E; k++) {
-            const int tk = t0 + k * TREE_SM_T, t = tk + tid;
-            if (tk >= T) break;
-            if (LONG) x[k] = t < T ? row[t] : INT64_MIN;
-            const uint64_t d = (uint64_t)m - (uint64_t)x[k];
-            int64_t e = tree_exp(d);   // (anything where d is beyond 10)
-            bool in = d <= 10 * (uint64_t)IQ_ONE;
-            if (tk + TREE_SM_T <= s.len) {
-                wraps |= (int)(d >> 32);
-            } else if (sees(t)) {
-                wraps |= (int)(d >> 32);
-            } else {
-                in = false;
-            }
-            x[k] = in ? e : 0;
-            sum += (uint64_t)x[k];
-            if (LONG && t < T) row[t] = x[k];
-        }
-    }
-    int64_t *out = a.out + ((size_t)r * a.nh + h) * hd;
-    if (__syncthreads_or(wraps < 0)) {
-        tree_wrapped<PK>(a, s, r, h, T, m, row, out, red, sees);
-        return;
-    }
-    const int64_t S = (int64_t)(uint64_t)cta_sum_i128((i128)(u128)sum, red);
-    const double inv = tree_inv(S);
-    double *p = reinterpret_cast<double *>(row);
     const int end = min(a.Tw, (s.len + s.n + 3) & ~3);   // k_tree_pv reads fours up to here
-    for (int t0 = 0; t0 < (LONG ? end : 1); t0 += TREE_SM_T * TREE_SM_E) {
+    const int h0 = blockIdx.y * a.heads, h1 = min(h0 + a.heads, a.nh);
+    for (int h = h0; h < h1; h++) {
+        const int par = h & 1;   // the other half of wmax and wsum may still be read
+        int64_t *row = a.sc + ((size_t)r * a.nh + h) * a.Tw;
+        int64_t x[TREE_SM_E], m = INT64_MIN;
+        for (int t0 = 0; t0 < (LONG ? T : 1); t0 += TREE_SM_T * TREE_SM_E) {
 #pragma unroll
-        for (int k = 0; k < TREE_SM_E; k++) {
-            const int t = t0 + k * TREE_SM_T + tid;
-            if (t0 + k * TREE_SM_T >= end) break;
-            const int64_t e = LONG ? (t < T ? row[t] : 0) : t < T ? x[k] : 0;
-            if (t < end) p[t] = tree_prob(e, S, inv);
+            for (int k = 0; k < TREE_SM_E; k++) {
+                const int tk = t0 + k * TREE_SM_T, t = tk + tid;
+                x[k] = INT64_MIN;
+                if (tk + TREE_SM_T <= s.len) {   // all before the draft
+                    x[k] = row[t];
+                } else if (tk < T) {
+                    if (t < T) x[k] = row[t];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < TREE_SM_E; k++) {
+                const int tk = t0 + k * TREE_SM_T, t = tk + tid;
+                if (tk + TREE_SM_T <= s.len) m = max(m, x[k]);
+                else if (tk < T && sees(t)) m = max(m, x[k]);
+            }
         }
+        for (int k = 16; k >= 1; k >>= 1) m = max(m, (int64_t)__shfl_xor_sync(0xffffffffu, m, k));
+        if ((tid & 31) == 0) wmax[par][tid >> 5] = m;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < TREE_SM_T / 32; k++) m = max(m, wmax[par][k]);
+        uint64_t sum = 0;
+        int wraps = 0;   // sign: a seen difference of 2^63 or more
+        for (int t0 = 0; t0 < (LONG ? T : 1); t0 += TREE_SM_T * TREE_SM_E) {
+#pragma unroll
+            for (int k = 0; k < TREE_SM_E; k++) {
+                const int tk = t0 + k * TREE_SM_T, t = tk + tid;
+                if (tk < T) {
+                    if (LONG) x[k] = t < T ? row[t] : INT64_MIN;
+                    const uint64_t d = (uint64_t)m - (uint64_t)x[k];
+                    const int64_t e = tree_exp(d);   // (anything where d is beyond 10)
+                    bool in = d <= 10 * (uint64_t)IQ_ONE;
+                    if (tk + TREE_SM_T > s.len && !sees(t)) in = false;
+                    else wraps |= (int)(d >> 32);
+                    x[k] = in ? e : 0;
+                    sum += (uint64_t)x[k];
+                    if (LONG && t < T) row[t] = x[k];
+                }
+            }
+        }
+        for (int k = 16; k >= 1; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+        if ((tid & 31) == 0) wsum[par][tid >> 5] = sum;
+        int64_t *out = a.out + ((size_t)r * a.nh + h) * hd;
+        if (__syncthreads_or(wraps < 0)) {
+            tree_wrapped<PK>(a, s, r, h, T, m, row, out, red, sees);
+            continue;
+        }
+        uint64_t S = 0;
+#pragma unroll
+        for (int k = 0; k < TREE_SM_T / 32; k++) S += wsum[par][k];
+        const double inv = tree_rcp(tree_u64(S)) * (0x1p48 - 0x1p-2);
+        double *p = reinterpret_cast<double *>(row);
+        for (int t0 = 0; t0 < (LONG ? end : 1); t0 += TREE_SM_T * TREE_SM_E) {
+#pragma unroll
+            for (int k = 0; k < TREE_SM_E; k++) {
+                const int tk = t0 + k * TREE_SM_T, t = tk + tid;
+                if (tk < end) {
+                    const int64_t e = LONG ? (t < T ? row[t] : 0) : t < T ? x[k] : 0;
+                    if (t < end) p[t] = tree_prob(e, (int64_t)S, inv);
+                }
+            }
+        }
+        for (int d = tid; d < hd; d += TREE_SM_T) out[d] = 0;   // k_tree_pv adds
     }
-    for (int d = tid; d < hd; d += TREE_SM_T) out[d] = 0;   // k_tree_pv adds
 }
 
 // ---------------------------------------------------- 3. probabilities x values
