@@ -104,7 +104,7 @@ static void tree_plan(TreeArgs *a) {
     while (a->tpc > 1 && pairs * ((tiles + a->tpc - 1) / a->tpc) < 6 * sms) a->tpc /= 2;
     a->tiles = (tiles + a->tpc - 1) / a->tpc;
     a->groups = (blocks + a->passes - 1) / a->passes;
-    a->cg = cols > 32 && a->c.hd <= 64 ? 4 : cols > 16 && a->c.hd <= 128 ? 2 : 1;
+    a->cg = cols > 32 && a->c.hd <= 64 ? 4 : cols > 16 && a->c.hd <= 128 ? 2 : 1;   // 16 cg hd <= TREE_RED
     a->heads = 1;
     while (a->heads < 8 && (int64_t)a->rows * a->nh > (int64_t)a->heads * 32 * sms) a->heads *= 2;
     const int per = cols <= 8 ? 8 : 16 * a->cg;
@@ -132,23 +132,23 @@ static int tree_launch(void (*k)(P...), int64_t grid_x, int grid_y, int threads,
     return IQ_OK;
 }
 
-template <int NT, bool PK>
+template <int NT, bool PK, bool W>
 static int tree_scores(const TreeArgs &a, cudaStream_t s) {
     static std::atomic<uint64_t> set{0};   // devices whose shared-memory limit is raised
     int dev = 0;
     IQ_CUDA(cudaGetDevice(&dev));
     if (!(set.load() >> dev & 1)) {
-        IQ_CUDA(cudaFuncSetAttribute(k_tree_scores<NT, PK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        IQ_CUDA(cudaFuncSetAttribute(k_tree_scores<NT, PK, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      (int)tree_scores_smem(NT, 256)));
         set.fetch_or(1ull << dev);
     }
-    return tree_launch(k_tree_scores<NT, PK>, (int64_t)a.n_seq * a.c.nkv * a.groups * a.tiles, 1, 256,
+    return tree_launch(k_tree_scores<NT, PK, W>, (int64_t)a.n_seq * a.c.nkv * a.groups * a.tiles, 1, 256,
                        tree_scores_smem(NT, a.c.hd), s, false, a);
 }
-template <bool PK>
+template <bool PK, bool W>
 static int launch_tree(const TreeArgs &a, cudaStream_t s) {
-    const int64_t cols = (int64_t)std::min(a.max_nodes, a.rows) * (a.nh / a.c.nkv);
-    int rc = cols <= 8 ? tree_scores<1, PK>(a, s) : tree_scores<2, PK>(a, s);
+    const bool eight = (int64_t)std::min(a.max_nodes, a.rows) * (a.nh / a.c.nkv) <= 8;
+    int rc = eight ? tree_scores<1, PK, W>(a, s) : tree_scores<2, PK, W>(a, s);
     if (rc) return rc;
     const int64_t rows = (int64_t)a.n_seq * a.max_nodes;
     const int hb = (a.nh + a.heads - 1) / a.heads;
@@ -156,8 +156,8 @@ static int launch_tree(const TreeArgs &a, cudaStream_t s) {
                                             : tree_launch(k_tree_softmax<PK, true>, rows, hb, TREE_SM_T, 0, s, true, a);
     if (rc) return rc;
     const int64_t pv = (int64_t)a.n_seq * a.c.nkv * a.cblocks * a.chunks;
-    return cols <= 8 ? tree_launch(k_tree_pv<1, PK>, pv, 1, 256, 0, s, true, a)
-                     : tree_launch(k_tree_pv<2, PK>, pv, 1, 256, 0, s, true, a);
+    return eight ? tree_launch(k_tree_pv<1, PK, W>, pv, 1, 256, 0, s, true, a)
+                 : tree_launch(k_tree_pv<2, PK, W>, pv, 1, 256, 0, s, true, a);
 }
 
 extern "C" {
@@ -289,11 +289,13 @@ IQ_API int iq_attn_tree_dev(int64_t *d_out, const int64_t *d_q, const iq_kv_cach
     const int64_t most = std::max({(int64_t)n_seq * a.c.nkv * a.groups * a.tiles,
                                    (int64_t)n_seq * a.c.nkv * a.cblocks * a.chunks, (int64_t)n_seq * max_nodes});
     if (most > INT_MAX) return IQ_ERR_RANGE;
-    // whole 32-wide steps in aligned pieces: 16 bytes of exact vectors, 16 key and 2 value codes of packed ones
-    a.vec = a.c.hd % 32 == 0 && (a.c.kbits ? !misaligned(a.c.kq, 16) && !misaligned(a.c.vq, 4)
-                                           : !misaligned(a.c.k, 16) && !misaligned(a.c.v, 16));
-    a.vecq = a.c.hd % 32 == 0 && !misaligned(d_q, 16) && q_stride % 2 == 0;
-    return a.c.kbits ? launch_tree<true>(a, pick(stream)) : launch_tree<false>(a, pick(stream));
+    // whole 32-wide steps in aligned pieces: 16 bytes of queries and exact vectors, 16 key and 2 value codes of packed ones
+    const bool wide = a.c.hd % 32 == 0 && !misaligned(d_q, 16) && q_stride % 2 == 0 &&
+                      (a.c.kbits ? !misaligned(a.c.kq, 16) && !misaligned(a.c.vq, 4)
+                                 : !misaligned(a.c.k, 16) && !misaligned(a.c.v, 16));
+    cudaStream_t st = pick(stream);
+    if (a.c.kbits) return wide ? launch_tree<true, true>(a, st) : launch_tree<true, false>(a, st);
+    return wide ? launch_tree<false, true>(a, st) : launch_tree<false, false>(a, st);
 }
 
 IQ_API int iq_logprobs_dev(const int64_t *d_logits, int64_t ld, int rows, int vocab, const int *d_tokens,

@@ -48,7 +48,7 @@ struct TreeArgs {
     int n_seq, rows, max_nodes, max_len, nh;
     int64_t qs, scale;
     int64_t *sc;    // workspace [rows][nh][Tw]: scores, then p 2^-48 as doubles
-    int Tw, vec, vecq;
+    int Tw;
     int tiles, tpc, groups, passes;   // k_tree_scores: CTAs along the positions, tiles each, groups of column blocks, blocks a group
     int heads;                        // k_tree_softmax: heads a CTA
     int chunk, chunks, cg, cblocks;   // k_tree_pv: positions a CTA, their number, groups of 8 CB columns a block, blocks
@@ -81,13 +81,12 @@ __device__ __forceinline__ int tree_d(int h, int e) {
 // loads never branch: a position or d beyond the end is clamped into the
 // vectors (such keys meet a query plane of zeros or a score that no row sees,
 // such values a probability of zero or an output column that is not kept).
-// wide: aligned pieces; else element by element.
+// W: whole 32-wide steps in aligned pieces; else element by element.
 struct TreeRows {
     const char *x;         // exact elements or codes
     const int64_t *mag;    // packed
     uint32_t rs, ms;       // bytes of a position, magnitudes of a position
     int T, hd, bits;
-    bool wide;
 };
 template <bool PK>
 __device__ __forceinline__ TreeRows tree_rows(const TreeArgs &a, bool val, size_t vec0, int T) {
@@ -102,16 +101,15 @@ __device__ __forceinline__ TreeRows tree_rows(const TreeArgs &a, bool val, size_
     r.T = T;
     r.hd = c.hd;
     r.bits = val ? c.vbits : c.kbits;
-    r.wide = a.vec;
     return r;
 }
 // Half h of one position's 32-wide key step from d0 on, as loaded.
-template <bool PK> struct TreeKeys;
-template <> struct TreeKeys<false> {
+template <bool PK, bool W> struct TreeKeys;
+template <bool W> struct TreeKeys<false, W> {
     longlong2 x[8];
     __device__ __forceinline__ void load(const TreeRows &r, int t, int d0, int h) {
         const int64_t *p = reinterpret_cast<const int64_t *>(r.x + (size_t)(uint32_t)min(t, r.T - 1) * r.rs);
-        if (r.wide) {
+        if constexpr (W) {
             const longlong2 *q = reinterpret_cast<const longlong2 *>(p + d0 + 2 * h);
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = __ldg(q + 2 * j);
@@ -127,14 +125,14 @@ template <> struct TreeKeys<false> {
         o[0] = x[2 * w].x; o[1] = x[2 * w].y; o[2] = x[2 * w + 1].x; o[3] = x[2 * w + 1].y;
     }
 };
-template <> struct TreeKeys<true> {
+template <bool W> struct TreeKeys<true, W> {
     uint32_t q[4];
     int64_t m;
     __device__ __forceinline__ void load(const TreeRows &r, int t, int d0, int h) {
         t = min(t, r.T - 1);
         const uint8_t *p = reinterpret_cast<const uint8_t *>(r.x) + (size_t)(uint32_t)t * r.rs;
         m = __ldg(r.mag + (size_t)(uint32_t)t * r.ms);
-        if (r.wide) {
+        if constexpr (W) {
             const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p + d0 + h * 16));
             q[0] = u.x; q[1] = u.y; q[2] = u.z; q[3] = u.w;
         } else {
@@ -151,42 +149,35 @@ template <> struct TreeKeys<true> {
         for (int i = 0; i < 4; i++) o[i] = kv_value((q[w] >> (8 * i)) & 0xFF, m, r.bits);
     }
 };
-// A lane's values of one position, as loaded: pairs at d + 16 k, k < 4 (d in the
-// 64-wide block from db on; beyond hd anything).
-template <bool PK> struct TreeVals;
-template <> struct TreeVals<false> {
-    longlong2 x[4];
-    __device__ __forceinline__ void load(const TreeRows &r, int t, int d, int db) {
+// A lane's values of one position, as loaded: pairs at d and d + 16 (beyond hd anything).
+template <bool PK, bool W> struct TreeVals;
+template <bool W> struct TreeVals<false, W> {
+    longlong2 x[2];
+    __device__ __forceinline__ void load(const TreeRows &r, int t, int d) {
         const int64_t *p = reinterpret_cast<const int64_t *>(r.x + (size_t)(uint32_t)min(t, r.T - 1) * r.rs) + d;
-        if (r.wide) {   // hd a multiple of 32: a block is whole or half
-            const longlong2 *q = reinterpret_cast<const longlong2 *>(p), *q2 = r.hd - db >= 64 ? q + 16 : q;
-            x[0] = q[0];
-            x[1] = q[8];
-            x[2] = q2[0];
-            x[3] = q2[8];
+        if constexpr (W) {
+            x[0] = *reinterpret_cast<const longlong2 *>(p);
+            x[1] = *reinterpret_cast<const longlong2 *>(p + 16);
         } else {
 #pragma unroll
-            for (int k = 0; k < 4; k++) x[k] = make_longlong2(p[min(16 * k, r.hd - 1 - d)], p[min(16 * k + 1, r.hd - 1 - d)]);
+            for (int k = 0; k < 2; k++) x[k] = make_longlong2(p[min(16 * k, r.hd - 1 - d)], p[min(16 * k + 1, r.hd - 1 - d)]);
         }
     }
     __device__ __forceinline__ longlong2 get(const TreeRows &, int k) const { return x[k]; }
 };
-template <> struct TreeVals<true> {
-    ushort2 q[4];
+template <bool W> struct TreeVals<true, W> {
+    ushort2 q[2];
     int64_t m;
-    __device__ __forceinline__ void load(const TreeRows &r, int t, int d, int db) {
+    __device__ __forceinline__ void load(const TreeRows &r, int t, int d) {
         t = min(t, r.T - 1);
         const uint16_t *p = reinterpret_cast<const uint16_t *>(r.x + (size_t)(uint32_t)t * r.rs) + d;
-        m = __ldg(r.mag + (size_t)(uint32_t)t * r.ms);
-        if (r.wide) {
-            const ushort2 *u = reinterpret_cast<const ushort2 *>(p), *u2 = r.hd - db >= 64 ? u + 16 : u;
-            q[0] = u[0];
-            q[1] = u[8];
-            q[2] = u2[0];
-            q[3] = u2[8];
+        m = r.mag[(size_t)(uint32_t)t * r.ms];
+        if constexpr (W) {
+            q[0] = *reinterpret_cast<const ushort2 *>(p);
+            q[1] = *reinterpret_cast<const ushort2 *>(p + 16);
         } else {
 #pragma unroll
-            for (int k = 0; k < 4; k++) q[k] = make_ushort2(p[min(16 * k, r.hd - 1 - d)], p[min(16 * k + 1, r.hd - 1 - d)]);
+            for (int k = 0; k < 2; k++) q[k] = make_ushort2(p[min(16 * k, r.hd - 1 - d)], p[min(16 * k + 1, r.hd - 1 - d)]);
         }
     }
     __device__ __forceinline__ longlong2 get(const TreeRows &r, int k) const {
@@ -285,7 +276,7 @@ __host__ __device__ constexpr size_t tree_scores_smem(int NT, int hd) { return 1
 // once for all its blocks, with one block the query planes once for all its tiles.
 // Two CTAs an SM (three with 8 columns) overlap one another's loads, products
 // and epilogues; TMEM holds 128 NT columns a CTA.
-template <int NT, bool PK>
+template <int NT, bool PK, bool W>
 __global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __grid_constant__ TreeArgs a) {
     extern __shared__ __align__(16) char tree_smem[];
     constexpr int NC = 8 * NT, HC = NC / 2;
@@ -309,7 +300,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __gr
     // swizzles differ, so that their 16-byte stores meet no bank twice
     const int cq = lane >> 1, ch = lane & 1, cp = warp * 16 + ((cq & 8) | ((cq & 3) << 1) | ((cq >> 2) & 1));
     const TreeRows kr = tree_rows<PK>(a, false, (size_t)s.sq * a.c.max_seq * a.c.nkv + g, T);
-    TreeKeys<PK> kx;
+    TreeKeys<PK, W> kx;
     if (tb0 + cp < te) kx.load(kr, tb0 + cp, 0, ch);
     if (warp == 0) tmem_alloc(&tmem_s, 128 * NT);
     if (tid == 0) {
@@ -346,7 +337,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __gr
                 const int cc = c0 + min(col, nc - 1), nd = cc / grp;
                 const int64_t *q = a.q + (int64_t)(s.row0 + nd) * a.qs + (int64_t)(g * grp + cc - nd * grp) * hd + ks * 32;
                 int64_t x[4];
-                if (a.vecq) {   // whole steps, aligned pairs
+                if constexpr (W) {
                     const longlong2 u = __ldg(reinterpret_cast<const longlong2 *>(q + tree_d<PK>(h, 4 * w)));
                     const longlong2 v = __ldg(reinterpret_cast<const longlong2 *>(q + tree_d<PK>(h, 4 * w + 2)));
                     x[0] = u.x; x[1] = u.y; x[2] = v.x; x[3] = v.y;
@@ -357,7 +348,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __gr
                 uint32_t o[8];
                 byte_planes4(x, o);
                 o[7] ^= 0x80808080u;
-                if (!a.vecq)   // beyond hd x_u is 0, not 2^63: nothing meets whatever the keys hold there
+                if (!W)   // beyond hd x_u is 0, not 2^63: nothing meets whatever the keys hold there
 #pragma unroll
                     for (int i = 0; i < 4; i++)
                         if (ks * 32 + tree_d<PK>(h, 4 * w + i) >= hd) o[7] &= ~(0xFFu << (8 * i));
@@ -394,7 +385,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __gr
                     if (pass == p0)
 #pragma unroll
                         for (int i = 0; i < 16; i++)
-                            if (kr.wide || ks * 32 + tree_d<PK>(ch, i) < hd) sum += (unsigned long long)x[i];
+                            if (W || ks * 32 + tree_d<PK>(ch, i) < hd) sum += (unsigned long long)x[i];
                     char *const A = sA + (size_t)half * 32768;
 #pragma unroll
                     for (int hw = 0; hw < 2; hw++) {   // planes 0-3 from the low words, 4-7 from the high ones
@@ -684,57 +675,63 @@ __global__ void __launch_bounds__(TREE_SM_T) k_tree_softmax(const __grid_constan
 #define TREE_RED 4096   // whole numbers of the buffer in which partial outputs meet
 
 // A CTA takes a.chunk positions of CG x 8 CB columns of one (sequence, kv head); a
-// warp 64 d of 8 CB columns and every tg_n-th four positions. A lane holds V of
-// position lane & 3 at d = 16 k + 2 (lane >> 2) + {0, 1}, k < 4, i.e. column lane >> 2 of
+// warp 32 d of 8 CB columns and every tg_n-th four positions. A lane holds V of
+// position lane & 3 at d = 16 k + 2 (lane >> 2) + {0, 1}, k < 2, i.e. column lane >> 2 of
 // the 8-wide tiles 2k and 2k + 1, and of each tile's output the columns
-// 2 (lane & 3) + {0, 1}. Values come straight from global memory: nothing is
-// staged and no barrier runs inside the loop.
-template <int CB, bool PK>
+// 2 (lane & 3) + {0, 1}. Values come straight from global memory (the warps of the
+// CG column groups meet them in L1), two steps ahead: nothing is staged and no
+// barrier runs inside the loop.
+template <int CB, bool PK, bool W>
 __global__ void __launch_bounds__(256, 2) k_tree_pv(const __grid_constant__ TreeArgs a) {
     __shared__ __align__(16) unsigned long long red[TREE_RED];
     constexpr int CW = 8 * CB;
     const int chunk = blockIdx.x % a.chunks, rest = blockIdx.x / a.chunks;
     const int blk = rest % a.cblocks, g = rest / a.cblocks % a.c.nkv, b = rest / a.cblocks / a.c.nkv;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
-    const int grp = a.nh / a.c.nkv, hd = a.c.hd, hdp = (hd + 63) / 64 * 64, nd = hdp >> 6;
+    const int grp = a.nh / a.c.nkv, hd = a.c.hd, nd = (hd + 31) >> 5, hdp = nd * 32;
     TreeSeq s;
     if (!tree_seq(a, b, s)) return;
-    const int CG = a.cg, NC = CG * CW;   // NC hdp <= TREE_RED
+    const int CG = a.cg, NC = CG * CW;   // NC hdp <= TREE_RED, CG nd <= 8
     const int cols = min(NC, s.n * grp - blk * NC), c0 = blk * NC, tb = chunk * a.chunk;
     const int Tl = min(a.chunk, s.len + s.n - tb);
     if (Tl <= 0 || cols <= 0) return;
-    const int units = CG * nd, tg_n = 8 / units;   // units <= 8; warps from units * tg_n on idle
-    const int unit = warp % units, tg = warp / units, pc = unit / nd * CW, db = unit % nd * 64;
+    const int units = CG * nd, tg_n = 8 / units;   // warps from units * tg_n on idle
+    const int unit = warp % units, tg = warp / units, pc = unit % CG * CW, db = unit / CG * 32;
     const bool on = tg < tg_n && pc < cols;
     for (int e = tid; e < NC * hdp; e += 256) red[e] = 0;
     const TreeRows vr = tree_rows<PK>(a, true, ((size_t)s.sq * a.c.max_seq + tb) * a.c.nkv + g, Tl);
     const double *pp[CB];   // this lane's columns (a missing one: the last, not kept)
 #pragma unroll
     for (int cb = 0; cb < CB; cb++) {
-        const int cc = c0 + min(pc + cb * 8 + gq, cols - 1);
+        const int cc = c0 + min(pc + cb * 8 + gq, cols - 1), n = cc / grp;
         pp[cb] = reinterpret_cast<const double *>(a.sc) +
-                 ((size_t)(s.row0 + cc / grp) * a.nh + g * grp + cc % grp) * a.Tw + tb;
+                 ((size_t)(s.row0 + n) * a.nh + g * grp + cc - n * grp) * a.Tw + tb + tq;
     }
-    double f[CB][8][2];
+    double f[CB][4][2];
     uint32_t vm = 0;
+    const int step = tg_n * 4, tlast = (Tl - 1) & ~3;
     // SPLIT: values beyond the chain as n 2^51 + f, 8 p n added in shared memory
     auto sum = [&](auto split) {
         constexpr bool SPLIT = decltype(split)::value;
 #pragma unroll
         for (int cb = 0; cb < CB; cb++)
 #pragma unroll
-            for (int k = 0; k < 8; k++) f[cb][k][0] = f[cb][k][1] = TREE_A;
-        TreeVals<PK> vx;
-        double pn[CB];
-        vx.load(vr, tg * 4 + tq, db + 2 * gq, db);
+            for (int k = 0; k < 4; k++) f[cb][k][0] = f[cb][k][1] = TREE_A;
+        TreeVals<PK, W> vx[2];
+        double pn[2][CB];
+        auto load = [&](int st, int t0) {   // beyond the end: the last four once more
+            const int t = min(t0, tlast);
+            vx[st].load(vr, t + tq, db + 2 * gq);
 #pragma unroll
-        for (int cb = 0; cb < CB; cb++) pn[cb] = tg * 4 < Tl ? pp[cb][tg * 4 + tq] : 0;
-#pragma unroll 1
-        for (int t0 = tg * 4; t0 < Tl; t0 += tg_n * 4) {
-            double p[CB], v[8];
+            for (int cb = 0; cb < CB; cb++) pn[st][cb] = pp[cb][t];
+        };
+        auto four = [&](int st, int t0) {
+            double p[CB], v[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const longlong2 u = vx.get(vr, k);
+            for (int cb = 0; cb < CB; cb++) p[cb] = pn[st][cb];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const longlong2 u = vx[st].get(vr, k);
                 int64_t w[2] = {u.x, u.y};
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
@@ -742,12 +739,7 @@ __global__ void __launch_bounds__(256, 2) k_tree_pv(const __grid_constant__ Tree
                     else w[j] = (int64_t)((uint64_t)w[j] << 13) >> 13;
                     v[2 * k + j] = __hiloint2double((int)(w[j] >> 32) + 0x43380000, (int)w[j]) - TREE_A;
                 }
-            }
-#pragma unroll
-            for (int cb = 0; cb < CB; cb++) p[cb] = pn[cb];
-            if (SPLIT)
-                for (int k = 0; k < 4; k++) {
-                    const longlong2 u = vx.get(vr, k);
+                if (SPLIT) {
                     const int64_t n0 = (u.x >> 51) + (u.x >> 50 & 1), n1 = (u.y >> 51) + (u.y >> 50 & 1);
                     // the other lanes' columns of this position too: p from the lane that holds it
                     for (int i = 0; i < CW; i++) {
@@ -758,15 +750,19 @@ __global__ void __launch_bounds__(256, 2) k_tree_pv(const __grid_constant__ Tree
                         if (n1 && t0 + tq < Tl) atomicAdd(dst + 1, (unsigned long long)(p8 * (uint64_t)n1));
                     }
                 }
-            // the next four are on their way meanwhile (the last once more at the end)
-            const int t1 = min(t0 + tg_n * 4, (Tl - 1) & ~3);
-            vx.load(vr, t1 + tq, db + 2 * gq, db);
+            }
+            load(st, t0 + 2 * step);
 #pragma unroll
-            for (int cb = 0; cb < CB; cb++) pn[cb] = pp[cb][t1 + tq];
-#pragma unroll
-            for (int k = 0; k < 8; k++)
+            for (int k = 0; k < 4; k++)
 #pragma unroll
                 for (int cb = 0; cb < CB; cb++) dmma_rd(f[cb][k][0], f[cb][k][1], p[cb], v[k]);
+        };
+        load(0, tg * 4);
+        load(1, tg * 4 + step);
+#pragma unroll 1
+        for (int t0 = tg * 4; t0 < Tl; t0 += 2 * step) {
+            four(0, t0);
+            if (t0 + step < Tl) four(1, t0 + step);
         }
     };
     tree_prev_kernel();
@@ -784,7 +780,7 @@ __global__ void __launch_bounds__(256, 2) k_tree_pv(const __grid_constant__ Tree
             for (int cb = 0; cb < CB; cb++) {
                 unsigned long long *dst = red + (pc + cb * 8 + gq) * hdp + od;
 #pragma unroll
-                for (int k = 0; k < 8; k += 2) {   // tiles k, k + 1: four outputs in a row
+                for (int k = 0; k < 4; k += 2) {   // tiles k, k + 1: four outputs in a row
                     ulonglong2 *q = reinterpret_cast<ulonglong2 *>(dst + 8 * k);
                     ulonglong2 u = q[0], w = q[1];
                     u.x += (unsigned long long)__double_as_longlong(f[cb][k][0]) - TREE_AB;
@@ -798,10 +794,10 @@ __global__ void __launch_bounds__(256, 2) k_tree_pv(const __grid_constant__ Tree
     }
     __syncthreads();
     for (int e = tid; e < cols * hdp; e += 256) {
-        const int col = e / hdp, d = e - col * hdp, cc = c0 + col;
+        const int col = e / hdp, d = e - col * hdp, cc = c0 + col, n = cc / grp;
         if (d < hd && red[e])
             atomicAdd(reinterpret_cast<unsigned long long *>(a.out) +
-                          ((size_t)(s.row0 + cc / grp) * a.nh + g * grp + cc % grp) * hd + d, red[e]);
+                          ((size_t)(s.row0 + n) * a.nh + g * grp + cc - n * grp) * hd + d, red[e]);
     }
 }
 
