@@ -267,17 +267,18 @@ __device__ __forceinline__ int64_t tree_scale(int64_t s, const TreeScale &c) {
 
 // ---------------------------------------------------------------- 1. scores
 
-#define TREE_A_BYTES 65536   // key planes: two steps of (128 positions x 4 planes x 32 d) x 2
+// key planes of a step: two tiles of 128 positions x 4 planes x 32 d; two steps where several blocks share them
+__host__ __device__ constexpr int tree_a_bytes(int NT) { return 32768 * NT; }
 __host__ __device__ constexpr size_t tree_b_bytes(int NT, int hd) { return (size_t)((hd + 127) / 128) * 64 * NT * 128; }
-__host__ __device__ constexpr size_t tree_scores_smem(int NT, int hd) { return 1024 + TREE_A_BYTES + tree_b_bytes(NT, hd); }
+__host__ __device__ constexpr size_t tree_scores_smem(int NT, int hd) { return 1024 + tree_a_bytes(NT) + tree_b_bytes(NT, hd); }
 
 // A CTA takes a.tpc tiles of 128 positions of one (sequence, kv head) and up to
 // a.passes blocks of NC = 8 NT columns. With hd <= 64 the key planes of a tile are made
 // once for all its blocks, with one block the query planes once for all its tiles.
-// Two CTAs an SM (three with 8 columns) overlap one another's loads, products
+// Two CTAs an SM (four with 8 columns) overlap one another's loads, products
 // and epilogues; TMEM holds 128 NT columns a CTA.
 template <int NT, bool PK, bool W>
-__global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __grid_constant__ TreeArgs a) {
+__global__ void __launch_bounds__(256, NT == 1 ? 4 : 2) k_tree_scores(const __grid_constant__ TreeArgs a) {
     extern __shared__ __align__(16) char tree_smem[];
     constexpr int NC = 8 * NT, HC = NC / 2;
     __shared__ int64_t ksum[128];              // sum of a position's key
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __gr
     const int cols = s.n * grp, T = s.len + s.n, tb0 = tile * a.tpc * 128, te = min(T, tb0 + a.tpc * 128);
     const int p0 = group * a.passes, p1 = min(p0 + a.passes, (cols + NC - 1) / NC);   // column blocks
     if (tb0 >= te || p0 >= p1) return;
-    char *const sA = tree_smem + ((1024 - (smem_u32(tree_smem) & 1023)) & 1023), *const sB = sA + TREE_A_BYTES;
+    char *const sA = tree_smem + ((1024 - (smem_u32(tree_smem) & 1023)) & 1023), *const sB = sA + tree_a_bytes(NT);
 
     // conversion: two threads a position; eight lanes in a row take positions whose
     // swizzles differ, so that their 16-byte stores meet no bank twice
@@ -366,13 +367,13 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __gr
                 if (lane == 0) qsum[col] = qs << 15;
             }
         }
-        const bool made = KS <= 2 && pass > p0;   // the key planes stand
+        const bool made = NT == 2 && KS <= 2 && pass > p0;   // the key planes stand
         for (int ks = 0; ks < KS; ks++, batch++) {
             // the half that this step's planes are in: batch & 1, or, when they stand, where they were made
-            const int half = made ? (made_at + ks) & 1 : batch & 1;
+            const int half = NT == 1 ? 0 : made ? (made_at + ks) & 1 : batch & 1;
             if (!made) {
                 if (ks == 0) made_at = half;
-                if (batch >= 2) mbar_wait(&mbar[batch & 1], (uint32_t)((batch >> 1) - 1) & 1u);
+                if (batch >= NT) mbar_wait(&mbar[(batch - NT) & 1], (uint32_t)((batch - NT) >> 1) & 1u);
                 if (cp < Tl) {
                     int64_t x[16];
 #pragma unroll
@@ -679,12 +680,12 @@ __global__ void __launch_bounds__(TREE_SM_T) k_tree_softmax(const __grid_constan
 // position lane & 3 at d = 16 k + 2 (lane >> 2) + {0, 1}, k < 2, i.e. column lane >> 2 of
 // the 8-wide tiles 2k and 2k + 1, and of each tile's output the columns
 // 2 (lane & 3) + {0, 1}. Values come straight from global memory (the warps of the
-// CG column groups meet them in L1), two steps ahead: nothing is staged and no
+// CG column groups meet them in L1), D steps ahead: nothing is staged and no
 // barrier runs inside the loop.
 template <int CB, bool PK, bool W>
 __global__ void __launch_bounds__(256, 2) k_tree_pv(const __grid_constant__ TreeArgs a) {
     __shared__ __align__(16) unsigned long long red[TREE_RED];
-    constexpr int CW = 8 * CB;
+    constexpr int CW = 8 * CB, D = 2;   // steps ahead
     const int chunk = blockIdx.x % a.chunks, rest = blockIdx.x / a.chunks;
     const int blk = rest % a.cblocks, g = rest / a.cblocks % a.c.nkv, b = rest / a.cblocks / a.c.nkv;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
@@ -717,8 +718,8 @@ __global__ void __launch_bounds__(256, 2) k_tree_pv(const __grid_constant__ Tree
         for (int cb = 0; cb < CB; cb++)
 #pragma unroll
             for (int k = 0; k < 4; k++) f[cb][k][0] = f[cb][k][1] = TREE_A;
-        TreeVals<PK, W> vx[2];
-        double pn[2][CB];
+        TreeVals<PK, W> vx[D];
+        double pn[D][CB];
         auto load = [&](int st, int t0) {   // beyond the end: the last four once more
             const int t = min(t0, tlast);
             vx[st].load(vr, t + tq, db + 2 * gq);
@@ -751,18 +752,19 @@ __global__ void __launch_bounds__(256, 2) k_tree_pv(const __grid_constant__ Tree
                     }
                 }
             }
-            load(st, t0 + 2 * step);
+            load(st, t0 + D * step);
 #pragma unroll
             for (int k = 0; k < 4; k++)
 #pragma unroll
                 for (int cb = 0; cb < CB; cb++) dmma_rd(f[cb][k][0], f[cb][k][1], p[cb], v[k]);
         };
-        load(0, tg * 4);
-        load(1, tg * 4 + step);
+#pragma unroll
+        for (int st = 0; st < D; st++) load(st, tg * 4 + st * step);
 #pragma unroll 1
-        for (int t0 = tg * 4; t0 < Tl; t0 += 2 * step) {
-            four(0, t0);
-            if (t0 + step < Tl) four(1, t0 + step);
+        for (int t0 = tg * 4; t0 < Tl; t0 += D * step) {
+#pragma unroll
+            for (int st = 0; st < D; st++)
+                if (st == 0 || t0 + st * step < Tl) four(st, t0 + st * step);
         }
     };
     tree_prev_kernel();
