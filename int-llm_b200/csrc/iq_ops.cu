@@ -160,6 +160,38 @@ static int launch_tree(const TreeArgs &a, cudaStream_t s) {
                  : tree_launch(k_tree_pv<2, PK, W>, pv, 1, 256, 0, s, true, a);
 }
 
+// CTAs a row (1, 2, 4 or 8): as many as fill the GPU with the rows at hand, but at least
+// 2048 logits a CTA; more where the slice would not fit beside another CTA's (two an
+// SM). A slice beyond one CTA's shared memory is read twice.
+static int lp_launch(LpArgs *a, cudaStream_t s) {
+    static std::atomic<uint64_t> set{0};   // devices whose shared-memory limit is raised
+    const size_t two = 90 * 1024, one = 200 * 1024;
+    int dev = 0;
+    IQ_CUDA(cudaGetDevice(&dev));
+    auto bytes = [&]() { return (size_t)((a->V + a->cs - 1) / a->cs + 1) * 8; };
+    const int sms = dev_info().sms;
+    a->cs = 1;
+    while (a->cs < 8 && (bytes() > two || ((int64_t)a->rows * a->cs < 2 * sms && a->V / a->cs > 4096))) a->cs *= 2;
+    const bool sm = bytes() <= one;
+    if (sm && !(set.load() >> dev & 1)) {
+        IQ_CUDA(cudaFuncSetAttribute(k_logprobs<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)one));
+        set.fetch_or(1ull << dev);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)a->cs;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)((int64_t)a->rows * a->cs));
+    cfg.blockDim = dim3(LP_T);
+    cfg.dynamicSmemBytes = sm ? bytes() : 0;
+    cfg.stream = s;
+    cfg.attrs = at;
+    cfg.numAttrs = a->cs > 1 ? 1 : 0;
+    IQ_CUDA(sm ? cudaLaunchKernelEx(&cfg, k_logprobs<true>, *a) : cudaLaunchKernelEx(&cfg, k_logprobs<false>, *a));
+    return IQ_OK;
+}
+
 extern "C" {
 
 IQ_API int iq_rope_tables_dev(int64_t *d_cos, int64_t *d_sin, int rot_dim, int n_pos, int theta,
@@ -305,14 +337,12 @@ IQ_API int iq_logprobs_dev(const int64_t *d_logits, int64_t ld, int rows, int vo
         (top && (!d_top_ids || !d_top_logp)) || misaligned(d_logits, 8) || misaligned(d_tokens, 4) ||
         misaligned(d_logp, 8) || misaligned(d_entropy, 8) || misaligned(d_top_ids, 4) || misaligned(d_top_logp, 8))
         return IQ_ERR_ARG;
-    if (vocab > (1 << 20) || top > IQ_LP_MAX_TOP) return IQ_ERR_RANGE;
+    if (vocab > (1 << 20) || top > IQ_LP_MAX_TOP || rows > INT_MAX / 8) return IQ_ERR_RANGE;
     if (rows == 0) return IQ_OK;
     int dev, rc;
     if ((rc = cur_device(&dev))) return rc;
-    const LpArgs a = {d_logits, ld, rows, vocab, top, d_tokens, d_logp, d_entropy, d_top_ids, d_top_logp};
-    k_logprobs_simple<<<rows, 1024, 0, pick(stream)>>>(a);
-    IQ_CHECK_LAUNCH();
-    return IQ_OK;
+    LpArgs a = {d_logits, ld, rows, vocab, top, d_tokens, d_logp, d_entropy, d_top_ids, d_top_logp, 1};
+    return lp_launch(&a, pick(stream));
 }
 
 }  // extern "C"

@@ -6,6 +6,11 @@
 
 namespace iq {
 
+// acc += x y, unsigned
+__device__ __forceinline__ void madu(uint64_t &acc, uint32_t x, uint32_t y) {
+    asm("mad.wide.u32 %0, %1, %2, %0;" : "+l"(acc) : "r"(x), "r"(y));
+}
+
 // A bad index of a device array (not the -1 of a padding row): left out and recorded.
 __device__ __forceinline__ bool index_ok(int i, int n) {
     if (i >= 0 && i < n) return true;

@@ -9,6 +9,7 @@
 //   below 2^-46 in all, before the shift.
 //   ln S: log2 of S by 50 squarings of its mantissa, times ln 2.
 #pragma once
+#include <cooperative_groups.h>
 #include "iq_ops.cuh"
 
 namespace iq {
@@ -36,18 +37,30 @@ __constant__ int64_t c_lp_pow[64] = {
     153475319327372ll, 151822085212527ll, 150186659713755ll, 148568850996877ll,
     146968469294152ll, 145385326882014ll, 143819238059052ll, 142270019124227ll};
 
-// floor(e^-d) in Q16.48, d = max - logit as an unsigned difference
-__device__ __forceinline__ int64_t lp_exp(uint64_t d, const int64_t *pw) {
-    if (d >= (34ull << 48)) return 0;
+#define IQ_LP_C0 281474976710656.0   // ln2^i / i! 2^48
+#define IQ_LP_C1 195103586505167.0
+#define IQ_LP_C2 67617750451595.0
+#define IQ_LP_C3 15623017693776.0
+#define IQ_LP_C4 2707262666570.0
+#define IQ_LP_C5 375306296874.0
+
+// E(d) in Q16.48, d = max - logit as an unsigned difference; pw: the table of powers,
+// as doubles. The floors are those of fma.rd in the binade of 2^52 (one unit = one
+// ulp): g = M + floor(h r 2^-48), and c - floor(h r 2^-48) = (c + M) - g exactly.
+__device__ __forceinline__ uint64_t lp_exp(uint64_t d, const double *pw) {
+    const double M = 4503599627370496.0;
     const uint64_t y = __umul64hi(d << 4, (uint64_t)IQ_LP_LOG2E_60);   // (d log2e) >> 60
-    const int64_t f = (int64_t)(y & ((1ull << 48) - 1)), r = f & ((1ll << 42) - 1);
-    int64_t h = 375306296874ll;
-    h = 2707262666570ll - d_mul(h, r);
-    h = 15623017693776ll - d_mul(h, r);
-    h = 67617750451595ll - d_mul(h, r);
-    h = 195103586505167ll - d_mul(h, r);
-    h = 281474976710656ll - d_mul(h, r);
-    return d_mul(pw[f >> 42], h) >> (y >> 48);
+    // r 2^-48 from the low 42 bits of y, j the next 6, k = y >> 48
+    const double r = __hiloint2double((int)(((uint32_t)(y >> 32) & 0x3FF) | 0x43300000), (int)(uint32_t)y) * 0x1p-48 - M * 0x1p-48;
+    double h = IQ_LP_C5;
+    h = (IQ_LP_C4 + M) - __fma_rd(h, r, M);
+    h = (IQ_LP_C3 + M) - __fma_rd(h, r, M);
+    h = (IQ_LP_C2 + M) - __fma_rd(h, r, M);
+    h = (IQ_LP_C1 + M) - __fma_rd(h, r, M);
+    h = (IQ_LP_C0 + M) - __fma_rd(h, r, M);
+    const uint32_t hi = (uint32_t)(y >> 32);
+    const uint64_t e = (uint64_t)__double_as_longlong(__fma_rd(pw[hi >> 10 & 63], h, M)) & 0xFFFFFFFFFFFFFull;   // pw: 2^(-j/64)
+    return d < (34ull << 48) ? e >> (hi >> 16) : 0;
 }
 
 __device__ __forceinline__ int u128_bits(u128 x) {
@@ -89,58 +102,225 @@ struct LpArgs {
     int64_t *logp, *ent;
     int *ids;
     int64_t *tl;
+    int cs;   // CTAs a row
 };
 
-// One CTA a row; the top alternatives by one search of the row for each.
-__global__ void __launch_bounds__(1024) k_logprobs_simple(LpArgs a) {
-    __shared__ uint64_t red[64];
-    __shared__ int64_t bv[32];
-    __shared__ int bi[32];
-    const int row = blockIdx.x;
-    const int64_t *l = a.lg + row * a.ld;
+// A cluster of CTAs takes a row, each a slice of it held in shared memory (SM; else read
+// again, from L2): one pass over the logits from HBM gives the maximum (distributed
+// shared memory joins the slices') and each thread's own maximum, a second one
+// the sums. Alternatives: the n-th largest of 32 groups' maxima is a lower bound
+// of the slice's n-th largest logit; the few logits not below it are ranked by
+// counting. Where more than LP_CAND reach it (many equal logits) the slice is searched
+// n times instead. CTA 0 ranks the slices' lists the same way.
+#define LP_T 512
+#define LP_CAND 1024
+
+__device__ __forceinline__ bool lp_before(int64_t v, int i, int64_t w, int k) { return v > w || (v == w && i < k); }
+
+// The `top` first of n <= cap (value, index) pairs in falling order by counting, into ov, oi (smem)
+__device__ __forceinline__ void lp_rank(const int64_t *v, const int *ix, int n, int top, int64_t *ov, int *oi) {
+    for (int a = threadIdx.x; a < n; a += LP_T) {
+        const int64_t w = v[a];
+        const int k = ix[a];
+        int c = 0;
+        for (int b = 0; b < n; b++) c += lp_before(v[b], ix[b], w, k);
+        if (c < top) { ov[c] = w; oi[c] = k; }
+    }
+}
+
+template <bool SM>
+__global__ void __launch_bounds__(LP_T) k_logprobs(const __grid_constant__ LpArgs a) {
+    namespace cg = cooperative_groups;
+    extern __shared__ __align__(16) int64_t lp_buf[];
+    __shared__ int64_t tmax[LP_T], cv[LP_CAND], lv[IQ_LP_MAX_TOP], gv[8 * IQ_LP_MAX_TOP];
+    __shared__ int ci[LP_CAND], li[IQ_LP_MAX_TOP], gi[8 * IQ_LP_MAX_TOP], cnt, last_i;
+    __shared__ uint64_t wred[4 * (LP_T / 32)], part[4];
+    __shared__ double pw[64];
+    __shared__ int64_t cmax, last_v, tau_s;
+    cg::cluster_group cl = cg::this_cluster();
+    const int cs = a.cs, rank = blockIdx.x % cs, row = blockIdx.x / cs, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t *l = a.lg + (int64_t)row * a.ld;
+    const int per = (a.V + cs - 1) / cs, b0 = min(a.V, rank * per), n = min(per, a.V - b0);
+    const int64_t *x = SM ? lp_buf : l + b0;
+    if (tid < 64) pw[tid] = (double)c_lp_pow[tid] * 0x1p-48;
+    if (tid == 0) cnt = 0;
+
+    // the maximum
     int64_t m = INT64_MIN;
-    for (int i = threadIdx.x; i < a.V; i += blockDim.x) m = max(m, l[i]);
-    m = cta_max_i64(m, (int64_t *)red);
-    u128 S = 0, A = 0;
-    for (int i = threadIdx.x; i < a.V; i += blockDim.x) {
-        const uint64_t d = (uint64_t)m - (uint64_t)l[i];
-        const int64_t e = lp_exp(d, c_lp_pow);
-        S += (uint64_t)e;
-        if (e) A += (uint64_t)d_mul(e, (int64_t)d);
-    }
-    S = (u128)cta_sum_i128((i128)S, red);
-    A = (u128)cta_sum_i128((i128)A, red);
-    const int64_t z = lp_ln(S);
-    if (threadIdx.x == 0) {
-        if (a.tok && index_ok(a.tok[row], a.V)) a.logp[row] = lp_of((uint64_t)m - (uint64_t)l[a.tok[row]], z);
-        if (a.ent) a.ent[row] = lp_entropy(S, A, z);
-    }
-    int64_t pv = INT64_MAX;
-    int pi = -1;
-    for (int k = 0; k < a.top; k++) {   // the first after (pv, pi) in falling value, rising index
-        int64_t best = INT64_MIN;
-        int idx = 0x7fffffff;
-        for (int i = threadIdx.x; i < a.V; i += blockDim.x) {
-            const int64_t v = l[i];
-            if ((v < pv || (v == pv && i > pi)) && (v > best || (v == best && i < idx))) { best = v; idx = i; }
+    const int64_t *src = l + b0;
+    const int skew = (int)(((uintptr_t)src >> 3) & 1);   // pairs from the first 16-byte boundary on
+    const longlong2 *s2 = reinterpret_cast<const longlong2 *>(src + skew);
+    const int n2 = n > skew ? (n - skew) >> 1 : 0;
+    for (int i0 = 0; i0 < n2; i0 += 4 * LP_T) {
+        longlong2 u[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int i = i0 + k * LP_T + tid;
+            u[k] = i < n2 ? __ldg(s2 + i) : make_longlong2(INT64_MIN, INT64_MIN);
         }
-        for (int o = 16; o >= 1; o >>= 1) {
-            const int64_t ov = __shfl_xor_sync(0xffffffffu, best, o);
-            const int oi = __shfl_xor_sync(0xffffffffu, idx, o);
-            if (ov > best || (ov == best && oi < idx)) { best = ov; idx = oi; }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int i = i0 + k * LP_T + tid;
+            m = max(m, (int64_t)max(u[k].x, u[k].y));
+            if (SM && i < n2) {   // in pairs, the skewed first element behind the last pair
+                reinterpret_cast<longlong2 *>(lp_buf)[i] = u[k];
+            }
+        }
+    }
+    const int odd = n - 2 * n2;   // 0 .. 2 elements outside the pairs: the first (skew) and the last
+    int64_t ov = INT64_MIN;
+    if (tid < odd) {
+        const int i = skew && n > 0 && tid == 0 ? 0 : n - 1;
+        ov = __ldg(src + i);
+        if (SM) lp_buf[2 * n2 + tid] = ov;
+        m = max(m, ov);
+    }
+    // where element i of the buffer stands in the row
+    auto at = [&](int i) { return SM ? (i < 2 * n2 ? b0 + skew + i : b0 + (skew && i == 2 * n2 ? 0 : n - 1)) : b0 + i; };
+    tmax[tid] = m;
+    for (int k = 16; k >= 1; k >>= 1) m = max(m, (int64_t)__shfl_xor_sync(0xffffffffu, m, k));
+    if (lane == 0) wred[warp] = (uint64_t)m;
+    __syncthreads();
+    m = (int64_t)wred[0];
+#pragma unroll
+    for (int k = 1; k < LP_T / 32; k++) m = max(m, (int64_t)wred[k]);
+    if (tid == 0) cmax = m;
+    if (cs > 1) {
+        cl.sync();
+        int64_t o = lane < cs ? *cl.map_shared_rank(&cmax, lane) : INT64_MIN;
+        for (int k = 4; k >= 1; k >>= 1) o = max(o, (int64_t)__shfl_xor_sync(0xffffffffu, o, k));
+        m = __shfl_sync(0xffffffffu, o, 0);
+    }
+
+    // the sums: S and A in two words each (a thread's own stay below 2^64: at most 2^15 terms of 2^48)
+    uint64_t S = 0, A = 0, Sh = 0, Ah = 0;
+    const bool ent = a.ent != nullptr;
+    for (int i0 = 0; i0 < n; i0 += 4 * LP_T) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int i = i0 + k * LP_T + tid;
+            if (i < n) {
+                const uint64_t d = (uint64_t)m - (uint64_t)x[i], e = lp_exp(d, pw);
+                S += e;
+                if (ent) {   // floor(e d / 2^48), e <= 2^48 and 0 from d = 34 on: from 32-bit pieces
+                    const uint32_t el = (uint32_t)e, eh = (uint32_t)(e >> 32), dl = (uint32_t)d, dh = (uint32_t)(d >> 32);
+                    uint64_t t = __umulhi(el, dl);
+                    madu(t, eh, dl);
+                    madu(t, el, dh);
+                    uint64_t w = t >> 16;
+                    madu(w, eh << 8, dh << 8);
+                    A += w;
+                }
+            }
+        }
+    }
+    Sh = S >> 32;
+    S &= 0xFFFFFFFFull;
+    Ah = A >> 32;
+    A &= 0xFFFFFFFFull;
+    for (int k = 16; k >= 1; k >>= 1) {
+        S += __shfl_xor_sync(0xffffffffu, S, k);
+        Sh += __shfl_xor_sync(0xffffffffu, Sh, k);
+        A += __shfl_xor_sync(0xffffffffu, A, k);
+        Ah += __shfl_xor_sync(0xffffffffu, Ah, k);
+    }
+    __syncthreads();
+    if (lane == 0) { wred[4 * warp] = S; wred[4 * warp + 1] = Sh; wred[4 * warp + 2] = A; wred[4 * warp + 3] = Ah; }
+    // the bound for the alternatives: the top-th largest of 32 maxima of LP_T / 32 threads each
+    const int top = min(a.top, n);
+    if (warp == 0 && top) {
+        int64_t g = INT64_MIN;
+        for (int k = 0; k < LP_T / 32; k++) g = max(g, tmax[k * 32 + lane]);
+        int c = 0;
+        for (int k = 0; k < 32; k++) {
+            const int64_t o = __shfl_sync(0xffffffffu, g, k);
+            c += lp_before(o, k, g, lane);
+        }
+        if (c == top - 1) tau_s = g;
+    }
+    __syncthreads();
+    if (tid < 4) {
+        uint64_t t = 0;
+        for (int k = 0; k < LP_T / 32; k++) t += wred[4 * k + tid];
+        part[tid] = t;
+    }
+    if (top) {
+        const int64_t tau = tau_s;
+        for (int i = tid; i < n; i += LP_T) {
+            const int64_t v = x[i];
+            if (v >= tau) {
+                const int c = atomicAdd(&cnt, 1);
+                if (c < LP_CAND) { cv[c] = v; ci[c] = at(i); }
+            }
         }
         __syncthreads();
-        if ((threadIdx.x & 31) == 0) { bv[threadIdx.x >> 5] = best; bi[threadIdx.x >> 5] = idx; }
-        __syncthreads();
-        for (int w = 0; w < 32; w++)
-            if (bv[w] > best || (bv[w] == best && bi[w] < idx)) { best = bv[w]; idx = bi[w]; }
-        if (threadIdx.x == 0) {
-            a.ids[(size_t)row * a.top + k] = idx;
-            a.tl[(size_t)row * a.top + k] = lp_of((uint64_t)m - (uint64_t)best, z);
+        if (cnt <= LP_CAND) {
+            lp_rank(cv, ci, cnt, top, lv, li);
+        } else {
+            int64_t pv = INT64_MAX;
+            int pi = -1;
+            for (int k = 0; k < top; k++) {   // the first after (pv, pi)
+                int64_t best = INT64_MIN;
+                int idx = 0x7fffffff;
+                for (int i = tid; i < n; i += LP_T) {
+                    const int64_t v = x[i];
+                    const int p = at(i);
+                    if (lp_before(pv, pi, v, p) && (idx == 0x7fffffff || lp_before(v, p, best, idx))) { best = v; idx = p; }
+                }
+                for (int o = 16; o >= 1; o >>= 1) {
+                    const int64_t w = __shfl_xor_sync(0xffffffffu, best, o);
+                    const int j = __shfl_xor_sync(0xffffffffu, idx, o);
+                    if (lp_before(w, j, best, idx)) { best = w; idx = j; }
+                }
+                __syncthreads();
+                if (lane == 0) { cv[warp] = best; ci[warp] = idx; }
+                __syncthreads();
+                if (tid == 0) {
+                    for (int w = 1; w < LP_T / 32; w++)
+                        if (lp_before(cv[w], ci[w], best, idx)) { best = cv[w]; idx = ci[w]; }
+                    lv[k] = last_v = best;
+                    li[k] = last_i = idx;
+                }
+                __syncthreads();
+                pv = last_v;
+                pi = last_i;
+            }
         }
-        pv = best;
-        pi = idx;
     }
+    if (tid >= top && tid < IQ_LP_MAX_TOP) { lv[tid] = INT64_MIN; li[tid] = 0x7fffffff; }   // a short slice's missing ones
+    if (cs > 1) cl.sync();
+    else __syncthreads();
+    if (rank == 0) {
+        if (cs > 1) {
+            for (int e = tid; e < cs * a.top; e += LP_T) {
+                const int r = e / a.top, k = e - r * a.top;
+                gv[e] = cl.map_shared_rank(lv, r)[k];
+                gi[e] = cl.map_shared_rank(li, r)[k];
+            }
+            if (tid >= 32 && tid < 36) {
+                uint64_t t = 0;
+                for (int r = 0; r < cs; r++) t += cl.map_shared_rank(part, r)[tid - 32];
+                wred[tid - 32] = t;
+            }
+        } else {
+            if (tid < a.top) { gv[tid] = lv[tid]; gi[tid] = li[tid]; }
+            if (tid >= 32 && tid < 36) wred[tid - 32] = part[tid - 32];
+        }
+        __syncthreads();
+        if (cs > 1) lp_rank(gv, gi, cs * a.top, a.top, cv, ci);
+        const u128 St = ((u128)wred[1] << 32) + wred[0];
+        if (cs > 1) __syncthreads();
+        if (warp < 2) {
+            const int64_t z = lp_ln(St);
+            if (tid == 32 && a.tok && index_ok(a.tok[row], a.V)) a.logp[row] = lp_of((uint64_t)m - (uint64_t)l[a.tok[row]], z);
+            if (tid == 33 && ent) a.ent[row] = lp_entropy(St, ((u128)wred[3] << 32) + wred[2], z);
+            if (tid < a.top) {
+                a.ids[(size_t)row * a.top + tid] = cs > 1 ? ci[tid] : gi[tid];
+                a.tl[(size_t)row * a.top + tid] = lp_of((uint64_t)m - (uint64_t)(cs > 1 ? cv[tid] : gv[tid]), z);
+            }
+        }
+    }
+    if (cs > 1) cl.sync();   // CTA 0 has read the others' lists and sums
 }
 
 }  // namespace iq

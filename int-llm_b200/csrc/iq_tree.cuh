@@ -228,10 +228,6 @@ __device__ __forceinline__ void tmem_zero4(uint32_t taddr) {
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // this thread's shared-memory writes before the tensor cores' reads
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void madu(uint64_t &acc, uint32_t x, uint32_t y) {
-    asm("mad.wide.u32 %0, %1, %2, %0;" : "+l"(acc) : "r"(x), "r"(y));
-}
-
 // Range check from the high words, gathered with a maximum: hi + b as unsigned stays
 // below 2b exactly when -b <= hi < b.
 __device__ __forceinline__ void tree_hi(uint32_t &m, int64_t x, uint32_t b) { m = max(m, (uint32_t)(x >> 32) + b); }
