@@ -161,18 +161,18 @@ static int launch_tree(const TreeArgs &a, cudaStream_t s) {
 }
 
 // CTAs a row (1, 2, 4 or 8): as many as fill the GPU with the rows at hand, but at least
-// 2048 logits a CTA; more where the slice would not fit beside another CTA's (two an
-// SM). A slice beyond one CTA's shared memory is read twice.
+// 2048 logits a CTA; more where the slices of five CTAs would not fit an SM. A slice beyond one CTA's shared memory is read twice.
 static int lp_launch(LpArgs *a, cudaStream_t s) {
     static std::atomic<uint64_t> set{0};   // devices whose shared-memory limit is raised
-    const size_t two = 90 * 1024, one = 200 * 1024;
+    const size_t many = 36 * 1024, one = 200 * 1024;
     int dev = 0;
     IQ_CUDA(cudaGetDevice(&dev));
     auto bytes = [&]() { return (size_t)((a->V + a->cs - 1) / a->cs + 1) * 8; };
     const int sms = dev_info().sms;
     a->cs = 1;
-    while (a->cs < 8 && (bytes() > two || ((int64_t)a->rows * a->cs < 2 * sms && a->V / a->cs > 4096))) a->cs *= 2;
-    const bool sm = bytes() <= one;
+    const bool full = a->rows >= 2 * sms;   // one CTA a row keeps every SM busy
+    while (!full && a->cs < 8 && (bytes() > many || ((int64_t)a->rows * a->cs < 4 * sms && a->V / a->cs > 4096))) a->cs *= 2;
+    const bool sm = bytes() <= (full ? many : one);
     if (sm && !(set.load() >> dev & 1)) {
         IQ_CUDA(cudaFuncSetAttribute(k_logprobs<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)one));
         set.fetch_or(1ull << dev);

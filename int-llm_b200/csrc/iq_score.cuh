@@ -49,7 +49,13 @@ __constant__ int64_t c_lp_pow[64] = {
 // ulp): g = M + floor(h r 2^-48), and c - floor(h r 2^-48) = (c + M) - g exactly.
 __device__ __forceinline__ uint64_t lp_exp(uint64_t d, const double *pw) {
     const double M = 4503599627370496.0;
-    const uint64_t y = __umul64hi(d << 4, (uint64_t)IQ_LP_LOG2E_60);   // (d log2e) >> 60
+    // y = d log2e >> 60 from 32-bit pieces (d < 2^54, log2e < 2^61)
+    const uint32_t dl = (uint32_t)d, dh = (uint32_t)(d >> 32);
+    uint64_t y = __umulhi(dl, (uint32_t)IQ_LP_LOG2E_60);
+    madu(y, dh, (uint32_t)IQ_LP_LOG2E_60);
+    madu(y, dl, (uint32_t)(IQ_LP_LOG2E_60 >> 32));
+    y >>= 28;
+    madu(y, dh << 4, (uint32_t)(IQ_LP_LOG2E_60 >> 32));
     // r 2^-48 from the low 42 bits of y, j the next 6, k = y >> 48
     const double r = __hiloint2double((int)(((uint32_t)(y >> 32) & 0x3FF) | 0x43300000), (int)(uint32_t)y) * 0x1p-48 - M * 0x1p-48;
     double h = IQ_LP_C5;
@@ -60,7 +66,7 @@ __device__ __forceinline__ uint64_t lp_exp(uint64_t d, const double *pw) {
     h = (IQ_LP_C0 + M) - __fma_rd(h, r, M);
     const uint32_t hi = (uint32_t)(y >> 32);
     const uint64_t e = (uint64_t)__double_as_longlong(__fma_rd(pw[hi >> 10 & 63], h, M)) & 0xFFFFFFFFFFFFFull;   // pw: 2^(-j/64)
-    return d < (34ull << 48) ? e >> (hi >> 16) : 0;
+    return dh < (34u << 16) ? e >> (hi >> 16) : 0;
 }
 
 __device__ __forceinline__ int u128_bits(u128 x) {
@@ -112,8 +118,8 @@ struct LpArgs {
 // of the slice's n-th largest logit; the few logits not below it are ranked by
 // counting. Where more than LP_CAND reach it (many equal logits) the slice is searched
 // n times instead. CTA 0 ranks the slices' lists the same way.
-#define LP_T 512
-#define LP_CAND 1024
+#define LP_T 256
+#define LP_CAND 512
 
 __device__ __forceinline__ bool lp_before(int64_t v, int i, int64_t w, int k) { return v > w || (v == w && i < k); }
 
@@ -141,7 +147,6 @@ __global__ void __launch_bounds__(LP_T) k_logprobs(const __grid_constant__ LpArg
     const int cs = a.cs, rank = blockIdx.x % cs, row = blockIdx.x / cs, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t *l = a.lg + (int64_t)row * a.ld;
     const int per = (a.V + cs - 1) / cs, b0 = min(a.V, rank * per), n = min(per, a.V - b0);
-    const int64_t *x = SM ? lp_buf : l + b0;
     if (tid < 64) pw[tid] = (double)c_lp_pow[tid] * 0x1p-48;
     if (tid == 0) cnt = 0;
 
@@ -162,9 +167,7 @@ __global__ void __launch_bounds__(LP_T) k_logprobs(const __grid_constant__ LpArg
         for (int k = 0; k < 4; k++) {
             const int i = i0 + k * LP_T + tid;
             m = max(m, (int64_t)max(u[k].x, u[k].y));
-            if (SM && i < n2) {   // in pairs, the skewed first element behind the last pair
-                reinterpret_cast<longlong2 *>(lp_buf)[i] = u[k];
-            }
+            if (SM && i < n2) reinterpret_cast<longlong2 *>(lp_buf)[i] = u[k];
         }
     }
     const int odd = n - 2 * n2;   // 0 .. 2 elements outside the pairs: the first (skew) and the last
@@ -172,11 +175,29 @@ __global__ void __launch_bounds__(LP_T) k_logprobs(const __grid_constant__ LpArg
     if (tid < odd) {
         const int i = skew && n > 0 && tid == 0 ? 0 : n - 1;
         ov = __ldg(src + i);
-        if (SM) lp_buf[2 * n2 + tid] = ov;
         m = max(m, ov);
     }
-    // where element i of the buffer stands in the row
-    auto at = [&](int i) { return SM ? (i < 2 * n2 ? b0 + skew + i : b0 + (skew && i == 2 * n2 ? 0 : n - 1)) : b0 + i; };
+    const longlong2 *x2 = SM ? reinterpret_cast<const longlong2 *>(lp_buf) : s2;
+    // f(logit, its place in the row) for each of the thread's logits
+    auto each = [&](auto f) {
+        int i = tid;
+        for (; i + 3 * LP_T < n2; i += 4 * LP_T) {
+            longlong2 u[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) u[k] = x2[i + k * LP_T];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                f(u[k].x, b0 + skew + 2 * (i + k * LP_T));
+                f(u[k].y, b0 + skew + 2 * (i + k * LP_T) + 1);
+            }
+        }
+        for (; i < n2; i += LP_T) {
+            const longlong2 u = x2[i];
+            f(u.x, b0 + skew + 2 * i);
+            f(u.y, b0 + skew + 2 * i + 1);
+        }
+        if (tid < odd) f(ov, b0 + (skew && tid == 0 ? 0 : n - 1));
+    };
     tmax[tid] = m;
     for (int k = 16; k >= 1; k >>= 1) m = max(m, (int64_t)__shfl_xor_sync(0xffffffffu, m, k));
     if (lane == 0) wred[warp] = (uint64_t)m;
@@ -185,47 +206,6 @@ __global__ void __launch_bounds__(LP_T) k_logprobs(const __grid_constant__ LpArg
 #pragma unroll
     for (int k = 1; k < LP_T / 32; k++) m = max(m, (int64_t)wred[k]);
     if (tid == 0) cmax = m;
-    if (cs > 1) {
-        cl.sync();
-        int64_t o = lane < cs ? *cl.map_shared_rank(&cmax, lane) : INT64_MIN;
-        for (int k = 4; k >= 1; k >>= 1) o = max(o, (int64_t)__shfl_xor_sync(0xffffffffu, o, k));
-        m = __shfl_sync(0xffffffffu, o, 0);
-    }
-
-    // the sums: S and A in two words each (a thread's own stay below 2^64: at most 2^15 terms of 2^48)
-    uint64_t S = 0, A = 0, Sh = 0, Ah = 0;
-    const bool ent = a.ent != nullptr;
-    for (int i0 = 0; i0 < n; i0 += 4 * LP_T) {
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int i = i0 + k * LP_T + tid;
-            if (i < n) {
-                const uint64_t d = (uint64_t)m - (uint64_t)x[i], e = lp_exp(d, pw);
-                S += e;
-                if (ent) {   // floor(e d / 2^48), e <= 2^48 and 0 from d = 34 on: from 32-bit pieces
-                    const uint32_t el = (uint32_t)e, eh = (uint32_t)(e >> 32), dl = (uint32_t)d, dh = (uint32_t)(d >> 32);
-                    uint64_t t = __umulhi(el, dl);
-                    madu(t, eh, dl);
-                    madu(t, el, dh);
-                    uint64_t w = t >> 16;
-                    madu(w, eh << 8, dh << 8);
-                    A += w;
-                }
-            }
-        }
-    }
-    Sh = S >> 32;
-    S &= 0xFFFFFFFFull;
-    Ah = A >> 32;
-    A &= 0xFFFFFFFFull;
-    for (int k = 16; k >= 1; k >>= 1) {
-        S += __shfl_xor_sync(0xffffffffu, S, k);
-        Sh += __shfl_xor_sync(0xffffffffu, Sh, k);
-        A += __shfl_xor_sync(0xffffffffu, A, k);
-        Ah += __shfl_xor_sync(0xffffffffu, Ah, k);
-    }
-    __syncthreads();
-    if (lane == 0) { wred[4 * warp] = S; wred[4 * warp + 1] = Sh; wred[4 * warp + 2] = A; wred[4 * warp + 3] = Ah; }
     // the bound for the alternatives: the top-th largest of 32 maxima of LP_T / 32 threads each
     const int top = min(a.top, n);
     if (warp == 0 && top) {
@@ -238,6 +218,48 @@ __global__ void __launch_bounds__(LP_T) k_logprobs(const __grid_constant__ LpArg
         }
         if (c == top - 1) tau_s = g;
     }
+    if (cs > 1) {
+        cl.sync();
+        int64_t o = lane < cs ? *cl.map_shared_rank(&cmax, lane) : INT64_MIN;
+        for (int k = 4; k >= 1; k >>= 1) o = max(o, (int64_t)__shfl_xor_sync(0xffffffffu, o, k));
+        m = __shfl_sync(0xffffffffu, o, 0);
+    } else {
+        __syncthreads();
+    }
+
+    // the sums: S and A in two words each (a thread's own stay below 2^64: at most 2^15 terms of 2^48)
+    uint64_t S = 0, A = 0, Sh = 0, Ah = 0;
+    const bool ent = a.ent != nullptr;
+    const int64_t tau = top ? tau_s : INT64_MAX;
+    each([&](int64_t v, int i) {
+        const uint64_t d = (uint64_t)m - (uint64_t)v, e = lp_exp(d, pw);
+        S += e;
+        if (ent) {   // floor(e d / 2^48), e <= 2^48 and 0 from d = 34 on: from 32-bit pieces
+            const uint32_t el = (uint32_t)e, eh = (uint32_t)(e >> 32), dl = (uint32_t)d, dh = (uint32_t)(d >> 32);
+            uint64_t t = __umulhi(el, dl);
+            madu(t, eh, dl);
+            madu(t, el, dh);
+            t >>= 16;
+            madu(t, eh << 8, dh << 8);
+            A += t;
+        }
+        if (v >= tau && top) {
+            const int c = atomicAdd(&cnt, 1);
+            if (c < LP_CAND) { cv[c] = v; ci[c] = i; }
+        }
+    });
+    Sh = S >> 32;
+    S &= 0xFFFFFFFFull;
+    Ah = A >> 32;
+    A &= 0xFFFFFFFFull;
+    for (int k = 16; k >= 1; k >>= 1) {
+        S += __shfl_xor_sync(0xffffffffu, S, k);
+        Sh += __shfl_xor_sync(0xffffffffu, Sh, k);
+        A += __shfl_xor_sync(0xffffffffu, A, k);
+        Ah += __shfl_xor_sync(0xffffffffu, Ah, k);
+    }
+    __syncthreads();
+    if (lane == 0) { wred[4 * warp] = S; wred[4 * warp + 1] = Sh; wred[4 * warp + 2] = A; wred[4 * warp + 3] = Ah; }
     __syncthreads();
     if (tid < 4) {
         uint64_t t = 0;
@@ -245,15 +267,6 @@ __global__ void __launch_bounds__(LP_T) k_logprobs(const __grid_constant__ LpArg
         part[tid] = t;
     }
     if (top) {
-        const int64_t tau = tau_s;
-        for (int i = tid; i < n; i += LP_T) {
-            const int64_t v = x[i];
-            if (v >= tau) {
-                const int c = atomicAdd(&cnt, 1);
-                if (c < LP_CAND) { cv[c] = v; ci[c] = at(i); }
-            }
-        }
-        __syncthreads();
         if (cnt <= LP_CAND) {
             lp_rank(cv, ci, cnt, top, lv, li);
         } else {
@@ -262,11 +275,9 @@ __global__ void __launch_bounds__(LP_T) k_logprobs(const __grid_constant__ LpArg
             for (int k = 0; k < top; k++) {   // the first after (pv, pi)
                 int64_t best = INT64_MIN;
                 int idx = 0x7fffffff;
-                for (int i = tid; i < n; i += LP_T) {
-                    const int64_t v = x[i];
-                    const int p = at(i);
+                each([&](int64_t v, int p) {
                     if (lp_before(pv, pi, v, p) && (idx == 0x7fffffff || lp_before(v, p, best, idx))) { best = v; idx = p; }
-                }
+                });
                 for (int o = 16; o >= 1; o >>= 1) {
                     const int64_t w = __shfl_xor_sync(0xffffffffu, best, o);
                     const int j = __shfl_xor_sync(0xffffffffu, idx, o);
@@ -306,21 +317,24 @@ __global__ void __launch_bounds__(LP_T) k_logprobs(const __grid_constant__ LpArg
             if (tid < a.top) { gv[tid] = lv[tid]; gi[tid] = li[tid]; }
             if (tid >= 32 && tid < 36) wred[tid - 32] = part[tid - 32];
         }
+    }
+    if (cs > 1) cl.sync();   // CTA 0 holds the others' lists and sums: they are done
+    else __syncthreads();
+    if (rank != 0) return;
+    if (cs > 1) {
+        lp_rank(gv, gi, cs * a.top, a.top, cv, ci);
         __syncthreads();
-        if (cs > 1) lp_rank(gv, gi, cs * a.top, a.top, cv, ci);
-        const u128 St = ((u128)wred[1] << 32) + wred[0];
-        if (cs > 1) __syncthreads();
-        if (warp < 2) {
-            const int64_t z = lp_ln(St);
-            if (tid == 32 && a.tok && index_ok(a.tok[row], a.V)) a.logp[row] = lp_of((uint64_t)m - (uint64_t)l[a.tok[row]], z);
-            if (tid == 33 && ent) a.ent[row] = lp_entropy(St, ((u128)wred[3] << 32) + wred[2], z);
-            if (tid < a.top) {
-                a.ids[(size_t)row * a.top + tid] = cs > 1 ? ci[tid] : gi[tid];
-                a.tl[(size_t)row * a.top + tid] = lp_of((uint64_t)m - (uint64_t)(cs > 1 ? cv[tid] : gv[tid]), z);
-            }
+    }
+    const u128 St = ((u128)wred[1] << 32) + wred[0];
+    if (warp < 2) {
+        const int64_t z = lp_ln(St);
+        if (tid == 32 && a.tok && index_ok(a.tok[row], a.V)) a.logp[row] = lp_of((uint64_t)m - (uint64_t)l[a.tok[row]], z);
+        if (tid == 33 && ent) a.ent[row] = lp_entropy(St, ((u128)wred[3] << 32) + wred[2], z);
+        if (tid < a.top) {
+            a.ids[(size_t)row * a.top + tid] = cs > 1 ? ci[tid] : gi[tid];
+            a.tl[(size_t)row * a.top + tid] = lp_of((uint64_t)m - (uint64_t)(cs > 1 ? cv[tid] : gv[tid]), z);
         }
     }
-    if (cs > 1) cl.sync();   // CTA 0 has read the others' lists and sums
 }
 
 }  // namespace iq
