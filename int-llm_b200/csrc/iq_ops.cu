@@ -49,6 +49,36 @@ static int64_t h_att_scale(int hd) {
     return y >> k;
 }
 
+// fp_math_init (fp_math.h:785-858): pi by Machin, atan(2^-i), the CORDIC gain
+static int64_t h_atan(int64_t x, int terms) {
+    const int64_t x2 = h_mul(x, x);
+    int64_t t = x, s = x;
+    for (int n = 1; n <= terms; n++) {
+        t = -h_mul(t, x2);
+        const int64_t c = t / (2 * n + 1);
+        if (c == 0) break;
+        s += c;
+    }
+    return s;
+}
+struct HostCordic {
+    int64_t pi, gain, angles[25];
+    HostCordic() {
+        pi = (h_atan(IQ_ONE / 5, 40) << 4) - (h_atan(IQ_ONE / 239, 15) << 2);
+        angles[0] = pi >> 2;
+        for (int i = 1; i < 25; i++) angles[i] = h_atan(IQ_ONE >> i, 40);
+        int64_t k = IQ_ONE;
+        for (int i = 0; i < 48; i++) k = h_mul(k, IQ_ONE + (2 * i < 63 ? IQ_ONE >> (2 * i) : 0));
+        // fp_sqrt (fp_math.h:624-650): the largest r with r^2 <= k 2^48, bit by bit
+        int64_t r = 0;
+        for (int b = 50; b >= 0; b--) {
+            const int64_t c = r | (int64_t)1 << b;
+            if ((i128)c * c <= (i128)k << 48) r = c;
+        }
+        gain = (int64_t)(((i128)IQ_ONE << 48) / r);
+    }
+};
+
 static int rope_check(const iq_rope *r, int hd, RopeArgs *a) {
     if (!r || !r->d_cos || !r->d_sin || !r->d_pos || r->n_pos < 1 || r->rot_dim < 2 || (r->rot_dim & 1) ||
         r->rot_dim > hd || (r->layout != IQ_ROPE_HALF && r->layout != IQ_ROPE_INTERLEAVED))
@@ -56,6 +86,11 @@ static int rope_check(const iq_rope *r, int hd, RopeArgs *a) {
     if (misaligned(r->d_cos, 8) || misaligned(r->d_sin, 8) || misaligned(r->d_pos, 4)) return IQ_ERR_ARG;
     *a = RopeArgs{r->d_cos, r->d_sin, r->d_pos, r->n_pos, r->rot_dim, r->layout};
     return IQ_OK;
+}
+
+// the 16-byte form: whole items of four elements, aligned tables
+static bool rope_wide(const RopeArgs &r, int hd) {
+    return hd % 4 == 0 && r.rot % 4 == 0 && !misaligned(r.cos, 16) && !misaligned(r.sin, 16);
 }
 
 static int cache_check(const iq_kv_cache *c, KVArgs *a) {
@@ -199,7 +234,9 @@ IQ_API int iq_rope_tables_dev(int64_t *d_cos, int64_t *d_sin, int rot_dim, int n
     if (!d_cos || !d_sin || misaligned(d_cos, 8) || misaligned(d_sin, 8) || rot_dim < 2 || rot_dim > 256 ||
         (rot_dim & 1) || n_pos < 1 || n_pos > (1 << 24) || theta < 1)
         return IQ_ERR_ARG;
-    RopeTab t = {rot_dim / 2, rot_dim, n_pos, IQ_ROPE_SCALE_NONE, 0, h_ln_int(theta), IQ_ONE, 0, IQ_ONE, 0};
+    static const HostCordic hc;
+    RopeTab t = {rot_dim / 2, rot_dim, n_pos, IQ_ROPE_SCALE_NONE, 0, h_ln_int(theta), IQ_ONE, 0, IQ_ONE, 0, hc.pi, hc.gain, {}};
+    std::copy(hc.angles, hc.angles + 25, t.angles);
     if (sc) {
         if (sc->kind < IQ_ROPE_SCALE_NONE || sc->kind > IQ_ROPE_SCALE_PARTS || sc->mscale < 0 ||
             sc->mscale > 1024 * IQ_ONE)
@@ -241,11 +278,14 @@ IQ_API int iq_rope_dev(int64_t *d_out, const int64_t *d_x, const iq_rope *rope, 
     if ((rc = rope_check(rope, head_dim, &r))) return rc;
     if (rows == 0) return IQ_OK;
     if ((rc = cur_device(&dev))) return rc;
-    const int items = heads * ((head_dim + 1) / 2);
+    const bool wide = rope_wide(r, head_dim) && !misaligned(d_x, 16) && !misaligned(d_out, 16) && x_stride % 2 == 0 &&
+                      out_stride % 2 == 0;
+    const int items = heads * (wide ? head_dim / 4 : (head_dim + 1) / 2);
     int tx = 256;
     while (tx > 32 && tx / 2 >= items) tx /= 2;
     const dim3 block(tx, 256 / tx), grid((rows + block.y - 1) / block.y, std::min(64, (items + tx - 1) / tx));
-    k_rope<<<grid, block, 0, pick(stream)>>>(d_out, d_x, r, rows, heads, head_dim, x_stride, out_stride);
+    if (wide) k_rope<true><<<grid, block, 0, pick(stream)>>>(d_out, d_x, r, rows, heads, head_dim, x_stride, out_stride);
+    else k_rope<false><<<grid, block, 0, pick(stream)>>>(d_out, d_x, r, rows, heads, head_dim, x_stride, out_stride);
     IQ_CHECK_LAUNCH();
     return IQ_OK;
 }
@@ -264,11 +304,25 @@ IQ_API int iq_kv_write_dev(const iq_kv_cache *cache, const int64_t *d_k, const i
     if (rope && (rc = rope_check(rope, c.hd, &r))) return rc;
     if (rows == 0) return IQ_OK;
     if ((rc = cur_device(&dev))) return rc;
-    const int blocks = (int)(((int64_t)rows * c.nkv * 2 + 7) / 8);
-    if (c.kbits)
-        k_kv_write<true><<<blocks, 256, 0, pick(stream)>>>(c, d_k, d_v, d_seq, d_slot, rows, k_stride, v_stride, r);
-    else
-        k_kv_write<false><<<blocks, 256, 0, pick(stream)>>>(c, d_k, d_v, d_seq, d_slot, rows, k_stride, v_stride, r);
+    const int64_t vecs = (int64_t)rows * c.nkv * 2;
+    cudaStream_t st = pick(stream);
+    const bool wide = rope_wide(r, c.hd) && !misaligned(d_k, 16) && !misaligned(d_v, 16) && k_stride % 2 == 0 && v_stride % 2 == 0 &&
+                      (c.kbits ? !misaligned(c.kq, 2) && !misaligned(c.vq, 4) : !misaligned(c.k, 16) && !misaligned(c.v, 16));
+    if (wide) {
+        int log_l = 0;   // lanes a vector
+        while (log_l < 5 && 1 << log_l < c.hd / 4) log_l++;
+        const int blocks = (int)(((vecs << log_l) + 255) / 256);
+        if (c.kbits)
+            k_kv_write_wide<true><<<blocks, 256, 0, st>>>(c, d_k, d_v, d_seq, d_slot, rows, k_stride, v_stride, r, log_l);
+        else
+            k_kv_write_wide<false><<<blocks, 256, 0, st>>>(c, d_k, d_v, d_seq, d_slot, rows, k_stride, v_stride, r, log_l);
+    } else {
+        const int blocks = (int)((vecs + 7) / 8);
+        if (c.kbits)
+            k_kv_write<true><<<blocks, 256, 0, st>>>(c, d_k, d_v, d_seq, d_slot, rows, k_stride, v_stride, r);
+        else
+            k_kv_write<false><<<blocks, 256, 0, st>>>(c, d_k, d_v, d_seq, d_slot, rows, k_stride, v_stride, r);
+    }
     IQ_CHECK_LAUNCH();
     return IQ_OK;
 }
@@ -283,8 +337,12 @@ IQ_API int iq_kv_read_dev(int64_t *d_k, int64_t *d_v, const iq_kv_cache *cache, 
         return IQ_ERR_ARG;
     if (rows == 0) return IQ_OK;
     if ((rc = cur_device(&dev))) return rc;
-    const int blocks = (int)(((int64_t)rows * c.nkv * 2 + 7) / 8);
-    k_kv_read<<<blocks, 256, 0, pick(stream)>>>(d_k, d_v, c, d_seq, d_slot, rows);
+    const bool wide = c.hd % 4 == 0 && !misaligned(d_k, 16) && !misaligned(d_v, 16) &&
+                      (c.kbits ? !misaligned(c.kq, 4) && !misaligned(c.vq, 8) : !misaligned(c.k, 16) && !misaligned(c.v, 16));
+    const int64_t blocks = ((int64_t)rows * c.nkv * 2 * (wide ? c.hd / 4 : c.hd) + 255) / 256, cap = (int64_t)dev_info().sms * 64;
+    cudaStream_t st = pick(stream);
+    if (wide) k_kv_read<true><<<(int)std::min(blocks, cap), 256, 0, st>>>(d_k, d_v, c, d_seq, d_slot, rows);
+    else k_kv_read<false><<<(int)std::min(blocks, cap), 256, 0, st>>>(d_k, d_v, c, d_seq, d_slot, rows);
     IQ_CHECK_LAUNCH();
     return IQ_OK;
 }

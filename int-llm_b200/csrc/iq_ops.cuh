@@ -23,10 +23,11 @@ __device__ __forceinline__ bool index_ok(int i, int n) {
 struct RopeTab {
     int half, rot, n_pos, kind, orig_len;
     int64_t ln_theta, factor, low, span, mscale;   // span = high - low
+    int64_t pi, gain, angles[25];                  // of the CORDIC; from step 25 on the angle is 2^(48 - i)
 };
 
 // One frequency a pair (see iq_rope_scaling in iq.h).
-__device__ __forceinline__ int64_t rope_freq(const RopeTab &t, int i, int64_t pi) {
+__device__ __forceinline__ int64_t rope_freq(const RopeTab &t, int i) {
     const int64_t y = d_mul(-d_div(d_from_int(2 * i), d_from_int(t.rot)), t.ln_theta);
     int64_t th;
     if (y < -10 * IQ_ONE) {   // fp_exp squares up to e^10.4 only
@@ -38,7 +39,7 @@ __device__ __forceinline__ int64_t rope_freq(const RopeTab &t, int i, int64_t pi
     if (t.kind == IQ_ROPE_SCALE_LINEAR) return d_div(th, t.factor);
     if (t.kind == IQ_ROPE_SCALE_PARTS) {
         const uint64_t turns = (uint64_t)d_udiv128_64((u128)((u128)(uint64_t)t.orig_len * (uint64_t)th) << 48,
-                                                      (uint64_t)(2 * pi));
+                                                      (uint64_t)(2 * t.pi));
         int64_t w = (int64_t)turns - t.low;
         w = d_div(min(max(w, (int64_t)0), t.span), t.span);
         return d_mul(th, w) + d_mul(d_div(th, t.factor), IQ_ONE - w);
@@ -46,32 +47,55 @@ __device__ __forceinline__ int64_t rope_freq(const RopeTab &t, int i, int64_t pi
     return th;
 }
 
+// CORDIC steps I .. 47 of (x, y) by the angle z (fp_sincos, fp_math.h:861-902). From step
+// 18 on the shifted values and the angle fit 32 bits (|x|, |y| stay below 2^48.1), so
+// that sign and sum are one wide multiply-add: 7 instructions a step against 17.
+template <int I>
+__device__ __forceinline__ void cordic(const RopeTab &t, int64_t &x, int64_t &y, int64_t &z) {
+    if constexpr (I < 48) {
+        if constexpr (I < 18) {
+            const int64_t xs = x >> I, ys = y >> I, a = t.angles[I];
+            if (z >= 0) { x -= ys; y += xs; z -= a; }
+            else        { x += ys; y -= xs; z += a; }
+        } else {
+            const int sg = (int)(z >> 63) | 1, xs = (int)(x >> I), ys = (int)(y >> I);
+            const int a = I < 25 ? (int)t.angles[I] : (int)(IQ_ONE >> I);
+            madw(x, -sg, ys);
+            madw(y, sg, xs);
+            madw(z, -sg, a);
+        }
+        cordic<I + 1>(t, x, y, z);
+    }
+}
+
 // cos, sin [n_pos][half] of p th_i. The angle is reduced mod 2 pi from the exact
 // product (p < 2^24, th <= 2^48): a double estimate of the quotient is within
 // one of it, and the wrapped remainder is exact, so it equals fp_sincos's
-// repeated subtraction (fp_math.h:861-902) at the positions where that has no
-// overflow. Issue-bound on the 48 integer CORDIC steps, not on the 16 bytes an
-// entry writes.
-__global__ void __launch_bounds__(256) k_rope_tables(int64_t *__restrict__ cs, int64_t *__restrict__ sn, RopeTab t) {
+// repeated subtraction at the positions where that has no overflow.
+// Issue-bound on the 48 CORDIC steps, not on the 16 bytes an entry writes.
+__global__ void __launch_bounds__(256) k_rope_tables(int64_t *__restrict__ cs, int64_t *__restrict__ sn,
+                                                     const __grid_constant__ RopeTab t) {
     __shared__ int64_t th[128];
-    const CordicTables &ct = g_cordic;
-    const int64_t pi = ct.pi, w = 2 * pi;
-    for (int i = threadIdx.x; i < t.half; i += blockDim.x) th[i] = rope_freq(t, i, pi);
+    const int64_t pi = t.pi, w = 2 * pi, half_pi = pi >> 1;
+    for (int i = threadIdx.x; i < t.half; i += blockDim.x) th[i] = rope_freq(t, i);
     __syncthreads();
     const int64_t n = (int64_t)t.n_pos * t.half, step = (int64_t)gridDim.x * blockDim.x;
+    const double inv_w = 1.0 / (double)w;
     for (int64_t e = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; e < n; e += step) {
-        const int p = (int)(e / t.half);
+        const int p = (int)((uint32_t)e / (uint32_t)t.half);   // n <= 2^31
         const int64_t f = th[(int)(e - (int64_t)p * t.half)];
-        const int64_t q = (int64_t)((double)p * (double)f / (double)w);
+        const int64_t q = (int64_t)((double)p * (double)f * inv_w);
         int64_t a = (int64_t)((uint64_t)p * (uint64_t)f - (uint64_t)q * (uint64_t)w);
         if (a < 0) a += w;
         else if (a >= w) a -= w;
         if (a > pi) a -= w;
-        int64_t c, s;
-        d_sincos(ct, a, &c, &s);
-        if (t.mscale) { c = d_mul(c, t.mscale); s = d_mul(s, t.mscale); }
-        cs[e] = c;
-        sn[e] = s;
+        const bool neg = a > half_pi || a < -half_pi;
+        int64_t z = a > half_pi ? pi - a : a < -half_pi ? -pi - a : a, x = t.gain, y = 0;
+        cordic<0>(t, x, y, z);
+        if (neg) x = -x;
+        if (t.mscale) { x = d_mul(x, t.mscale); y = d_mul(y, t.mscale); }
+        cs[e] = x;
+        sn[e] = y;
     }
 }
 
@@ -97,8 +121,33 @@ __device__ __forceinline__ void rope_turn(int64_t &a, int64_t &b, int64_t c, int
     a = u;
 }
 
-// One thread a pair; blockDim.y rows a block, blockIdx.y steps over the pairs
-// of a row. Memory-bound: 8 bytes read and 8 written an element.
+// Wide form (hd and rot multiples of 4, everything 16-byte aligned): item q of a
+// head is the four elements ea, ea + 1, eb, eb + 1, moved as two pieces of 16 bytes.
+struct RopeItem { int ea, eb, turn; };
+__device__ __forceinline__ RopeItem rope_item(const RopeArgs &r, int q) {
+    RopeItem it;
+    it.turn = 4 * q < r.rot;
+    if (it.turn && r.layout == IQ_ROPE_HALF) { it.ea = 2 * q; it.eb = 2 * q + (r.rot >> 1); }
+    else { it.ea = 4 * q; it.eb = 4 * q + 2; }
+    return it;
+}
+// (a, b) and the row's tables c, s of the item's two pairs
+__device__ __forceinline__ void rope_turn4(const RopeArgs &r, longlong2 &a, longlong2 &b, const longlong2 &c, const longlong2 &s) {
+    int64_t v[4] = {a.x, a.y, b.x, b.y};
+    if (r.layout == IQ_ROPE_HALF) {
+        rope_turn(v[0], v[2], c.x, s.x);
+        rope_turn(v[1], v[3], c.y, s.y);
+    } else {
+        rope_turn(v[0], v[1], c.x, s.x);
+        rope_turn(v[2], v[3], c.y, s.y);
+    }
+    a = make_longlong2(v[0], v[1]);
+    b = make_longlong2(v[2], v[3]);
+}
+
+// One thread an item (W) or a pair; blockDim.y rows a block, blockIdx.y steps
+// over the items of a row. Memory-bound: 8 bytes read and 8 written an element.
+template <bool W>
 __global__ void __launch_bounds__(256)
 k_rope(int64_t *__restrict__ out, const int64_t *__restrict__ x, RopeArgs r, int rows, int heads, int hd,
        int64_t xs, int64_t os) {
@@ -106,12 +155,23 @@ k_rope(int64_t *__restrict__ out, const int64_t *__restrict__ x, RopeArgs r, int
     if (row >= rows) return;
     const int pos = r.pos[row];
     if (!index_ok(pos, r.n_pos)) return;
-    const int half = r.rot >> 1, np = (hd + 1) >> 1;
+    const int half = r.rot >> 1, np = W ? hd >> 2 : (hd + 1) >> 1;
     const int64_t *c = r.cos + (size_t)pos * half, *s = r.sin + (size_t)pos * half;
     const int64_t *xr = x + row * xs;
     int64_t *orow = out + row * os;
     for (int it = blockIdx.y * blockDim.x + threadIdx.x; it < heads * np; it += gridDim.y * blockDim.x) {
         const int h = it / np, p = it - h * np;
+        if (W) {
+            const RopeItem q = rope_item(r, p);
+            longlong2 a = *reinterpret_cast<const longlong2 *>(xr + h * hd + q.ea);
+            longlong2 b = *reinterpret_cast<const longlong2 *>(xr + h * hd + q.eb);
+            if (q.turn)
+                rope_turn4(r, a, b, __ldg(reinterpret_cast<const longlong2 *>(c) + p),
+                           __ldg(reinterpret_cast<const longlong2 *>(s) + p));
+            *reinterpret_cast<longlong2 *>(orow + h * hd + q.ea) = a;
+            *reinterpret_cast<longlong2 *>(orow + h * hd + q.eb) = b;
+            continue;
+        }
         int e0, e1;
         rope_pair(r, p, e0, e1);
         e0 += h * hd;
@@ -131,25 +191,33 @@ k_rope(int64_t *__restrict__ out, const int64_t *__restrict__ x, RopeArgs r, int
 // ------------------------------------------------------------------- cache
 
 // b-bit code of x against the magnitude M (kv_pack_vector, llama_int.c:1197-1218):
-// ((x + M) 2^b) / (2M) truncated, clamped to [0, 2^b - 1]. For M < 2^61 a double
-// estimate (inv = 2^b / 2M; the quotient is below 2^17, so three roundings move
-// it by less than 2^-34) is corrected by its exact remainder.
+// ((x + M) 2^b) / (2M) truncated, clamped to [0, 2^b - 1]. For M < 2^61 the quotient
+// (at most 2^16) by a double factor (kv_inv: three roundings, then lowered, so
+// that its floor is q or q - 1); the exact remainder's sign tells which.
 __device__ __forceinline__ int kv_code(int64_t x, int64_t M, int bits, double inv) {
     if (M == 0) return 0;
     const int64_t top = ((int64_t)1 << bits) - 1;
     if (M < (1ll << 61)) {
-        const int64_t u = x + M, D = 2 * M;   // 0 <= u <= D
-        int64_t q = (int64_t)((double)u * inv);
-        const int64_t rem = (int64_t)(((uint64_t)u << bits) - (uint64_t)q * (uint64_t)D);
-        if (rem < 0) q--;
-        else if (rem >= D) q++;
-        return (int)min(q, top);
+        const uint64_t u = (uint64_t)(x + M), D = 2 * (uint64_t)M;   // u <= D
+        // u as a double from its halves, floored quotient in the binade of 2^52
+        const double ud = (__hiloint2double((int)0x45300000, (int)(uint32_t)(u >> 32)) - 19342813118337666422669312.0) +
+                          __hiloint2double(0x43300000, (int)(uint32_t)u);
+        const uint32_t q = (uint32_t)__double_as_longlong(__fma_rd(ud, inv, 4503599627370496.0));
+        // sign of (q + 1) D - u 2^b - 1
+        uint64_t t = D - 1 - (u << bits);
+        madu(t, q, (uint32_t)D);
+        const uint32_t h = (uint32_t)(t >> 32) + q * (uint32_t)(D >> 32);
+        return (int)min(q + (h >> 31), (uint32_t)top);
     }
     const i128 num = (i128)(int64_t)((uint64_t)x + (uint64_t)M) * ((i128)1 << bits);
     i128 t = d_sdiv128_64(num, (int64_t)((uint64_t)M * 2));
     if (t < 0) t = 0;
     if (t > top) t = top;
     return (int)t;
+}
+// 2^b / 2M lowered by 2^-50 (M < 2^61)
+__device__ __forceinline__ double kv_inv(int64_t M, int bits) {
+    return M && M < (1ll << 61) ? (double)(1 << bits) / (double)(2 * M) * (1.0 - 0x1p-50) : 0;
 }
 
 // ((2q + 1) M >> b) - M (kv_unpack_vector, llama_int.c:1226-1235) from 32-bit halves of M:
@@ -169,8 +237,84 @@ struct KVArgs {
     int seqs, max_seq, nkv, hd, kbits, vbits;
 };
 
-// One warp a vector of (row, kv head, K or V), the vector in registers (hd <=
-// 256: up to 4 pairs a lane): rotate, take the magnitude, write the codes.
+// Wide form: L lanes (a power of two) a vector of (row, kv head, K or V), each with
+// up to two items of four elements: rotate, take the magnitude, write the codes.
+template <bool PACKED>
+__global__ void __launch_bounds__(256)
+k_kv_write_wide(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restrict__ v, const int *__restrict__ seq,
+                const int *__restrict__ slot, int rows, int64_t ks, int64_t vs, RopeArgs r, int log_l) {
+    const int L = 1 << log_l;
+    const int64_t gv = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> log_l;
+    const int lane = threadIdx.x & (L - 1);
+    bool live = gv < (int64_t)rows * c.nkv * 2;
+    const int which = (int)(gv & 1);
+    const uint32_t rh = (uint32_t)(gv >> 1), row = rh / (uint32_t)c.nkv, h = rh - row * c.nkv;
+    int sq = 0, t = 0, pos = 0;
+    if (live) {
+        sq = seq ? seq[row] : 0;
+        t = slot[row];
+        if (r.cos) pos = r.pos[row];   // both vectors of a row without a position are left out
+        live = index_ok(sq, c.seqs) && index_ok(t, c.max_seq) && (!r.cos || index_ok(pos, r.n_pos));
+    }
+    if (which || !r.cos) r.rot = 0;
+    const int half = r.rot >> 1, np = c.hd >> 2;
+    const int64_t *src = which ? v + row * vs + (int64_t)h * c.hd : k + row * ks + (int64_t)h * c.hd;
+    const longlong2 *cs = reinterpret_cast<const longlong2 *>(r.cos + (size_t)pos * half);
+    const longlong2 *sn = reinterpret_cast<const longlong2 *>(r.sin + (size_t)pos * half);
+    const size_t vec = ((size_t)sq * c.max_seq + t) * c.nkv + h, e0 = vec * c.hd;
+    longlong2 a[2], b[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const int q = lane + j * L;
+        a[j] = b[j] = make_longlong2(0, 0);
+        if (live && q < np) {
+            const RopeItem it = rope_item(r, q);
+            a[j] = __ldg(reinterpret_cast<const longlong2 *>(src + it.ea));
+            b[j] = __ldg(reinterpret_cast<const longlong2 *>(src + it.eb));
+        }
+    }
+    int64_t M = 0;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const int q = lane + j * L;
+        if (live && q < np && 4 * q < r.rot) rope_turn4(r, a[j], b[j], __ldg(cs + q), __ldg(sn + q));
+        if (PACKED) {   // |INT64_MIN| wraps to itself, below every magnitude, as in the reference
+            const int64_t w[4] = {a[j].x, a[j].y, b[j].x, b[j].y};
+#pragma unroll
+            for (int i = 0; i < 4; i++) M = max(M, w[i] < 0 ? (int64_t)(0 - (uint64_t)w[i]) : w[i]);
+        }
+    }
+    const int bits = which ? c.vbits : c.kbits;
+    double inv = 0;
+    if (PACKED) {
+        for (int m = L >> 1; m >= 1; m >>= 1) M = max(M, (int64_t)__shfl_xor_sync(0xffffffffu, M, m));
+        if (live && lane == 0) (which ? c.vmag : c.kmag)[vec] = M;
+        inv = kv_inv(M, bits);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const int q = lane + j * L;
+        if (!live || q >= np) continue;
+        const RopeItem it = rope_item(r, q);
+        if (PACKED) {
+            const int c0 = kv_code(a[j].x, M, bits, inv), c1 = kv_code(a[j].y, M, bits, inv);
+            const int c2 = kv_code(b[j].x, M, bits, inv), c3 = kv_code(b[j].y, M, bits, inv);
+            if (which) {
+                *reinterpret_cast<ushort2 *>(c.vq + e0 + it.ea) = make_ushort2(c0, c1);
+                *reinterpret_cast<ushort2 *>(c.vq + e0 + it.eb) = make_ushort2(c2, c3);
+            } else {
+                *reinterpret_cast<uchar2 *>(c.kq + e0 + it.ea) = make_uchar2(c0, c1);
+                *reinterpret_cast<uchar2 *>(c.kq + e0 + it.eb) = make_uchar2(c2, c3);
+            }
+        } else {
+            int64_t *dst = (which ? c.v : c.k) + e0;
+            *reinterpret_cast<longlong2 *>(dst + it.ea) = a[j];
+            *reinterpret_cast<longlong2 *>(dst + it.eb) = b[j];
+        }
+    }
+}
+
+// One warp a vector, any hd <= 256 and alignment: up to 4 pairs a lane.
 template <bool PACKED>
 __global__ void __launch_bounds__(256)
 k_kv_write(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restrict__ v, const int *__restrict__ seq,
@@ -216,7 +360,7 @@ k_kv_write(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restrict__ 
     if (PACKED) {
         for (int m = 16; m >= 1; m >>= 1) M = max(M, (int64_t)__shfl_xor_sync(0xffffffffu, M, m));
         if (lane == 0) (which ? c.vmag : c.kmag)[vec] = M;
-        if (M && M < (1ll << 61)) inv = (double)(1 << bits) / (double)(2 * M);
+        inv = kv_inv(M, bits);
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -241,27 +385,44 @@ k_kv_write(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restrict__ 
     }
 }
 
-// One warp a vector, as k_kv_write.
+// A thread four elements (W: hd a multiple of 4, aligned) or one, K and V in turn.
+template <bool W>
 __global__ void __launch_bounds__(256)
 k_kv_read(int64_t *__restrict__ k, int64_t *__restrict__ v, KVArgs c, const int *__restrict__ seq,
           const int *__restrict__ slot, int rows) {
-    const int64_t gw = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (gw >= (int64_t)rows * c.nkv * 2) return;
-    const int which = (int)(gw & 1);
-    const int64_t row = (gw >> 1) / c.nkv;
-    const int h = (int)((gw >> 1) - row * c.nkv);
-    const int sq = seq ? seq[row] : 0, t = slot[row];
-    if (!index_ok(sq, c.seqs) || !index_ok(t, c.max_seq)) return;
-    const size_t vec = ((size_t)sq * c.max_seq + t) * c.nkv + h, e0 = vec * c.hd;
-    int64_t *dst = (which ? v : k) + (row * c.nkv + h) * c.hd;
-    if (c.kbits) {
-        const int64_t M = (which ? c.vmag : c.kmag)[vec];
+    const uint32_t np = W ? c.hd >> 2 : c.hd;
+    const int64_t n = (int64_t)rows * c.nkv * 2 * np;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t gv = n >> 32 ? i / np : (uint32_t)i / np;
+        const int d = (int)(i - gv * np) * (W ? 4 : 1), which = (int)(gv & 1);
+        const uint32_t rh = (uint32_t)(gv >> 1), row = rh / (uint32_t)c.nkv, h = rh - row * c.nkv;
+        const int sq = seq ? seq[row] : 0, t = slot[row];
+        if (!index_ok(sq, c.seqs) || !index_ok(t, c.max_seq)) continue;
+        const size_t vec = ((size_t)sq * c.max_seq + t) * c.nkv + h, e = vec * c.hd + d;
+        int64_t *dst = (which ? v : k) + (size_t)rh * c.hd + d;
+        const int64_t M = c.kbits ? __ldg((which ? c.vmag : c.kmag) + vec) : 0;
         const int bits = which ? c.vbits : c.kbits;
-        for (int d = lane; d < c.hd; d += 32) dst[d] = kv_value(which ? c.vq[e0 + d] : c.kq[e0 + d], M, bits);
-    } else {
-        const int64_t *src = (which ? c.v : c.k) + e0;
-        for (int d = lane; d < c.hd; d += 32) dst[d] = src[d];
+        if (!W) {
+            *dst = c.kbits ? kv_value(which ? c.vq[e] : c.kq[e], M, bits) : (which ? c.v : c.k)[e];
+            continue;
+        }
+        longlong2 a, b;
+        if (c.kbits) {
+            ushort4 q;
+            if (which) q = __ldg(reinterpret_cast<const ushort4 *>(c.vq + e));
+            else {
+                const uchar4 u = __ldg(reinterpret_cast<const uchar4 *>(c.kq + e));
+                q = make_ushort4(u.x, u.y, u.z, u.w);
+            }
+            a = make_longlong2(kv_value(q.x, M, bits), kv_value(q.y, M, bits));
+            b = make_longlong2(kv_value(q.z, M, bits), kv_value(q.w, M, bits));
+        } else {
+            const longlong2 *p = reinterpret_cast<const longlong2 *>((which ? c.v : c.k) + e);
+            a = p[0];
+            b = p[1];
+        }
+        reinterpret_cast<longlong2 *>(dst)[0] = a;
+        reinterpret_cast<longlong2 *>(dst)[1] = b;
     }
 }
 
