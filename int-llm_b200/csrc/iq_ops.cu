@@ -312,10 +312,9 @@ IQ_API int iq_kv_write_dev(const iq_kv_cache *cache, const int64_t *d_k, const i
         int log_l = 0;   // lanes a vector
         while (log_l < 5 && 1 << log_l < c.hd / 4) log_l++;
         const int blocks = (int)(((vecs << log_l) + 255) / 256);
-        if (c.kbits)
-            k_kv_write_wide<true><<<blocks, 256, 0, st>>>(c, d_k, d_v, d_seq, d_slot, rows, k_stride, v_stride, r, log_l);
-        else
-            k_kv_write_wide<false><<<blocks, 256, 0, st>>>(c, d_k, d_v, d_seq, d_slot, rows, k_stride, v_stride, r, log_l);
+        auto *kern = c.kbits ? c.hd <= 128 ? k_kv_write_wide<true, 1> : k_kv_write_wide<true, 2>
+                             : c.hd <= 128 ? k_kv_write_wide<false, 1> : k_kv_write_wide<false, 2>;
+        kern<<<blocks, 256, 0, st>>>(c, d_k, d_v, d_seq, d_slot, rows, k_stride, v_stride, r, log_l);
     } else {
         const int blocks = (int)((vecs + 7) / 8);
         if (c.kbits)

@@ -11,6 +11,18 @@ __device__ __forceinline__ void madu(uint64_t &acc, uint32_t x, uint32_t y) {
     asm("mad.wide.u32 %0, %1, %2, %0;" : "+l"(acc) : "r"(x), "r"(y));
 }
 
+// 1 / x by two Newton steps, relative error below 2^-51
+__device__ __forceinline__ double f64_rcp(double x) {
+    double y;
+    asm("rcp.approx.ftz.f64 %0, %1;" : "=d"(y) : "d"(x));
+    y = __fma_rn(y, __fma_rn(-x, y, 1.0), y);
+    return __fma_rn(y, __fma_rn(-x, y, 1.0), y);
+}
+// the positive 64-bit x as a double (one rounding)
+__device__ __forceinline__ double f64_u64(uint64_t x) {
+    return (__longlong_as_double((long long)((x >> 32) | 0x4530000000000000ull)) - 19342813118337666422669312.0) +
+           __longlong_as_double((long long)((x & 0xFFFFFFFFull) | 0x4330000000000000ull));
+}
 // A bad index of a device array (not the -1 of a padding row): left out and recorded.
 __device__ __forceinline__ bool index_ok(int i, int n) {
     if (i >= 0 && i < n) return true;
@@ -131,15 +143,46 @@ __device__ __forceinline__ RopeItem rope_item(const RopeArgs &r, int q) {
     else { it.ea = 4 * q; it.eb = 4 * q + 2; }
     return it;
 }
+// fp_mul for |x| < 2^60 and |c| < 2^49: with both halves signed, x = xh 2^32 + xl and
+// c = ch 2^32 + cl, every product is one wide multiply-add:
+// floor(x c / 2^48) = 4 xh 2^14 ch + floor((xh cl + xl ch + floor(xl cl / 2^32)) / 2^16).
+struct Half { int h, l; };
+__device__ __forceinline__ Half halves(int64_t x) {
+    const int l = (int)(uint32_t)x;
+    return Half{(int)(x >> 32) - (l >> 31), l};
+}
+__device__ __forceinline__ int64_t mul_small(const Half &x, const Half &c) {
+    int64_t t = __mulhi(x.l, c.l);
+    madw(t, x.h, c.l);
+    madw(t, x.l, c.h);
+    t >>= 16;
+    madw(t, x.h * 4, c.h * (1 << 14));
+    return t;
+}
+__device__ __forceinline__ void turn_small(int64_t &a, int64_t &b, int64_t c, int64_t s) {
+    const Half x = halves(a), y = halves(b), u = halves(c), v = halves(s);
+    a = mul_small(x, u) - mul_small(y, v);
+    b = mul_small(y, u) + mul_small(x, v);
+}
+// 0 where -2^(32 + k) <= x < 2^(32 + k)
+__device__ __forceinline__ uint32_t beyond(int64_t x, int k) { return ((uint32_t)(x >> 32) + (1u << k)) >> (k + 1); }
+
 // (a, b) and the row's tables c, s of the item's two pairs
 __device__ __forceinline__ void rope_turn4(const RopeArgs &r, longlong2 &a, longlong2 &b, const longlong2 &c, const longlong2 &s) {
     int64_t v[4] = {a.x, a.y, b.x, b.y};
-    if (r.layout == IQ_ROPE_HALF) {
-        rope_turn(v[0], v[2], c.x, s.x);
-        rope_turn(v[1], v[3], c.y, s.y);
+    if (r.layout == IQ_ROPE_HALF) { v[1] = b.x; v[2] = a.y; }   // pairs (0, 1), (2, 3)
+    if ((beyond(a.x, 28) | beyond(a.y, 28) | beyond(b.x, 28) | beyond(b.y, 28) | beyond(c.x, 17) | beyond(c.y, 17) |
+         beyond(s.x, 17) | beyond(s.y, 17)) == 0) {
+        turn_small(v[0], v[1], c.x, s.x);
+        turn_small(v[2], v[3], c.y, s.y);
     } else {
         rope_turn(v[0], v[1], c.x, s.x);
         rope_turn(v[2], v[3], c.y, s.y);
+    }
+    if (r.layout == IQ_ROPE_HALF) {
+        const int64_t w = v[1];
+        v[1] = v[2];
+        v[2] = w;
     }
     a = make_longlong2(v[0], v[1]);
     b = make_longlong2(v[2], v[3]);
@@ -199,9 +242,8 @@ __device__ __forceinline__ int kv_code(int64_t x, int64_t M, int bits, double in
     const int64_t top = ((int64_t)1 << bits) - 1;
     if (M < (1ll << 61)) {
         const uint64_t u = (uint64_t)(x + M), D = 2 * (uint64_t)M;   // u <= D
-        // u as a double from its halves, floored quotient in the binade of 2^52
-        const double ud = (__hiloint2double((int)0x45300000, (int)(uint32_t)(u >> 32)) - 19342813118337666422669312.0) +
-                          __hiloint2double(0x43300000, (int)(uint32_t)u);
+        // the floored quotient in the binade of 2^52
+        const double ud = f64_u64(u);
         const uint32_t q = (uint32_t)__double_as_longlong(__fma_rd(ud, inv, 4503599627370496.0));
         // sign of (q + 1) D - u 2^b - 1
         uint64_t t = D - 1 - (u << bits);
@@ -215,9 +257,9 @@ __device__ __forceinline__ int kv_code(int64_t x, int64_t M, int bits, double in
     if (t > top) t = top;
     return (int)t;
 }
-// 2^b / 2M lowered by 2^-50 (M < 2^61)
+// 2^b / 2M lowered by 2^-50 (for 0 < M < 2^61; not used otherwise)
 __device__ __forceinline__ double kv_inv(int64_t M, int bits) {
-    return M && M < (1ll << 61) ? (double)(1 << bits) / (double)(2 * M) * (1.0 - 0x1p-50) : 0;
+    return f64_rcp(f64_u64(2 * (uint64_t)M)) * ((double)(1 << bits) * (1.0 - 0x1p-50));
 }
 
 // ((2q + 1) M >> b) - M (kv_unpack_vector, llama_int.c:1226-1235) from 32-bit halves of M:
@@ -238,8 +280,8 @@ struct KVArgs {
 };
 
 // Wide form: L lanes (a power of two) a vector of (row, kv head, K or V), each with
-// up to two items of four elements: rotate, take the magnitude, write the codes.
-template <bool PACKED>
+// NJ items of four elements: rotate, take the magnitude, write the codes.
+template <bool PACKED, int NJ>
 __global__ void __launch_bounds__(256)
 k_kv_write_wide(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restrict__ v, const int *__restrict__ seq,
                 const int *__restrict__ slot, int rows, int64_t ks, int64_t vs, RopeArgs r, int log_l) {
@@ -262,9 +304,9 @@ k_kv_write_wide(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restri
     const longlong2 *cs = reinterpret_cast<const longlong2 *>(r.cos + (size_t)pos * half);
     const longlong2 *sn = reinterpret_cast<const longlong2 *>(r.sin + (size_t)pos * half);
     const size_t vec = ((size_t)sq * c.max_seq + t) * c.nkv + h, e0 = vec * c.hd;
-    longlong2 a[2], b[2];
+    longlong2 a[NJ], b[NJ];
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
+    for (int j = 0; j < NJ; j++) {
         const int q = lane + j * L;
         a[j] = b[j] = make_longlong2(0, 0);
         if (live && q < np) {
@@ -275,7 +317,7 @@ k_kv_write_wide(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restri
     }
     int64_t M = 0;
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
+    for (int j = 0; j < NJ; j++) {
         const int q = lane + j * L;
         if (live && q < np && 4 * q < r.rot) rope_turn4(r, a[j], b[j], __ldg(cs + q), __ldg(sn + q));
         if (PACKED) {   // |INT64_MIN| wraps to itself, below every magnitude, as in the reference
@@ -292,7 +334,7 @@ k_kv_write_wide(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restri
         inv = kv_inv(M, bits);
     }
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
+    for (int j = 0; j < NJ; j++) {
         const int q = lane + j * L;
         if (!live || q >= np) continue;
         const RopeItem it = rope_item(r, q);

@@ -150,6 +150,15 @@ __global__ void __launch_bounds__(LP_T) k_logprobs(const __grid_constant__ LpArg
     if (tid < 64) pw[tid] = (double)c_lp_pow[tid] * 0x1p-48;
     if (tid == 0) cnt = 0;
 
+    // the given token's logit, early
+    int64_t given = 0;
+    bool has = false;
+    if (rank == 0 && tid == 32 && a.tok) {
+        const int t = a.tok[row];
+        has = index_ok(t, a.V);
+        if (has) given = l[t];
+    }
+
     // the maximum
     int64_t m = INT64_MIN;
     const int64_t *src = l + b0;
@@ -328,7 +337,7 @@ __global__ void __launch_bounds__(LP_T) k_logprobs(const __grid_constant__ LpArg
     const u128 St = ((u128)wred[1] << 32) + wred[0];
     if (warp < 2) {
         const int64_t z = lp_ln(St);
-        if (tid == 32 && a.tok && index_ok(a.tok[row], a.V)) a.logp[row] = lp_of((uint64_t)m - (uint64_t)l[a.tok[row]], z);
+        if (has) a.logp[row] = lp_of((uint64_t)m - (uint64_t)given, z);
         if (tid == 33 && ent) a.ent[row] = lp_entropy(St, ((u128)wred[3] << 32) + wred[2], z);
         if (tid < a.top) {
             a.ids[(size_t)row * a.top + tid] = cs > 1 ? ci[tid] : gi[tid];

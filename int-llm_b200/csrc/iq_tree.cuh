@@ -484,18 +484,6 @@ __device__ __forceinline__ uint64_t tree_sqr(uint64_t r) {
     madu(x, h << 8, h << 8);
     return x;
 }
-// 1 / x by two Newton steps, relative error below 2^-51
-__device__ __forceinline__ double tree_rcp(double x) {
-    double y;
-    asm("rcp.approx.ftz.f64 %0, %1;" : "=d"(y) : "d"(x));
-    y = __fma_rn(y, __fma_rn(-x, y, 1.0), y);
-    return __fma_rn(y, __fma_rn(-x, y, 1.0), y);
-}
-// the positive 64-bit x as a double (one rounding)
-__device__ __forceinline__ double tree_u64(uint64_t x) {
-    return (__longlong_as_double((long long)((x >> 32) | 0x4530000000000000ull)) - 19342813118337666422669312.0) +
-           __longlong_as_double((long long)((x & 0xFFFFFFFFull) | TREE_MB));
-}
 // 1 where q r + c < 0 (mod 2^64, as a signed number), else 0
 __device__ __forceinline__ uint32_t tree_more(uint64_t q, uint64_t r, uint64_t c) {
     madu(c, (uint32_t)q, (uint32_t)r);
@@ -514,12 +502,12 @@ __device__ __forceinline__ int64_t tree_exp(uint64_t d) {
     // floor(2^96 / r), at most 2^48: reciprocal by two Newton steps (relative error
     // below 2^-51), lowered by 2^-50 so that its floor is q or q - 1; the sign of
     // (q + 1) r - 2^96 - 1 (2^96 = 0 mod 2^64) tells which
-    const double y = tree_rcp(tree_u64(r));
+    const double y = f64_rcp(f64_u64(r));
     const uint64_t q = (uint64_t)__double_as_longlong(__fma_rd(y, 0x1p96 - 0x1p46, TREE_M)) & TREE_MASK;
     return (int64_t)(q + tree_more(q, r, r - 1));
 }
 // fp_div(e, S) 2^-48 as a double for 0 <= e <= S, 2^48 <= S < 2^63, e <= 2^48,
-// inv = tree_rcp(S) 2^48 lowered like the quotient of tree_exp
+// inv = f64_rcp(S) 2^48 lowered like the quotient of tree_exp
 __device__ __forceinline__ double tree_prob(int64_t e, int64_t S, double inv) {
     const uint64_t q = (uint64_t)__double_as_longlong(__fma_rd(tree_u52((uint64_t)e), inv, TREE_M)) & TREE_MASK;
     return tree_u52(q + tree_more(q, (uint64_t)S, (uint64_t)S - 1 - ((uint64_t)e << 48))) * 0x1p-48;
@@ -651,7 +639,7 @@ __global__ void __launch_bounds__(TREE_SM_T) k_tree_softmax(const __grid_constan
         uint64_t S = 0;
 #pragma unroll
         for (int k = 0; k < TREE_SM_T / 32; k++) S += wsum[par][k];
-        const double inv = tree_rcp(tree_u64(S)) * (0x1p48 - 0x1p-2);
+        const double inv = f64_rcp(f64_u64(S)) * (0x1p48 - 0x1p-2);
         double *p = reinterpret_cast<double *>(row);
         for (int t0 = 0; t0 < (LONG ? end : 1); t0 += TREE_SM_T * TREE_SM_E) {
 #pragma unroll

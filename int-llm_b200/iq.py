@@ -355,22 +355,36 @@ def softmax_dev(x, rows, n, stream=None):
 
 # ------------------------- drafted tokens: rotary, cache, tree attention, scores
 
+_raw_device = _raw_stream = None   # torch's current device and stream handle, bound at the first call
+
+
+def _bind_torch():
+    global _raw_device, _raw_stream
+    import torch
+    _raw_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _dev_ptr(t, itemsize, name):
     """Device pointer of t (None: NULL) after checking its element size and that
     it lies on the device that calls go to (torch's current one)."""
     if t is None:
         return None
-    size = t.element_size() if hasattr(t, "element_size") else t.itemsize
-    if size != itemsize:
-        raise ValueError(f"{name}: {itemsize}-byte elements expected, got {size}")
-    d = getattr(t, "device", None)
-    if d is not None and getattr(d, "type", "cuda") != "cuda":
-        raise ValueError(f"{name} must be in device memory, got {d}")
-    if d is not None and getattr(d, "index", None) is not None:
-        import torch
-        if d.index != torch.cuda.current_device():
-            raise ValueError(f"{name} lies on {d}, calls go to cuda:{torch.cuda.current_device()}")
+    if t.element_size() != itemsize:
+        raise ValueError(f"{name}: {itemsize}-byte elements expected, got {t.element_size()}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be in device memory, got {t.device}")
+    if _raw_device is None:
+        _bind_torch()
+    if t.get_device() != _raw_device():
+        raise ValueError(f"{name} lies on {t.device}, calls go to device {_raw_device()}")
     return t.data_ptr()
+
+
+def _cur(stream):
+    """Stream argument as _sp's: an explicit one, else torch's current stream."""
+    if stream is None:
+        return _raw_stream(_raw_device()) or _CUDA_STREAM_LEGACY
+    return getattr(stream, "cuda_stream", stream)
 
 
 ROPE_LAYOUT = dict(half=0, interleaved=1)
@@ -389,7 +403,7 @@ def rope_tables_dev(cos, sin, rot_dim, n_pos, theta, scaling=None, stream=None):
         f["kind"] = ROPE_SCALE[f.get("kind", "none")]
         sc = ctypes.byref(_RopeScaling(**f))
     _call("iq_rope_tables_dev", _dev_ptr(cos, 8, "cos"), _dev_ptr(sin, 8, "sin"), rot_dim, n_pos, theta, sc,
-          _sp(stream))
+          _cur(stream))
 
 
 class Rope(ctypes.Structure):
@@ -405,7 +419,7 @@ class Rope(ctypes.Structure):
 def rope_dev(out, x, rope, rows, heads, head_dim, x_stride=None, out_stride=None, stream=None):
     w = heads * head_dim
     _call("iq_rope_dev", _dev_ptr(out, 8, "out"), _dev_ptr(x, 8, "x"), ctypes.byref(rope), rows, heads, head_dim,
-          w if x_stride is None else x_stride, w if out_stride is None else out_stride, _sp(stream))
+          w if x_stride is None else x_stride, w if out_stride is None else out_stride, _cur(stream))
 
 
 class KVCache(ctypes.Structure):
@@ -425,12 +439,12 @@ def kv_write_dev(cache, k, v, slot, rows, seq=None, rope=None, k_stride=None, v_
     w = cache.kv_heads * cache.head_dim
     _call("iq_kv_write_dev", ctypes.byref(cache), _dev_ptr(k, 8, "k"), _dev_ptr(v, 8, "v"), _dev_ptr(seq, 4, "seq"),
           _dev_ptr(slot, 4, "slot"), rows, w if k_stride is None else k_stride, w if v_stride is None else v_stride,
-          ctypes.byref(rope) if rope is not None else None, _sp(stream))
+          ctypes.byref(rope) if rope is not None else None, _cur(stream))
 
 
 def kv_read_dev(k, v, cache, slot, rows, seq=None, stream=None):
     _call("iq_kv_read_dev", _dev_ptr(k, 8, "k"), _dev_ptr(v, 8, "v"), ctypes.byref(cache), _dev_ptr(seq, 4, "seq"),
-          _dev_ptr(slot, 4, "slot"), rows, _sp(stream))
+          _dev_ptr(slot, 4, "slot"), rows, _cur(stream))
 
 
 def attn_tree_work(cache, num_heads, n_seq, rows, max_nodes, max_len):
@@ -448,14 +462,14 @@ def attn_tree_dev(out, q, cache, num_heads, lens, starts, parents, n_seq, rows, 
           _dev_ptr(seqs, 4, "seqs"), _dev_ptr(lens, 4, "lens"), _dev_ptr(starts, 4, "starts"),
           _dev_ptr(parents, 4, "parents"), n_seq, rows, max_nodes, max_len,
           num_heads * cache.head_dim if q_stride is None else q_stride,
-          None if work is None else _dev_ptr(work, work.element_size(), "work"), nbytes, _sp(stream))
+          None if work is None else _dev_ptr(work, work.element_size(), "work"), nbytes, _cur(stream))
 
 
 def logprobs_dev(logits, rows, vocab, tokens=None, logp=None, entropy=None, top=0, top_ids=None, top_logp=None,
                  ld=None, stream=None):
     _call("iq_logprobs_dev", _dev_ptr(logits, 8, "logits"), vocab if ld is None else ld, rows, vocab,
           _dev_ptr(tokens, 4, "tokens"), _dev_ptr(logp, 8, "logp"), _dev_ptr(entropy, 8, "entropy"), top,
-          _dev_ptr(top_ids, 4, "top_ids"), _dev_ptr(top_logp, 8, "top_logp"), _sp(stream))
+          _dev_ptr(top_ids, 4, "top_ids"), _dev_ptr(top_logp, 8, "top_logp"), _cur(stream))
 
 
 # --------------------------------------------------------- synthetic inputs
