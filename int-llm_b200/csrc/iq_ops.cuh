@@ -235,31 +235,41 @@ k_rope(int64_t *__restrict__ out, const int64_t *__restrict__ x, RopeArgs r, int
 
 // b-bit code of x against the magnitude M (kv_pack_vector, llama_int.c:1197-1218):
 // ((x + M) 2^b) / (2M) truncated, clamped to [0, 2^b - 1]. For M < 2^61 the quotient
-// (at most 2^16) by a double factor (kv_inv: three roundings, then lowered, so
+// (at most 2^16) by a double factor (kv_mag: three roundings, then lowered, so
 // that its floor is q or q - 1); the exact remainder's sign tells which.
-__device__ __forceinline__ int kv_code(int64_t x, int64_t M, int bits, double inv) {
-    if (M == 0) return 0;
+struct KVMag {
+    int64_t M;
+    uint64_t D;     // 2M, or 1 where M is 0 (every code is 0 then)
+    double inv;     // 2^b / D lowered by 2^-50
+    int bits, top;
+};
+__device__ __forceinline__ KVMag kv_mag(int64_t M, int bits) {
+    KVMag m;
+    m.M = M;
+    m.D = M ? 2 * (uint64_t)M : 1;
+    m.inv = f64_rcp(f64_u64(m.D)) * ((double)(1 << bits) * (1.0 - 0x1p-50));
+    m.bits = bits;
+    m.top = (1 << bits) - 1;
+    return m;
+}
+__device__ __forceinline__ int kv_code(int64_t x, const KVMag &m) {   // M < 2^61
+    const uint64_t u = (uint64_t)(x + m.M);   // u <= D
+    // the floored quotient in the binade of 2^52
+    const uint32_t q = (uint32_t)__double_as_longlong(__fma_rd(f64_u64(u), m.inv, 4503599627370496.0));
+    // sign of (q + 1) D - u 2^b - 1
+    uint64_t t = m.D - 1 - (u << m.bits);
+    madu(t, q, (uint32_t)m.D);
+    const uint32_t h = (uint32_t)(t >> 32) + q * (uint32_t)(m.D >> 32);
+    return min((int)(q + (h >> 31)), m.top);
+}
+// the same for any M, as the reference's int64 wraps
+__device__ __noinline__ int kv_code_any(int64_t x, int64_t M, int bits) {
     const int64_t top = ((int64_t)1 << bits) - 1;
-    if (M < (1ll << 61)) {
-        const uint64_t u = (uint64_t)(x + M), D = 2 * (uint64_t)M;   // u <= D
-        // the floored quotient in the binade of 2^52
-        const double ud = f64_u64(u);
-        const uint32_t q = (uint32_t)__double_as_longlong(__fma_rd(ud, inv, 4503599627370496.0));
-        // sign of (q + 1) D - u 2^b - 1
-        uint64_t t = D - 1 - (u << bits);
-        madu(t, q, (uint32_t)D);
-        const uint32_t h = (uint32_t)(t >> 32) + q * (uint32_t)(D >> 32);
-        return (int)min(q + (h >> 31), (uint32_t)top);
-    }
     const i128 num = (i128)(int64_t)((uint64_t)x + (uint64_t)M) * ((i128)1 << bits);
     i128 t = d_sdiv128_64(num, (int64_t)((uint64_t)M * 2));
     if (t < 0) t = 0;
     if (t > top) t = top;
     return (int)t;
-}
-// 2^b / 2M lowered by 2^-50 (for 0 < M < 2^61; not used otherwise)
-__device__ __forceinline__ double kv_inv(int64_t M, int bits) {
-    return f64_rcp(f64_u64(2 * (uint64_t)M)) * ((double)(1 << bits) * (1.0 - 0x1p-50));
 }
 
 // ((2q + 1) M >> b) - M (kv_unpack_vector, llama_int.c:1226-1235) from 32-bit halves of M:
@@ -327,11 +337,11 @@ k_kv_write_wide(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restri
         }
     }
     const int bits = which ? c.vbits : c.kbits;
-    double inv = 0;
+    KVMag km = {};
     if (PACKED) {
         for (int m = L >> 1; m >= 1; m >>= 1) M = max(M, (int64_t)__shfl_xor_sync(0xffffffffu, M, m));
         if (live && lane == 0) (which ? c.vmag : c.kmag)[vec] = M;
-        inv = kv_inv(M, bits);
+        km = kv_mag(M, bits);
     }
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
@@ -339,8 +349,18 @@ k_kv_write_wide(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restri
         if (!live || q >= np) continue;
         const RopeItem it = rope_item(r, q);
         if (PACKED) {
-            const int c0 = kv_code(a[j].x, M, bits, inv), c1 = kv_code(a[j].y, M, bits, inv);
-            const int c2 = kv_code(b[j].x, M, bits, inv), c3 = kv_code(b[j].y, M, bits, inv);
+            int c0, c1, c2, c3;
+            if (M < (1ll << 61)) {
+                c0 = kv_code(a[j].x, km);
+                c1 = kv_code(a[j].y, km);
+                c2 = kv_code(b[j].x, km);
+                c3 = kv_code(b[j].y, km);
+            } else {
+                c0 = kv_code_any(a[j].x, M, bits);
+                c1 = kv_code_any(a[j].y, M, bits);
+                c2 = kv_code_any(b[j].x, M, bits);
+                c3 = kv_code_any(b[j].y, M, bits);
+            }
             if (which) {
                 *reinterpret_cast<ushort2 *>(c.vq + e0 + it.ea) = make_ushort2(c0, c1);
                 *reinterpret_cast<ushort2 *>(c.vq + e0 + it.eb) = make_ushort2(c2, c3);
@@ -397,12 +417,12 @@ k_kv_write(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restrict__ 
             M = max(M, max(ma, mb));
         }
     }
-    double inv = 0;
+    KVMag km = {};
     const int bits = which ? c.vbits : c.kbits;
     if (PACKED) {
         for (int m = 16; m >= 1; m >>= 1) M = max(M, (int64_t)__shfl_xor_sync(0xffffffffu, M, m));
         if (lane == 0) (which ? c.vmag : c.kmag)[vec] = M;
-        inv = kv_inv(M, bits);
+        km = kv_mag(M, bits);
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -411,7 +431,8 @@ k_kv_write(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restrict__ 
         int e0, e1;
         rope_pair(rr, p, e0, e1);
         if (PACKED) {
-            const int q0 = kv_code(a[j], M, bits, inv), q1 = kv_code(b[j], M, bits, inv);
+            const int q0 = M < (1ll << 61) ? kv_code(a[j], km) : kv_code_any(a[j], M, bits);
+            const int q1 = M < (1ll << 61) ? kv_code(b[j], km) : kv_code_any(b[j], M, bits);
             if (which) {
                 c.vq[e0v + e0] = (uint16_t)q0;
                 if (e1 < c.hd) c.vq[e0v + e1] = (uint16_t)q1;
