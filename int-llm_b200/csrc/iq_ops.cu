@@ -139,7 +139,11 @@ static void tree_plan(TreeArgs *a) {
     while (a->tpc > 1 && pairs * ((tiles + a->tpc - 1) / a->tpc) < 6 * sms) a->tpc /= 2;
     a->tiles = (tiles + a->tpc - 1) / a->tpc;
     a->groups = (blocks + a->passes - 1) / a->passes;
-    a->cg = cols > 32 && a->c.hd <= 64 ? 4 : cols > 16 && a->c.hd <= 128 ? 2 : 1;   // 16 cg hd <= TREE_RED
+    a->cg = cols > 32 && a->c.hd <= 64 ? 4 : cols > 16 && a->c.hd <= 128 ? 2 : 1;   // cg hd <= 256
+    // a tile's values and probabilities: two stages and the outputs of two CTAs an SM
+    // (whole sixteens: every row of a tile starts on a 16-byte boundary)
+    const int hdp = (a->c.hd + 31) / 32 * 32;
+    a->tp = std::max(16, (cols <= 8 ? std::min(64, 4096 / hdp) : std::min(32, 2048 / hdp)) / 16 * 16);
     a->heads = 1;
     while (a->heads < 8 && (int64_t)a->rows * a->nh > (int64_t)a->heads * 32 * sms) a->heads *= 2;
     const int per = cols <= 8 ? 8 : 16 * a->cg;
@@ -180,6 +184,17 @@ static int tree_scores(const TreeArgs &a, cudaStream_t s) {
     return tree_launch(k_tree_scores<NT, PK, W>, (int64_t)a.n_seq * a.c.nkv * a.groups * a.tiles, 1, 256,
                        tree_scores_smem(NT, a.c.hd), s, false, a);
 }
+template <int CB, bool PK, bool W>
+static int tree_pv(const TreeArgs &a, int64_t ctas, cudaStream_t s) {
+    static std::atomic<uint64_t> set{0};
+    int dev = 0;
+    IQ_CUDA(cudaGetDevice(&dev));
+    if (!(set.load() >> dev & 1)) {
+        IQ_CUDA(cudaFuncSetAttribute(k_tree_pv<CB, PK, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024));
+        set.fetch_or(1ull << dev);
+    }
+    return tree_launch(k_tree_pv<CB, PK, W>, ctas, 1, 256, tree_pv_smem<PK>(a.c.hd, a.cg * 8 * CB, a.tp, W), s, true, a);
+}
 template <bool PK, bool W>
 static int launch_tree(const TreeArgs &a, cudaStream_t s) {
     const bool eight = (int64_t)std::min(a.max_nodes, a.rows) * (a.nh / a.c.nkv) <= 8;
@@ -191,8 +206,7 @@ static int launch_tree(const TreeArgs &a, cudaStream_t s) {
                                             : tree_launch(k_tree_softmax<PK, true>, rows, hb, TREE_SM_T, 0, s, true, a);
     if (rc) return rc;
     const int64_t pv = (int64_t)a.n_seq * a.c.nkv * a.cblocks * a.chunks;
-    return eight ? tree_launch(k_tree_pv<1, PK, W>, pv, 1, 256, 0, s, true, a)
-                 : tree_launch(k_tree_pv<2, PK, W>, pv, 1, 256, 0, s, true, a);
+    return eight ? tree_pv<1, PK, W>(a, pv, s) : tree_pv<2, PK, W>(a, pv, s);
 }
 
 // CTAs a row (1, 2, 4 or 8): as many as fill the GPU with the rows at hand, but at least
@@ -378,9 +392,9 @@ IQ_API int iq_attn_tree_dev(int64_t *d_out, const int64_t *d_q, const iq_kv_cach
     const int64_t most = std::max({(int64_t)n_seq * a.c.nkv * a.groups * a.tiles,
                                    (int64_t)n_seq * a.c.nkv * a.cblocks * a.chunks, (int64_t)n_seq * max_nodes});
     if (most > INT_MAX) return IQ_ERR_RANGE;
-    // whole 32-wide steps in aligned pieces: 16 bytes of queries and exact vectors, 16 key and 2 value codes of packed ones
+    // whole 32-wide steps in aligned pieces: 16 bytes of queries, vectors and codes
     const bool wide = a.c.hd % 32 == 0 && !misaligned(d_q, 16) && q_stride % 2 == 0 &&
-                      (a.c.kbits ? !misaligned(a.c.kq, 16) && !misaligned(a.c.vq, 4)
+                      (a.c.kbits ? !misaligned(a.c.kq, 16) && !misaligned(a.c.vq, 16)
                                  : !misaligned(a.c.k, 16) && !misaligned(a.c.v, 16));
     cudaStream_t st = pick(stream);
     if (a.c.kbits) return wide ? launch_tree<true, true>(a, st) : launch_tree<true, false>(a, st);

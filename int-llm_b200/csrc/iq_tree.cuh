@@ -51,7 +51,7 @@ struct TreeArgs {
     int Tw;
     int tiles, tpc, groups, passes;   // k_tree_scores: CTAs along the positions, tiles each, groups of column blocks, blocks a group
     int heads;                        // k_tree_softmax: heads a CTA
-    int chunk, chunks, cg, cblocks;   // k_tree_pv: positions a CTA, their number, groups of 8 CB columns a block, blocks
+    int chunk, chunks, cg, cblocks, tp;   // k_tree_pv: positions a CTA, their number, groups of 8 CB columns a block, blocks, positions a tile
 };
 
 struct TreeSeq { int row0, n, len, sq; };
@@ -147,41 +147,6 @@ template <bool W> struct TreeKeys<true, W> {
     __device__ __forceinline__ void get(const TreeRows &r, int w, int64_t (&o)[4]) const {
 #pragma unroll
         for (int i = 0; i < 4; i++) o[i] = kv_value((q[w] >> (8 * i)) & 0xFF, m, r.bits);
-    }
-};
-// A lane's values of one position, as loaded: pairs at d and d + 16 (beyond hd anything).
-template <bool PK, bool W> struct TreeVals;
-template <bool W> struct TreeVals<false, W> {
-    longlong2 x[2];
-    __device__ __forceinline__ void load(const TreeRows &r, int t, int d) {
-        const int64_t *p = reinterpret_cast<const int64_t *>(r.x + (size_t)(uint32_t)min(t, r.T - 1) * r.rs) + d;
-        if constexpr (W) {
-            x[0] = *reinterpret_cast<const longlong2 *>(p);
-            x[1] = *reinterpret_cast<const longlong2 *>(p + 16);
-        } else {
-#pragma unroll
-            for (int k = 0; k < 2; k++) x[k] = make_longlong2(p[min(16 * k, r.hd - 1 - d)], p[min(16 * k + 1, r.hd - 1 - d)]);
-        }
-    }
-    __device__ __forceinline__ longlong2 get(const TreeRows &, int k) const { return x[k]; }
-};
-template <bool W> struct TreeVals<true, W> {
-    ushort2 q[2];
-    int64_t m;
-    __device__ __forceinline__ void load(const TreeRows &r, int t, int d) {
-        t = min(t, r.T - 1);
-        const uint16_t *p = reinterpret_cast<const uint16_t *>(r.x + (size_t)(uint32_t)t * r.rs) + d;
-        m = r.mag[(size_t)(uint32_t)t * r.ms];
-        if constexpr (W) {
-            q[0] = *reinterpret_cast<const ushort2 *>(p);
-            q[1] = *reinterpret_cast<const ushort2 *>(p + 16);
-        } else {
-#pragma unroll
-            for (int k = 0; k < 2; k++) q[k] = make_ushort2(p[min(16 * k, r.hd - 1 - d)], p[min(16 * k + 1, r.hd - 1 - d)]);
-        }
-    }
-    __device__ __forceinline__ longlong2 get(const TreeRows &r, int k) const {
-        return make_longlong2(kv_value(q[k].x, m, r.bits), kv_value(q[k].y, m, r.bits));
     }
 };
 // key or value d < hd of position t < T
@@ -657,105 +622,197 @@ __global__ void __launch_bounds__(TREE_SM_T) k_tree_softmax(const __grid_constan
 
 // ---------------------------------------------------- 3. probabilities x values
 
-#define TREE_RED 4096   // whole numbers of the buffer in which partial outputs meet
-
 // A CTA takes a.chunk positions of CG x 8 CB columns of one (sequence, kv head); a
 // warp 32 d of 8 CB columns and every tg_n-th four positions. A lane holds V of
 // position lane & 3 at d = 16 k + 2 (lane >> 2) + {0, 1}, k < 2, i.e. column lane >> 2 of
 // the 8-wide tiles 2k and 2k + 1, and of each tile's output the columns
-// 2 (lane & 3) + {0, 1}. Values come straight from global memory (the warps of the
-// CG column groups meet them in L1), D steps ahead: nothing is staged and no
-// barrier runs inside the loop.
+// 2 (lane & 3) + {0, 1}.
+// W: tiles of a.tp positions come through shared memory in two stages, each row of
+// values and of probabilities one bulk copy, so that whole rows are asked of HBM
+// at once, far ahead, and read once for all columns. Rows are 32 bytes apart
+// from a multiple of 128, which puts the four positions (or columns) of a
+// quarter-warp on different banks. Else the lanes read global memory themselves.
+struct TreeTile { int vrow, vpitch, ppitch, bytes; };   // bytes of a stage
+template <bool PK>
+__host__ __device__ constexpr TreeTile tree_tile(int hd, int nc, int tp) {
+    const int vrow = hd * (PK ? 2 : 8);
+    return TreeTile{vrow, vrow + 32, tp * 8 + 32, tp * (vrow + 32) + nc * (tp * 8 + 32) + (PK ? tp * 8 : 0)};
+}
+template <bool PK>
+__host__ __device__ constexpr size_t tree_pv_smem(int hd, int nc, int tp, bool w) {
+    return (size_t)nc * ((hd + 31) / 32 * 32) * 8 + (w ? 2 * (size_t)tree_tile<PK>(hd, nc, tp).bytes : 0);
+}
+__device__ __forceinline__ void bulk_row(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 :: "r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void async8(void *dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" :: "r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 template <int CB, bool PK, bool W>
 __global__ void __launch_bounds__(256, 2) k_tree_pv(const __grid_constant__ TreeArgs a) {
-    __shared__ __align__(16) unsigned long long red[TREE_RED];
-    constexpr int CW = 8 * CB, D = 2;   // steps ahead
+    extern __shared__ __align__(16) char tree_smem[];
+    __shared__ __align__(8) uint64_t full[2];
+    constexpr int CW = 8 * CB;
     const int chunk = blockIdx.x % a.chunks, rest = blockIdx.x / a.chunks;
     const int blk = rest % a.cblocks, g = rest / a.cblocks % a.c.nkv, b = rest / a.cblocks / a.c.nkv;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
     const int grp = a.nh / a.c.nkv, hd = a.c.hd, nd = (hd + 31) >> 5, hdp = nd * 32;
     TreeSeq s;
     if (!tree_seq(a, b, s)) return;
-    const int CG = a.cg, NC = CG * CW;   // NC hdp <= TREE_RED, CG nd <= 8
+    const int CG = a.cg, NC = CG * CW;   // CG nd <= 8
     const int cols = min(NC, s.n * grp - blk * NC), c0 = blk * NC, tb = chunk * a.chunk;
     const int Tl = min(a.chunk, s.len + s.n - tb);
     if (Tl <= 0 || cols <= 0) return;
+    unsigned long long *const red = reinterpret_cast<unsigned long long *>(tree_smem);   // [NC][hdp]
+    char *const stage = tree_smem + (size_t)NC * hdp * 8;
     const int units = CG * nd, tg_n = 8 / units;   // warps from units * tg_n on idle
     const int unit = warp % units, tg = warp / units, pc = unit % CG * CW, db = unit / CG * 32;
     const bool on = tg < tg_n && pc < cols;
     for (int e = tid; e < NC * hdp; e += 256) red[e] = 0;
     const TreeRows vr = tree_rows<PK>(a, true, ((size_t)s.sq * a.c.max_seq + tb) * a.c.nkv + g, Tl);
-    const double *pp[CB];   // this lane's columns (a missing one: the last, not kept)
-#pragma unroll
-    for (int cb = 0; cb < CB; cb++) {
-        const int cc = c0 + min(pc + cb * 8 + gq, cols - 1), n = cc / grp;
-        pp[cb] = reinterpret_cast<const double *>(a.sc) +
-                 ((size_t)(s.row0 + n) * a.nh + g * grp + cc - n * grp) * a.Tw + tb + tq;
-    }
+    auto prow = [&](int col) {   // a column's probabilities from tb on (a missing one: the last, not kept)
+        const int cc = c0 + min(col, cols - 1), n = cc / grp;
+        return reinterpret_cast<const double *>(a.sc) + ((size_t)(s.row0 + n) * a.nh + g * grp + cc - n * grp) * a.Tw + tb;
+    };
     double f[CB][4][2];
     uint32_t vm = 0;
-    const int step = tg_n * 4, tlast = (Tl - 1) & ~3;
-    // SPLIT: values beyond the chain as n 2^51 + f, 8 p n added in shared memory
-    auto sum = [&](auto split) {
+    const int step = tg_n * 4;
+    // four positions: probabilities p, values u (two pairs); SPLIT: values beyond the chain as
+    // n 2^51 + f, 8 p n added in shared memory
+    auto four = [&](auto split, const double (&p)[CB], const longlong2 (&u)[2], bool live) {
         constexpr bool SPLIT = decltype(split)::value;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            int64_t w[2] = {u[k].x, u[k].y};
+            if (SPLIT) {
+                const int64_t n0 = (w[0] >> 51) + (w[0] >> 50 & 1), n1 = (w[1] >> 51) + (w[1] >> 50 & 1);
+                // the other lanes' columns of this position too: p from the lane that holds it
+                for (int i = 0; i < CW; i++) {
+                    const double pi = __shfl_sync(0xffffffffu, CB == 1 || i < 8 ? p[0] : p[CB - 1], (i & 7) * 4 + tq);
+                    const uint64_t p8 = (uint64_t)(pi * 0x1p51);
+                    unsigned long long *dst = red + (pc + i) * hdp + db + 16 * k + 2 * gq;
+                    if (n0 && live) atomicAdd(dst, (unsigned long long)(p8 * (uint64_t)n0));
+                    if (n1 && live) atomicAdd(dst + 1, (unsigned long long)(p8 * (uint64_t)n1));
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                if (!SPLIT) tree_hi(vm, w[j], TREE_V1);
+                else w[j] = (int64_t)((uint64_t)w[j] << 13) >> 13;
+                const double v = __hiloint2double((int)(w[j] >> 32) + 0x43380000, (int)w[j]) - TREE_A;
+#pragma unroll
+                for (int cb = 0; cb < CB; cb++) dmma_rd(f[cb][2 * k + j][0], f[cb][2 * k + j][1], p[cb], v);
+            }
+        }
+    };
+    auto start = [&]() {
 #pragma unroll
         for (int cb = 0; cb < CB; cb++)
 #pragma unroll
             for (int k = 0; k < 4; k++) f[cb][k][0] = f[cb][k][1] = TREE_A;
-        TreeVals<PK, W> vx[D];
-        double pn[D][CB];
-        auto load = [&](int st, int t0) {   // beyond the end: the last four once more
-            const int t = min(t0, tlast);
-            vx[st].load(vr, t + tq, db + 2 * gq);
-#pragma unroll
-            for (int cb = 0; cb < CB; cb++) pn[st][cb] = pp[cb][t];
+    };
+    if constexpr (W) {
+        const int tp = a.tp, nst = (Tl + tp - 1) / tp;
+        const TreeTile tl = tree_tile<PK>(hd, NC, tp);
+        auto nv = [&](int i) { return min(tp, Tl - i * tp); };
+        // (p rows are zero up to the next multiple of four positions)
+        auto load_v = [&](int i, int sl) {
+            char *st = stage + sl * tl.bytes;
+            const int n = nv(i);
+            if (tid == 0)
+                mbar_expect_tx(&full[sl], (uint32_t)(n * tl.vrow + NC * ((n + 3) & ~3) * 8));
+            if (tid < n) {
+                const size_t t = (size_t)(i * tp + tid);
+                bulk_row(st + tid * tl.vpitch, vr.x + t * vr.rs, tl.vrow, &full[sl]);
+                if (PK) async8(st + tp * tl.vpitch + NC * tl.ppitch + tid * 8, vr.mag + t * vr.ms);
+            }
         };
-        auto four = [&](int st, int t0) {
-            double p[CB], v[4];
+        auto load_p = [&](int i, int sl) {
+            char *st = stage + sl * tl.bytes + tp * tl.vpitch;
+            if (tid >= 256 - NC)
+                bulk_row(st + (255 - tid) * tl.ppitch, prow(255 - tid) + i * tp, ((nv(i) + 3) & ~3) * 8, &full[sl]);
+        };
+        if (tid == 0) {
+            mbar_init(&full[0], 1);
+            mbar_init(&full[1], 1);
+            fence_mbar_init();
+        }
+        __syncthreads();
+        int batch = 0;   // tiles loaded: tile number batch of this CTA waits for phase batch >> 1 of its stage
+        auto sum = [&](auto split, bool first) {
+            start();
+            for (int i = 0; i < min(2, nst); i++) load_v(i, (batch + i) & 1);
+            if (first) tree_prev_kernel();
+            for (int i = 0; i < min(2, nst); i++) load_p(i, (batch + i) & 1);
+            async_wait();
+            __syncthreads();
+            for (int i = 0; i < nst; i++, batch++) {
+                const int sl = batch & 1, n = nv(i);
+                mbar_wait(&full[sl], (uint32_t)(batch >> 1) & 1u);
+                const char *sv = stage + sl * tl.bytes, *sp = sv + tp * tl.vpitch;
+                if (on)
+                    for (int t0 = tg * 4; t0 < n; t0 += step) {
+                        const int t = min(t0 + tq, n - 1);
+                        const char *row = sv + t * tl.vpitch;
+                        double p[CB];
 #pragma unroll
-            for (int cb = 0; cb < CB; cb++) p[cb] = pn[st][cb];
+                        for (int cb = 0; cb < CB; cb++)
+                            p[cb] = *reinterpret_cast<const double *>(sp + (pc + cb * 8 + gq) * tl.ppitch + (t0 + tq) * 8);
+                        longlong2 u[2];
+                        if (PK) {
+                            const int64_t M = *reinterpret_cast<const int64_t *>(sp + NC * tl.ppitch + t * 8);
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const longlong2 u = vx[st].get(vr, k);
-                int64_t w[2] = {u.x, u.y};
+                            for (int k = 0; k < 2; k++) {
+                                const ushort2 q = *reinterpret_cast<const ushort2 *>(row + (db + 16 * k + 2 * gq) * 2);
+                                u[k] = make_longlong2(kv_value(q.x, M, vr.bits), kv_value(q.y, M, vr.bits));
+                            }
+                        } else {
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    if (!SPLIT) tree_hi(vm, w[j], TREE_V1);
-                    else w[j] = (int64_t)((uint64_t)w[j] << 13) >> 13;
-                    v[2 * k + j] = __hiloint2double((int)(w[j] >> 32) + 0x43380000, (int)w[j]) - TREE_A;
-                }
-                if (SPLIT) {
-                    const int64_t n0 = (u.x >> 51) + (u.x >> 50 & 1), n1 = (u.y >> 51) + (u.y >> 50 & 1);
-                    // the other lanes' columns of this position too: p from the lane that holds it
-                    for (int i = 0; i < CW; i++) {
-                        const double pi = __shfl_sync(0xffffffffu, CB == 1 || i < 8 ? p[0] : p[CB - 1], (i & 7) * 4 + tq);
-                        const uint64_t p8 = (uint64_t)(pi * 0x1p51);
-                        unsigned long long *dst = red + (pc + i) * hdp + db + 16 * k + 2 * gq;
-                        if (n0 && t0 + tq < Tl) atomicAdd(dst, (unsigned long long)(p8 * (uint64_t)n0));
-                        if (n1 && t0 + tq < Tl) atomicAdd(dst + 1, (unsigned long long)(p8 * (uint64_t)n1));
+                            for (int k = 0; k < 2; k++)
+                                u[k] = *reinterpret_cast<const longlong2 *>(row + (db + 16 * k + 2 * gq) * 8);
+                        }
+                        four(split, p, u, t0 + tq < n);
                     }
+                async_wait();
+                __syncthreads();   // the tile is consumed, the next one's magnitudes are here
+                if (i + 2 < nst) {
+                    load_v(i + 2, sl);
+                    load_p(i + 2, sl);
                 }
             }
-            load(st, t0 + D * step);
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-#pragma unroll
-                for (int cb = 0; cb < CB; cb++) dmma_rd(f[cb][k][0], f[cb][k][1], p[cb], v[k]);
         };
+        sum(std::false_type{}, true);
+        if (__syncthreads_or(vm >= 2 * TREE_V1)) sum(std::true_type{}, false);   // a value beyond the chain: once more
+    } else {
+        const double *pp[CB];
 #pragma unroll
-        for (int st = 0; st < D; st++) load(st, tg * 4 + st * step);
+        for (int cb = 0; cb < CB; cb++) pp[cb] = prow(pc + cb * 8 + gq) + tq;
+        auto sum = [&](auto split) {
+            start();
 #pragma unroll 1
-        for (int t0 = tg * 4; t0 < Tl; t0 += D * step) {
+            for (int t0 = tg * 4; t0 < Tl; t0 += step) {
+                double p[CB];
 #pragma unroll
-            for (int st = 0; st < D; st++)
-                if (st == 0 || t0 + st * step < Tl) four(st, t0 + st * step);
+                for (int cb = 0; cb < CB; cb++) p[cb] = pp[cb][t0];
+                longlong2 u[2];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const int t = min(t0 + tq, Tl - 1), d = db + 16 * k + 2 * gq;
+                    u[k].x = tree_val<PK>(vr, t, min(d, hd - 1));
+                    u[k].y = tree_val<PK>(vr, t, min(d + 1, hd - 1));
+                }
+                four(split, p, u, t0 + tq < Tl);
+            }
+        };
+        tree_prev_kernel();
+        __syncthreads();
+        if (on) {
+            sum(std::false_type{});
+            if (__any_sync(0xffffffffu, vm >= 2 * TREE_V1)) sum(std::true_type{});
         }
-    };
-    tree_prev_kernel();
-    __syncthreads();
-    if (on) {
-        sum(std::false_type{});
-        if (__any_sync(0xffffffffu, vm >= 2 * TREE_V1)) sum(std::true_type{});   // a value beyond the chain: once more
     }
     // partial outputs of the tg_n position groups meet in shared memory, group after group
     const int od = db + 4 * tq;   // tile k, output j: + 16 (k >> 1) + (k & 1) + 2 j
