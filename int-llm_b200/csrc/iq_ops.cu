@@ -202,8 +202,9 @@ static int launch_tree(const TreeArgs &a, cudaStream_t s) {
     if (rc) return rc;
     const int64_t rows = (int64_t)a.n_seq * a.max_nodes;
     const int hb = (a.nh + a.heads - 1) / a.heads;
-    rc = a.max_len <= TREE_SM_T * TREE_SM_E ? tree_launch(k_tree_softmax<PK, false>, rows, hb, TREE_SM_T, 0, s, true, a)
-                                            : tree_launch(k_tree_softmax<PK, true>, rows, hb, TREE_SM_T, 0, s, true, a);
+    rc = a.Tw <= TREE_SM_MAX
+             ? tree_launch(k_tree_softmax<PK, true>, rows, hb, TREE_SM_T, (size_t)a.Tw * 8, s, true, a)
+             : tree_launch(k_tree_softmax<PK, false>, rows, hb, TREE_SM_T, 0, s, true, a);
     if (rc) return rc;
     const int64_t pv = (int64_t)a.n_seq * a.c.nkv * a.cblocks * a.chunks;
     return eight ? tree_pv<1, PK, W>(a, pv, s) : tree_pv<2, PK, W>(a, pv, s);

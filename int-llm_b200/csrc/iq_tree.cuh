@@ -512,14 +512,17 @@ __device__ __noinline__ void tree_wrapped(const TreeArgs &a, const TreeSeq &s, i
     for (int t = threadIdx.x; t < min(a.Tw, (s.len + s.n + 3) & ~3); t += blockDim.x) row[t] = 0;
 }
 
-// A CTA a node row and a.heads of its heads. E scores a thread stay in registers; longer rows go
-// through the workspace three times (LONG). A row whose score differences
-// wrap (the reference's int64 then gives other numbers, reproduced here) is
-// finished here term by term and leaves zeros to k_tree_pv.
+// A CTA a node row and a.heads of its heads. The scores stay in shared memory
+// (SM), longer rows in the workspace. Positions that the row does not see get a
+// score 11 below the maximum, whose exponential is 0, so that one loop serves
+// all. A row whose score differences wrap (the reference's int64 then gives other
+// numbers, reproduced here) is finished here term by term and leaves zeros to
+// k_tree_pv.
 #define TREE_SM_T 128
-#define TREE_SM_E 16
-template <bool PK, bool LONG>
-__global__ void __launch_bounds__(TREE_SM_T) k_tree_softmax(const __grid_constant__ TreeArgs a) {
+#define TREE_SM_MAX 2560   // positions whose scores are kept in shared memory
+template <bool PK, bool SM>
+__global__ void __launch_bounds__(TREE_SM_T, 8) k_tree_softmax(const __grid_constant__ TreeArgs a) {
+    extern __shared__ __align__(16) char tree_smem[];
     __shared__ uint64_t red[64];
     __shared__ int64_t wmax[2][TREE_SM_T / 32];
     __shared__ uint64_t wsum[2][TREE_SM_T / 32];
@@ -550,49 +553,37 @@ __global__ void __launch_bounds__(TREE_SM_T) k_tree_softmax(const __grid_constan
     const int h0 = blockIdx.y * a.heads, h1 = min(h0 + a.heads, a.nh);
     for (int h = h0; h < h1; h++) {
         const int par = h & 1;   // the other half of wmax and wsum may still be read
-        int64_t *row = a.sc + ((size_t)r * a.nh + h) * a.Tw;
-        int64_t x[TREE_SM_E], m = INT64_MIN;
-        for (int t0 = 0; t0 < (LONG ? T : 1); t0 += TREE_SM_T * TREE_SM_E) {
-#pragma unroll
-            for (int k = 0; k < TREE_SM_E; k++) {
-                const int tk = t0 + k * TREE_SM_T, t = tk + tid;
-                x[k] = INT64_MIN;
-                if (tk + TREE_SM_T <= s.len) {   // all before the draft
-                    x[k] = row[t];
-                } else if (tk < T) {
-                    if (t < T) x[k] = row[t];
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < TREE_SM_E; k++) {
-                const int tk = t0 + k * TREE_SM_T, t = tk + tid;
-                if (tk + TREE_SM_T <= s.len) m = max(m, x[k]);
-                else if (tk < T && sees(t)) m = max(m, x[k]);
-            }
+        int64_t *row = a.sc + ((size_t)r * a.nh + h) * a.Tw, m = INT64_MIN;
+        int64_t *x = SM ? reinterpret_cast<int64_t *>(tree_smem) : row;   // each thread its own positions throughout
+#pragma unroll 4
+        for (int t = tid; t < s.len; t += TREE_SM_T) {
+            const int64_t v = row[t];
+            m = max(m, v);
+            if (SM) x[t] = v;
         }
+        const int t_end = s.len + (tid - s.len % TREE_SM_T + TREE_SM_T) % TREE_SM_T;   // its first position from the draft on
+        for (int t = t_end; t < end; t += TREE_SM_T)
+            if (sees(t)) {
+                m = max(m, row[t]);
+                if (SM) x[t] = row[t];
+            }
         for (int k = 16; k >= 1; k >>= 1) m = max(m, (int64_t)__shfl_xor_sync(0xffffffffu, m, k));
         if ((tid & 31) == 0) wmax[par][tid >> 5] = m;
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < TREE_SM_T / 32; k++) m = max(m, wmax[par][k]);
+        for (int t = t_end; t < end; t += TREE_SM_T)
+            if (!sees(t)) x[t] = (int64_t)((uint64_t)m - 11 * (uint64_t)IQ_ONE);
         uint64_t sum = 0;
-        int wraps = 0;   // sign: a seen difference of 2^63 or more
-        for (int t0 = 0; t0 < (LONG ? T : 1); t0 += TREE_SM_T * TREE_SM_E) {
-#pragma unroll
-            for (int k = 0; k < TREE_SM_E; k++) {
-                const int tk = t0 + k * TREE_SM_T, t = tk + tid;
-                if (tk < T) {
-                    if (LONG) x[k] = t < T ? row[t] : INT64_MIN;
-                    const uint64_t d = (uint64_t)m - (uint64_t)x[k];
-                    const int64_t e = tree_exp(d);   // (anything where d is beyond 10)
-                    bool in = d <= 10 * (uint64_t)IQ_ONE;
-                    if (tk + TREE_SM_T > s.len && !sees(t)) in = false;
-                    else wraps |= (int)(d >> 32);
-                    x[k] = in ? e : 0;
-                    sum += (uint64_t)x[k];
-                    if (LONG && t < T) row[t] = x[k];
-                }
-            }
+        int wraps = 0;   // sign: a difference of 2^63 or more
+#pragma unroll 4
+        for (int t = tid; t < end; t += TREE_SM_T) {
+            const uint64_t d = (uint64_t)m - (uint64_t)x[t];
+            wraps |= (int)(d >> 32);
+            const int64_t e = tree_exp(d);   // (anything where d is beyond 10)
+            const int64_t v = d <= 10 * (uint64_t)IQ_ONE ? e : 0;
+            x[t] = v;
+            sum += (uint64_t)v;
         }
         for (int k = 16; k >= 1; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
         if ((tid & 31) == 0) wsum[par][tid >> 5] = sum;
@@ -606,16 +597,8 @@ __global__ void __launch_bounds__(TREE_SM_T) k_tree_softmax(const __grid_constan
         for (int k = 0; k < TREE_SM_T / 32; k++) S += wsum[par][k];
         const double inv = f64_rcp(f64_u64(S)) * (0x1p48 - 0x1p-2);
         double *p = reinterpret_cast<double *>(row);
-        for (int t0 = 0; t0 < (LONG ? end : 1); t0 += TREE_SM_T * TREE_SM_E) {
-#pragma unroll
-            for (int k = 0; k < TREE_SM_E; k++) {
-                const int tk = t0 + k * TREE_SM_T, t = tk + tid;
-                if (tk < end) {
-                    const int64_t e = LONG ? (t < T ? row[t] : 0) : t < T ? x[k] : 0;
-                    if (t < end) p[t] = tree_prob(e, (int64_t)S, inv);
-                }
-            }
-        }
+#pragma unroll 4
+        for (int t = tid; t < end; t += TREE_SM_T) p[t] = tree_prob(x[t], (int64_t)S, inv);
         for (int d = tid; d < hd; d += TREE_SM_T) out[d] = 0;   // k_tree_pv adds
     }
 }
@@ -718,22 +701,23 @@ __global__ void __launch_bounds__(256, 2) k_tree_pv(const __grid_constant__ Tree
         const int tp = a.tp, nst = (Tl + tp - 1) / tp;
         const TreeTile tl = tree_tile<PK>(hd, NC, tp);
         auto nv = [&](int i) { return min(tp, Tl - i * tp); };
+        const int own = lane * 8 + warp;   // the row that this thread copies: a warp issues its lanes' copies in turn, so all warps share them
+        const double *my_p = prow(own);
         // (p rows are zero up to the next multiple of four positions)
         auto load_v = [&](int i, int sl) {
             char *st = stage + sl * tl.bytes;
             const int n = nv(i);
             if (tid == 0)
                 mbar_expect_tx(&full[sl], (uint32_t)(n * tl.vrow + NC * ((n + 3) & ~3) * 8));
-            if (tid < n) {
-                const size_t t = (size_t)(i * tp + tid);
-                bulk_row(st + tid * tl.vpitch, vr.x + t * vr.rs, tl.vrow, &full[sl]);
-                if (PK) async8(st + tp * tl.vpitch + NC * tl.ppitch + tid * 8, vr.mag + t * vr.ms);
+            if (own < n) {
+                const size_t t = (size_t)(i * tp + own);
+                bulk_row(st + own * tl.vpitch, vr.x + t * vr.rs, tl.vrow, &full[sl]);
+                if (PK) async8(st + tp * tl.vpitch + NC * tl.ppitch + own * 8, vr.mag + t * vr.ms);
             }
         };
         auto load_p = [&](int i, int sl) {
             char *st = stage + sl * tl.bytes + tp * tl.vpitch;
-            if (tid >= 256 - NC)
-                bulk_row(st + (255 - tid) * tl.ppitch, prow(255 - tid) + i * tp, ((nv(i) + 3) & ~3) * 8, &full[sl]);
+            if (own < NC) bulk_row(st + own * tl.ppitch, my_p + i * tp, ((nv(i) + 3) & ~3) * 8, &full[sl]);
         };
         if (tid == 0) {
             mbar_init(&full[0], 1);
@@ -753,29 +737,33 @@ __global__ void __launch_bounds__(256, 2) k_tree_pv(const __grid_constant__ Tree
                 const int sl = batch & 1, n = nv(i);
                 mbar_wait(&full[sl], (uint32_t)(batch >> 1) & 1u);
                 const char *sv = stage + sl * tl.bytes, *sp = sv + tp * tl.vpitch;
-                if (on)
-                    for (int t0 = tg * 4; t0 < n; t0 += step) {
-                        const int t = min(t0 + tq, n - 1);
-                        const char *row = sv + t * tl.vpitch;
-                        double p[CB];
+                auto at = [&](int t0, int t) {   // positions t0 .. t0 + 3, this lane's values at t
+                    const char *row = sv + t * tl.vpitch;
+                    double p[CB];
 #pragma unroll
-                        for (int cb = 0; cb < CB; cb++)
-                            p[cb] = *reinterpret_cast<const double *>(sp + (pc + cb * 8 + gq) * tl.ppitch + (t0 + tq) * 8);
-                        longlong2 u[2];
-                        if (PK) {
-                            const int64_t M = *reinterpret_cast<const int64_t *>(sp + NC * tl.ppitch + t * 8);
+                    for (int cb = 0; cb < CB; cb++)
+                        p[cb] = *reinterpret_cast<const double *>(sp + (pc + cb * 8 + gq) * tl.ppitch + (t0 + tq) * 8);
+                    longlong2 u[2];
+                    if (PK) {
+                        const int64_t M = *reinterpret_cast<const int64_t *>(sp + NC * tl.ppitch + t * 8);
 #pragma unroll
-                            for (int k = 0; k < 2; k++) {
-                                const ushort2 q = *reinterpret_cast<const ushort2 *>(row + (db + 16 * k + 2 * gq) * 2);
-                                u[k] = make_longlong2(kv_value(q.x, M, vr.bits), kv_value(q.y, M, vr.bits));
-                            }
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 2; k++)
-                                u[k] = *reinterpret_cast<const longlong2 *>(row + (db + 16 * k + 2 * gq) * 8);
+                        for (int k = 0; k < 2; k++) {
+                            const ushort2 q = *reinterpret_cast<const ushort2 *>(row + (db + 16 * k + 2 * gq) * 2);
+                            u[k] = make_longlong2(kv_value(q.x, M, vr.bits), kv_value(q.y, M, vr.bits));
                         }
-                        four(split, p, u, t0 + tq < n);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 2; k++)
+                            u[k] = *reinterpret_cast<const longlong2 *>(row + (db + 16 * k + 2 * gq) * 8);
                     }
+                    four(split, p, u, t0 + tq < n);
+                };
+                if (on && n == tp) {
+#pragma unroll 4
+                    for (int t0 = tg * 4; t0 < tp; t0 += step) at(t0, t0 + tq);
+                } else if (on) {
+                    for (int t0 = tg * 4; t0 < n; t0 += step) at(t0, min(t0 + tq, n - 1));
+                }
                 async_wait();
                 __syncthreads();   // the tile is consumed, the next one's magnitudes are here
                 if (i + 2 < nst) {

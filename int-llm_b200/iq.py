@@ -383,6 +383,8 @@ def _dev_ptr(t, itemsize, name):
 def _cur(stream):
     """Stream argument as _sp's: an explicit one, else torch's current stream."""
     if stream is None:
+        if _raw_device is None:
+            _bind_torch()
         return _raw_stream(_raw_device()) or _CUDA_STREAM_LEGACY
     return getattr(stream, "cuda_stream", stream)
 
