@@ -654,3 +654,83 @@ def test_verifying_a_draft_equals_the_model(kvb):
     for i in range(n):
         lp, _, best, bl = ref.logprobs(logits[i].tolist(), tok[i], 4)
         assert (int(logp[i]), ids[i].tolist(), tl[i].tolist()) == (lp, best, bl)
+
+
+# -------------------------------------------- other shapes and paths of the kernels
+
+@pytest.mark.parametrize("nh,nkv,hd,n", [(8, 2, 128, 9), (8, 1, 192, 5), (16, 1, 64, 9), (24, 1, 32, 7), (3, 3, 160, 20)])
+@pytest.mark.parametrize("kvb", [(0, 0), (7, 13)])
+def test_tree_many_columns_a_kv_head(nh, nkv, hd, n, kvb):
+    """Several blocks of columns over one set of keys, narrow and wide heads."""
+    rng = np.random.default_rng(hd + n)
+    check_tree(rng, nh, nkv, hd, [150, 20], [bush(rng, n), bush(rng, max(1, n // 2))], kvb)
+
+
+def test_tree_unaligned_cache_and_queries():
+    """Cache and query pointers on 8-byte boundaries only give the same results."""
+    rng = np.random.default_rng(18)
+    nh, nkv, hd, S, M = 8, 2, 64, 2, 75
+    q, k, v = rnd(rng, 9, nh, hd), rnd(rng, S, M, nkv, hd), rnd(rng, S, M, nkv, hd)
+    trees = [bush(rng, 4), bush(rng, 5)]
+    args = ((0, 0), [70, 30], [0, 4, 9], trees[0] + trees[1], nh)
+    want = run_tree(dev(q.reshape(9, -1)), dict(k=dev(k), v=dev(v)), *args)
+
+    def shifted(a):
+        buf = torch.empty(a.size + 1, dtype=torch.int64, device="cuda")
+        buf[1:].copy_(dev(a).flatten())
+        return buf[1:].view(a.shape)
+
+    assert (run_tree(shifted(q.reshape(9, -1)), dict(k=shifted(k), v=shifted(v)), *args) == want).all()
+    assert (run_tree(dev(q.reshape(9, -1)), dict(k=dev(k), v=shifted(v)), *args) == want).all()
+    assert (want == ref.tree(q, list(k), list(v), [70, 30], [0, 4, 9], trees[0] + trees[1], nh).reshape(9, -1)).all()
+
+
+def test_tree_batched_decode_over_several_tiles():
+    """Many single tokens: a block of columns walks over several tiles of positions."""
+    rng = np.random.default_rng(19)
+    S, nh, nkv, hd, M = 150, 16, 8, 32, 1300
+    lens = [int(x) for x in rng.integers(0, M - 1, S)]
+    lens[:4] = [0, 127, 128, M - 1]
+    k, v, q = rnd(rng, S, M, nkv, hd), rnd(rng, S, M, nkv, hd), rnd(rng, S, nh, hd)
+    got = run_tree(dev(q.reshape(S, -1)), dict(k=dev(k), v=dev(v)), (0, 0), lens, list(range(S + 1)), [-1] * S, nh)
+    scale = ref.fp(ref.INV_SQRT, hd << 48)
+    for b in [0, 1, 2, 3, 77, 149]:
+        for h in (0, 7, 15):
+            want = ref.attend(q[b, h], k[b, : lens[b] + 1, h // 2], v[b, : lens[b] + 1, h // 2], scale)
+            assert (got[b, h * hd:(h + 1) * hd] == want).all()
+
+
+@pytest.mark.parametrize("vs", [7.99, 8.01, 63.0, 300.0])
+def test_tree_large_values_everywhere(vs):
+    """Every value near +-vs, wide tiles and several chunks of positions."""
+    rng = np.random.default_rng(20)
+    v = ref.q48(vs) * rng.choice([-1, 1], (1, 700, 2, 64)) + rng.integers(-1000, 1000, (1, 700, 2, 64))
+    k = rnd(rng, 1, 700, 2, 64)
+    check_tree(rng, 8, 2, 64, [690], [bush(rng, 3)], k=k, v=v, pad=7)
+
+
+def test_logprobs_a_block_a_row():
+    """Enough rows that each is one block's, rows longer than its shared memory, ties among them."""
+    rng = np.random.default_rng(21)
+    l = rnd(rng, 300, 6001, scale=3)
+    l[7] = 5
+    l[8, ::3] = l[8].max() + 1
+    l[9] = ref.I64_MIN
+    check_logprobs(l, rng.integers(0, 6001, 300), 4, ld=6002)
+
+
+def test_wide_and_narrow_forms_agree():
+    """Rotation and cache rows through 16-byte pieces and element by element (shifted pointers)."""
+    rng = np.random.default_rng(22)
+    rows, heads, hd, rot, n = 5, 3, 64, 48, 20
+    x, cos, sin = rnd(rng, rows, heads * hd, scale=2000), rnd(rng, n, rot // 2), rnd(rng, n, rot // 2)
+    x[0, :8] = [ref.I64_MAX, ref.I64_MIN, 1 << 60, -(1 << 60), (1 << 60) - 1, 0, 1, -1]
+    cos[0, :3] = [1 << 49, (1 << 49) - 1, -(1 << 49)]
+    pos = np.array([0, 1, 0, 19, 7])
+    for layout in ("half", "interleaved"):
+        r = iq.Rope(dev(cos), dev(sin), i32(pos), n, rot, layout)
+        a, b = full(rows, heads * hd), torch.full((rows * heads * hd + 1,), KEEP, dtype=torch.int64, device="cuda")
+        iq.rope_dev(a, dev(x), r, rows, heads, hd)
+        iq.rope_dev(b[1:], dev(x), r, rows, heads, hd)
+        want = ref.rotate(x.reshape(rows, heads, hd), cos[pos], sin[pos], rot, layout).reshape(rows, -1)
+        assert (a.cpu().numpy() == want).all() and (b[1:].cpu().numpy().reshape(rows, -1) == want).all()
