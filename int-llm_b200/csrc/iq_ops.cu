@@ -148,9 +148,11 @@ static void tree_plan(TreeArgs *a) {
     while (a->heads < 8 && (int64_t)a->rows * a->nh > (int64_t)a->heads * 32 * sms) a->heads *= 2;
     const int per = cols <= 8 ? 8 : 16 * a->cg;
     a->cblocks = (int)((cols + per - 1) / per);
-    a->chunk = 1024;
-    const int64_t pv = pairs * ((avg + per - 1) / per);
-    while (a->chunk > 128 && pv * ((a->max_len + a->chunk - 1) / a->chunk) < 4 * sms) a->chunk /= 2;
+    // long chunks (a CTA's start and end cost as much as 100 positions); with 8 columns
+    // already when they make one wave (decode batch: 512 positions 63 us, 1024 55 us)
+    a->chunk = 2048;
+    const int64_t pv = pairs * ((avg + per - 1) / per), want = cols <= 8 ? sms * 3 / 2 : 4 * sms;
+    while (a->chunk > 128 && pv * ((a->max_len + a->chunk - 1) / a->chunk) < want) a->chunk /= 2;
     a->chunks = (a->max_len + a->chunk - 1) / a->chunk;
 }
 

@@ -236,10 +236,10 @@ __host__ __device__ constexpr size_t tree_scores_smem(int NT, int hd) { return 1
 // A CTA takes a.tpc tiles of 128 positions of one (sequence, kv head) and up to
 // a.passes blocks of NC = 8 NT columns. With hd <= 64 the key planes of a tile are made
 // once for all its blocks, with one block the query planes once for all its tiles.
-// Two CTAs an SM (four with 8 columns) overlap one another's loads, products
-// and epilogues; TMEM holds 128 NT columns a CTA.
+// Two CTAs an SM (three with 8 columns; four would spill: 92 us for 90, decode
+// batch) overlap one another's loads, products and epilogues; TMEM holds 128 NT columns a CTA.
 template <int NT, bool PK, bool W>
-__global__ void __launch_bounds__(256, NT == 1 ? 4 : 2) k_tree_scores(const __grid_constant__ TreeArgs a) {
+__global__ void __launch_bounds__(256, NT == 1 ? 3 : 2) k_tree_scores(const __grid_constant__ TreeArgs a) {
     extern __shared__ __align__(16) char tree_smem[];
     constexpr int NC = 8 * NT, HC = NC / 2;
     __shared__ int64_t ksum[128];              // sum of a position's key
@@ -521,7 +521,7 @@ __device__ __noinline__ void tree_wrapped(const TreeArgs &a, const TreeSeq &s, i
 #define TREE_SM_T 128
 #define TREE_SM_MAX 2560   // positions whose scores are kept in shared memory
 template <bool PK, bool SM>
-__global__ void __launch_bounds__(TREE_SM_T, 8) k_tree_softmax(const __grid_constant__ TreeArgs a) {
+__global__ void __launch_bounds__(TREE_SM_T, 10) k_tree_softmax(const __grid_constant__ TreeArgs a) {
     extern __shared__ __align__(16) char tree_smem[];
     __shared__ uint64_t red[64];
     __shared__ int64_t wmax[2][TREE_SM_T / 32];
