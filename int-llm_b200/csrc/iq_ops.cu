@@ -128,9 +128,12 @@ static void tree_plan(TreeArgs *a) {
     a->Tw = (a->max_len + 3) / 4 * 4;
     // columns of all sequences, on average over them
     const int64_t avg = std::max<int64_t>(1, (int64_t)a->rows * grp / a->n_seq);
+    // 8 columns a block for single tokens of up to 8 heads a kv head (64 of them at 2000
+    // positions: 175 us, with half-empty blocks of 16: 190 us)
     const int nt = cols <= 8 ? 1 : 2, blocks = (int)((cols + 8 * nt - 1) / (8 * nt));
-    // up to 8 blocks share the key planes, fewer where that leaves SMs without a CTA;
-    // a single block's CTA walks over up to 8 tiles on the same terms
+    // up to 8 blocks share the key planes (8 drafts of 16-48 nodes: 339 us; 2 blocks 363, one
+    // 414), fewer where that leaves SMs without a CTA; a single block's CTA walks over up to
+    // 8 tiles on the same terms (64 single tokens: 175 us; one tile a CTA 179)
     const int tiles = (a->max_len + 127) / 128;
     const int64_t pairs = (int64_t)a->n_seq * a->c.nkv;
     a->passes = 8;
@@ -139,17 +142,19 @@ static void tree_plan(TreeArgs *a) {
     while (a->tpc > 1 && pairs * ((tiles + a->tpc - 1) / a->tpc) < 6 * sms) a->tpc /= 2;
     a->tiles = (tiles + a->tpc - 1) / a->tpc;
     a->groups = (blocks + a->passes - 1) / a->passes;
-    a->cg = cols > 32 && a->c.hd <= 64 ? 4 : cols > 16 && a->c.hd <= 128 ? 2 : 1;   // cg hd <= 256
-    // a tile's values and probabilities: two stages and the outputs of two CTAs an SM
-    // (whole sixteens: every row of a tile starts on a 16-byte boundary)
+    // groups of 16 columns that share a tile of values (cg hd <= 256), once the sequences fill
+    // them: 52 columns of 128: 2 groups 344 us, 1 group 360; 32 columns of 64: 139 and 126;
+    // 256 columns of 64: 4 groups 339 us, 2 groups 341, 1 group 355
+    a->cg = avg >= 96 && a->c.hd <= 64 ? 4 : avg >= 48 && a->c.hd <= 128 ? 2 : 1;
+    // positions a tile of values and probabilities: two stages and the outputs of two CTAs
+    // an SM (whole sixteens: every row of a tile starts on a 16-byte boundary). Short
+    // tiles cost: 16 positions for 64 take 206 us for 175 with single tokens, 352 for 339 with drafts
     const int hdp = (a->c.hd + 31) / 32 * 32;
     a->tp = std::max(16, (cols <= 8 ? std::min(64, 4096 / hdp) : std::min(32, 2048 / hdp)) / 16 * 16);
-    a->heads = 1;
-    while (a->heads < 8 && (int64_t)a->rows * a->nh > (int64_t)a->heads * 32 * sms) a->heads *= 2;
     const int per = cols <= 8 ? 8 : 16 * a->cg;
     a->cblocks = (int)((cols + per - 1) / per);
     // long chunks (a CTA's start and end cost as much as 100 positions); with 8 columns
-    // already when they make one wave (decode batch: 512 positions 63 us, 1024 55 us)
+    // already when they make one wave (64 single tokens: 512 positions 63 us, 1024 54 us)
     a->chunk = 2048;
     const int64_t pv = pairs * ((avg + per - 1) / per), want = cols <= 8 ? sms * 3 / 2 : 4 * sms;
     while (a->chunk > 128 && pv * ((a->max_len + a->chunk - 1) / a->chunk) < want) a->chunk /= 2;
@@ -203,17 +208,19 @@ static int launch_tree(const TreeArgs &a, cudaStream_t s) {
     int rc = eight ? tree_scores<1, PK, W>(a, s) : tree_scores<2, PK, W>(a, s);
     if (rc) return rc;
     const int64_t rows = (int64_t)a.n_seq * a.max_nodes;
-    const int hb = (a.nh + a.heads - 1) / a.heads;
+    // scores in shared memory: 339 us for 343 (drafts)
     rc = a.Tw <= TREE_SM_MAX
-             ? tree_launch(k_tree_softmax<PK, true>, rows, hb, TREE_SM_T, (size_t)a.Tw * 8, s, true, a)
-             : tree_launch(k_tree_softmax<PK, false>, rows, hb, TREE_SM_T, 0, s, true, a);
+             ? tree_launch(k_tree_softmax<PK, true>, rows, a.nh, TREE_SM_T, (size_t)a.Tw * 8, s, true, a)
+             : tree_launch(k_tree_softmax<PK, false>, rows, a.nh, TREE_SM_T, 0, s, true, a);
     if (rc) return rc;
     const int64_t pv = (int64_t)a.n_seq * a.c.nkv * a.cblocks * a.chunks;
     return eight ? tree_pv<1, PK, W>(a, pv, s) : tree_pv<2, PK, W>(a, pv, s);
 }
 
 // CTAs a row (1, 2, 4 or 8): as many as fill the GPU with the rows at hand, but at least
-// 2048 logits a CTA; more where the slices of five CTAs would not fit an SM. A slice beyond one CTA's shared memory is read twice.
+// 2048 logits a CTA; more where the slices of five CTAs would not fit an SM. A slice beyond
+// one CTA's shared memory is read twice, and so are rows that fill the GPU with one CTA
+// each (512 rows of 32000: 89 us; in shared memory over a cluster 124 us).
 static int lp_launch(LpArgs *a, cudaStream_t s) {
     static std::atomic<uint64_t> set{0};   // devices whose shared-memory limit is raised
     const size_t many = 36 * 1024, one = 200 * 1024;

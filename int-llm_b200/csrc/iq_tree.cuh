@@ -50,7 +50,6 @@ struct TreeArgs {
     int64_t *sc;    // workspace [rows][nh][Tw]: scores, then p 2^-48 as doubles
     int Tw;
     int tiles, tpc, groups, passes;   // k_tree_scores: CTAs along the positions, tiles each, groups of column blocks, blocks a group
-    int heads;                        // k_tree_softmax: heads a CTA
     int chunk, chunks, cg, cblocks, tp;   // k_tree_pv: positions a CTA, their number, groups of 8 CB columns a block, blocks, positions a tile
 };
 
@@ -512,7 +511,7 @@ __device__ __noinline__ void tree_wrapped(const TreeArgs &a, const TreeSeq &s, i
     for (int t = threadIdx.x; t < min(a.Tw, (s.len + s.n + 3) & ~3); t += blockDim.x) row[t] = 0;
 }
 
-// A CTA a node row and a.heads of its heads. The scores stay in shared memory
+// A CTA a node row and head (blockIdx.y). The scores stay in shared memory
 // (SM), longer rows in the workspace. Positions that the row does not see get a
 // score 11 below the maximum, whose exponential is 0, so that one loop serves
 // all. A row whose score differences wrap (the reference's int64 then gives other
@@ -524,8 +523,8 @@ template <bool PK, bool SM>
 __global__ void __launch_bounds__(TREE_SM_T, 10) k_tree_softmax(const __grid_constant__ TreeArgs a) {
     extern __shared__ __align__(16) char tree_smem[];
     __shared__ uint64_t red[64];
-    __shared__ int64_t wmax[2][TREE_SM_T / 32];
-    __shared__ uint64_t wsum[2][TREE_SM_T / 32];
+    __shared__ int64_t wmax[TREE_SM_T / 32];
+    __shared__ uint64_t wsum[TREE_SM_T / 32];
     __shared__ int up[TREE_MAX_NODES];
     __shared__ uint32_t anc[TREE_MAX_NODES / 32];
     const int b = blockIdx.x / a.max_nodes, node = blockIdx.x - b * a.max_nodes, tid = threadIdx.x;
@@ -550,57 +549,54 @@ __global__ void __launch_bounds__(TREE_SM_T, 10) k_tree_softmax(const __grid_con
         return j < 0 || (t < T && (anc[j >> 5] >> (j & 31) & 1));
     };
     const int end = min(a.Tw, (s.len + s.n + 3) & ~3);   // k_tree_pv reads fours up to here
-    const int h0 = blockIdx.y * a.heads, h1 = min(h0 + a.heads, a.nh);
-    for (int h = h0; h < h1; h++) {
-        const int par = h & 1;   // the other half of wmax and wsum may still be read
-        int64_t *row = a.sc + ((size_t)r * a.nh + h) * a.Tw, m = INT64_MIN;
-        int64_t *x = SM ? reinterpret_cast<int64_t *>(tree_smem) : row;   // each thread its own positions throughout
+    const int h = blockIdx.y;
+    int64_t *row = a.sc + ((size_t)r * a.nh + h) * a.Tw, m = INT64_MIN;
+    int64_t *x = SM ? reinterpret_cast<int64_t *>(tree_smem) : row;   // each thread its own positions throughout
 #pragma unroll 4
-        for (int t = tid; t < s.len; t += TREE_SM_T) {
-            const int64_t v = row[t];
-            m = max(m, v);
-            if (SM) x[t] = v;
-        }
-        const int t_end = s.len + (tid - s.len % TREE_SM_T + TREE_SM_T) % TREE_SM_T;   // its first position from the draft on
-        for (int t = t_end; t < end; t += TREE_SM_T)
-            if (sees(t)) {
-                m = max(m, row[t]);
-                if (SM) x[t] = row[t];
-            }
-        for (int k = 16; k >= 1; k >>= 1) m = max(m, (int64_t)__shfl_xor_sync(0xffffffffu, m, k));
-        if ((tid & 31) == 0) wmax[par][tid >> 5] = m;
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < TREE_SM_T / 32; k++) m = max(m, wmax[par][k]);
-        for (int t = t_end; t < end; t += TREE_SM_T)
-            if (!sees(t)) x[t] = (int64_t)((uint64_t)m - 11 * (uint64_t)IQ_ONE);
-        uint64_t sum = 0;
-        int wraps = 0;   // sign: a difference of 2^63 or more
-#pragma unroll 4
-        for (int t = tid; t < end; t += TREE_SM_T) {
-            const uint64_t d = (uint64_t)m - (uint64_t)x[t];
-            wraps |= (int)(d >> 32);
-            const int64_t e = tree_exp(d);   // (anything where d is beyond 10)
-            const int64_t v = d <= 10 * (uint64_t)IQ_ONE ? e : 0;
-            x[t] = v;
-            sum += (uint64_t)v;
-        }
-        for (int k = 16; k >= 1; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-        if ((tid & 31) == 0) wsum[par][tid >> 5] = sum;
-        int64_t *out = a.out + ((size_t)r * a.nh + h) * hd;
-        if (__syncthreads_or(wraps < 0)) {
-            tree_wrapped<PK>(a, s, r, h, T, m, row, out, red, sees);
-            continue;
-        }
-        uint64_t S = 0;
-#pragma unroll
-        for (int k = 0; k < TREE_SM_T / 32; k++) S += wsum[par][k];
-        const double inv = f64_rcp(f64_u64(S)) * (0x1p48 - 0x1p-2);
-        double *p = reinterpret_cast<double *>(row);
-#pragma unroll 4
-        for (int t = tid; t < end; t += TREE_SM_T) p[t] = tree_prob(x[t], (int64_t)S, inv);
-        for (int d = tid; d < hd; d += TREE_SM_T) out[d] = 0;   // k_tree_pv adds
+    for (int t = tid; t < s.len; t += TREE_SM_T) {
+        const int64_t v = row[t];
+        m = max(m, v);
+        if (SM) x[t] = v;
     }
+    const int t_end = s.len + (tid - s.len % TREE_SM_T + TREE_SM_T) % TREE_SM_T;   // its first position from the draft on
+    for (int t = t_end; t < end; t += TREE_SM_T)
+        if (sees(t)) {
+            m = max(m, row[t]);
+            if (SM) x[t] = row[t];
+        }
+    for (int k = 16; k >= 1; k >>= 1) m = max(m, (int64_t)__shfl_xor_sync(0xffffffffu, m, k));
+    if ((tid & 31) == 0) wmax[tid >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < TREE_SM_T / 32; k++) m = max(m, wmax[k]);
+    for (int t = t_end; t < end; t += TREE_SM_T)
+        if (!sees(t)) x[t] = (int64_t)((uint64_t)m - 11 * (uint64_t)IQ_ONE);
+    uint64_t sum = 0;
+    int wraps = 0;   // sign: a difference of 2^63 or more
+#pragma unroll 4
+    for (int t = tid; t < end; t += TREE_SM_T) {
+        const uint64_t d = (uint64_t)m - (uint64_t)x[t];
+        wraps |= (int)(d >> 32);
+        const int64_t e = tree_exp(d);   // (anything where d is beyond 10)
+        const int64_t v = d <= 10 * (uint64_t)IQ_ONE ? e : 0;
+        x[t] = v;
+        sum += (uint64_t)v;
+    }
+    for (int k = 16; k >= 1; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+    if ((tid & 31) == 0) wsum[tid >> 5] = sum;
+    int64_t *out = a.out + ((size_t)r * a.nh + h) * hd;
+    if (__syncthreads_or(wraps < 0)) {
+        tree_wrapped<PK>(a, s, r, h, T, m, row, out, red, sees);
+        return;
+    }
+    uint64_t S = 0;
+#pragma unroll
+    for (int k = 0; k < TREE_SM_T / 32; k++) S += wsum[k];
+    const double inv = f64_rcp(f64_u64(S)) * (0x1p48 - 0x1p-2);
+    double *p = reinterpret_cast<double *>(row);
+#pragma unroll 4
+    for (int t = tid; t < end; t += TREE_SM_T) p[t] = tree_prob(x[t], (int64_t)S, inv);
+    for (int d = tid; d < hd; d += TREE_SM_T) out[d] = 0;   // k_tree_pv adds
 }
 
 // ---------------------------------------------------- 3. probabilities x values
