@@ -300,7 +300,8 @@ IQ_API int iq_kv_read_dev(int64_t *d_k, int64_t *d_v, const iq_kv_cache *cache, 
  * overlap d_q. A parent that is not an earlier node counts as -1.
  * max_nodes (<= 256) and max_len (<= max_seq, <= 32767, the range of the
  * int64 softmax sum) bound n_i and d_len[i] + n_i; rows of a sequence beyond its
- * bounds, and rows outside d_start, stay as they were.
+ * bounds, and rows outside d_start, stay as they were. n_seq, rows, max_nodes and
+ * max_len are at least 1; several sequences may read the same d_seq.
  * d_work: iq_attn_tree_work bytes (16-byte aligned) that no other call uses
  * until this one has run. */
 IQ_API int iq_attn_tree_work(const iq_kv_cache *cache, int num_heads, int n_seq, int rows, int max_nodes, int max_len,

@@ -389,6 +389,17 @@ def _cur(stream):
     return getattr(stream, "cuda_stream", stream)
 
 
+def _ref(x):
+    """x (a Rope or KVCache) by reference, after checking that its tensors lie where calls go to."""
+    if x.dev is not None and x.dev != _raw_device():
+        raise ValueError(f"{type(x).__name__} of device {x.dev}, calls go to device {_raw_device()}")
+    return ctypes.byref(x)
+
+
+def _dev_of(*tensors):
+    return next((t.get_device() for t in tensors if t is not None), None)
+
+
 ROPE_LAYOUT = dict(half=0, interleaved=1)
 ROPE_SCALE = dict(none=0, linear=1, ntk=2, parts=3)
 
@@ -416,11 +427,12 @@ class Rope(ctypes.Structure):
         super().__init__(_dev_ptr(cos, 8, "cos"), _dev_ptr(sin, 8, "sin"), _dev_ptr(pos, 4, "pos"), n_pos, rot_dim,
                          ROPE_LAYOUT[layout])
         self.keep = (cos, sin, pos)
+        self.dev = _dev_of(*self.keep)
 
 
 def rope_dev(out, x, rope, rows, heads, head_dim, x_stride=None, out_stride=None, stream=None):
     w = heads * head_dim
-    _call("iq_rope_dev", _dev_ptr(out, 8, "out"), _dev_ptr(x, 8, "x"), ctypes.byref(rope), rows, heads, head_dim,
+    _call("iq_rope_dev", _dev_ptr(out, 8, "out"), _dev_ptr(x, 8, "x"), _ref(rope), rows, heads, head_dim,
           w if x_stride is None else x_stride, w if out_stride is None else out_stride, _cur(stream))
 
 
@@ -435,17 +447,18 @@ class KVCache(ctypes.Structure):
                          _dev_ptr(kq, 1, "kq"), _dev_ptr(vq, 2, "vq"), _dev_ptr(k_mag, 8, "k_mag"),
                          _dev_ptr(v_mag, 8, "v_mag"))
         self.keep = (k, v, kq, vq, k_mag, v_mag)
+        self.dev = _dev_of(*self.keep)
 
 
 def kv_write_dev(cache, k, v, slot, rows, seq=None, rope=None, k_stride=None, v_stride=None, stream=None):
     w = cache.kv_heads * cache.head_dim
-    _call("iq_kv_write_dev", ctypes.byref(cache), _dev_ptr(k, 8, "k"), _dev_ptr(v, 8, "v"), _dev_ptr(seq, 4, "seq"),
+    _call("iq_kv_write_dev", _ref(cache), _dev_ptr(k, 8, "k"), _dev_ptr(v, 8, "v"), _dev_ptr(seq, 4, "seq"),
           _dev_ptr(slot, 4, "slot"), rows, w if k_stride is None else k_stride, w if v_stride is None else v_stride,
-          ctypes.byref(rope) if rope is not None else None, _cur(stream))
+          None if rope is None else _ref(rope), _cur(stream))
 
 
 def kv_read_dev(k, v, cache, slot, rows, seq=None, stream=None):
-    _call("iq_kv_read_dev", _dev_ptr(k, 8, "k"), _dev_ptr(v, 8, "v"), ctypes.byref(cache), _dev_ptr(seq, 4, "seq"),
+    _call("iq_kv_read_dev", _dev_ptr(k, 8, "k"), _dev_ptr(v, 8, "v"), _ref(cache), _dev_ptr(seq, 4, "seq"),
           _dev_ptr(slot, 4, "slot"), rows, _cur(stream))
 
 
@@ -460,7 +473,7 @@ def attn_tree_dev(out, q, cache, num_heads, lens, starts, parents, n_seq, rows, 
                   seqs=None, q_stride=None, stream=None):
     """Tree attention; work: a device tensor of at least attn_tree_work(...) bytes."""
     nbytes = 0 if work is None else work.numel() * work.element_size()
-    _call("iq_attn_tree_dev", _dev_ptr(out, 8, "out"), _dev_ptr(q, 8, "q"), ctypes.byref(cache), num_heads,
+    _call("iq_attn_tree_dev", _dev_ptr(out, 8, "out"), _dev_ptr(q, 8, "q"), _ref(cache), num_heads,
           _dev_ptr(seqs, 4, "seqs"), _dev_ptr(lens, 4, "lens"), _dev_ptr(starts, 4, "starts"),
           _dev_ptr(parents, 4, "parents"), n_seq, rows, max_nodes, max_len,
           num_heads * cache.head_dim if q_stride is None else q_stride,

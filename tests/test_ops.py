@@ -137,6 +137,16 @@ def test_binding_refuses_host_and_wrong_types():
         iq.logprobs_dev(x.int(), 1, 4)
 
 
+def test_binding_refuses_a_cache_of_another_device(monkeypatch):
+    cache, rope = iq.KVCache(1, 1, 1, 4), iq.Rope(None, None, None, 1, 2)
+    monkeypatch.setattr(iq, "_raw_device", lambda: 1)
+    cache.dev = rope.dev = 0
+    with pytest.raises(ValueError, match="device 0"):
+        iq.kv_read_dev(None, None, cache, None, 1)
+    with pytest.raises(ValueError, match="device 0"):
+        iq.rope_dev(None, None, rope, 1, 1, 4)
+
+
 # ------------------------------------------------------------- identities
 
 def test_reference_tables_equal_rope_init():
@@ -192,3 +202,39 @@ def test_exp_down_and_ln_accuracy():
         s = rng.randrange(ONE, 1 << rng.randint(49, 68))
         assert abs(ref.ln_sum(s) / ONE - math.log(s / ONE)) < 2.0 ** -46
     assert ref.ln_sum(ONE) == 0
+
+
+def test_lowered_reciprocals_give_the_quotient_or_one_less():
+    # floor(2^96 / r) from a reciprocal off by at most 2^-51, lowered by 2^-50: the floor is q or
+    # q - 1, and the sign of (floor + 1) r - 2^96 - 1 in 64 bits tells which
+    rng = random.Random(11)
+    top = int(2 ** 62.5)
+    rs = [1 << 48, (1 << 48) + 1, (1 << 62), top] + [rng.randrange(1 << 48, top) for _ in range(2000)]
+    for r in rs:
+        q = (1 << 96) // r
+        for err in (Fraction(-1, 1 << 51), Fraction(0), Fraction(1, 1 << 51)):
+            f = math.floor(Fraction(1, r) * (1 + err) * ((1 << 96) - (1 << 46)))
+            assert f in (q - 1, q)
+            sign = (((f + 1) * r - (1 << 96) - 1) % (1 << 64)) >> 63
+            assert f + sign == q
+
+
+def test_score_from_shifted_bytes():
+    # q.k >> 48 (mod 2^64) from unsigned bytes of x + 2^63: diagonals i + j <= 13 and the sums of q and k
+    rng = random.Random(12)
+    for hd in (1, 7, 64):
+        for _ in range(20):
+            q = [rng.choice([rng.getrandbits(64) - (1 << 63), -(1 << 63), (1 << 63) - 1, 0]) for _ in range(hd)]
+            k = [rng.choice([rng.getrandbits(64) - (1 << 63), -(1 << 63), (1 << 63) - 1, -1]) for _ in range(hd)]
+            diag = [0] * 14
+            for a, b in zip(q, k):
+                a, b = a + (1 << 63), b + (1 << 63)
+                for i in range(8):
+                    for j in range(min(8, 14 - i)):
+                        diag[i + j] += (a >> 8 * j & 255) * (b >> 8 * i & 255)
+            assert max(diag) < 1 << 28
+            low = 0
+            for v in diag[:6]:
+                low = (low >> 8) + v   # floors of floors
+            dot = (low >> 8) + sum(v << 8 * (s - 6) for s, v in enumerate(diag) if s >= 6) - ((sum(q) + sum(k)) << 15)
+            assert dot % (1 << 64) == (sum(a * b for a, b in zip(q, k)) >> 48) % (1 << 64)
