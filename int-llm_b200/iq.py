@@ -371,11 +371,12 @@ def _dev_ptr(t, itemsize, name):
         return None
     if t.element_size() != itemsize:
         raise ValueError(f"{name}: {itemsize}-byte elements expected, got {t.element_size()}")
-    if not t.is_cuda:
+    dev = t.get_device()
+    if dev < 0:
         raise ValueError(f"{name} must be in device memory, got {t.device}")
     if _raw_device is None:
         _bind_torch()
-    if t.get_device() != _raw_device():
+    if dev != _raw_device():
         raise ValueError(f"{name} lies on {t.device}, calls go to device {_raw_device()}")
     return t.data_ptr()
 
@@ -394,10 +395,6 @@ def _ref(x):
     if x.dev is not None and x.dev != _raw_device():
         raise ValueError(f"{type(x).__name__} of device {x.dev}, calls go to device {_raw_device()}")
     return ctypes.byref(x)
-
-
-def _dev_of(*tensors):
-    return next((t.get_device() for t in tensors if t is not None), None)
 
 
 ROPE_LAYOUT = dict(half=0, interleaved=1)
@@ -427,7 +424,7 @@ class Rope(ctypes.Structure):
         super().__init__(_dev_ptr(cos, 8, "cos"), _dev_ptr(sin, 8, "sin"), _dev_ptr(pos, 4, "pos"), n_pos, rot_dim,
                          ROPE_LAYOUT[layout])
         self.keep = (cos, sin, pos)
-        self.dev = _dev_of(*self.keep)
+        self.dev = None if cos is None else cos.get_device()
 
 
 def rope_dev(out, x, rope, rows, heads, head_dim, x_stride=None, out_stride=None, stream=None):
@@ -447,7 +444,8 @@ class KVCache(ctypes.Structure):
                          _dev_ptr(kq, 1, "kq"), _dev_ptr(vq, 2, "vq"), _dev_ptr(k_mag, 8, "k_mag"),
                          _dev_ptr(v_mag, 8, "v_mag"))
         self.keep = (k, v, kq, vq, k_mag, v_mag)
-        self.dev = _dev_of(*self.keep)
+        t = kq if k is None else k
+        self.dev = None if t is None else t.get_device()
 
 
 def kv_write_dev(cache, k, v, slot, rows, seq=None, rope=None, k_stride=None, v_stride=None, stream=None):
