@@ -734,3 +734,67 @@ def test_wide_and_narrow_forms_agree():
         iq.rope_dev(b[1:], dev(x), r, rows, heads, hd)
         want = ref.rotate(x.reshape(rows, heads, hd), cos[pos], sin[pos], rot, layout).reshape(rows, -1)
         assert (a.cpu().numpy() == want).all() and (b[1:].cpu().numpy().reshape(rows, -1) == want).all()
+
+
+@pytest.mark.parametrize("nh,nkv,hd,n", [(16, 1, 128, 8), (16, 1, 96, 9), (24, 1, 64, 11), (32, 2, 32, 20), (12, 1, 120, 12)])
+@pytest.mark.parametrize("kvb", [(0, 0), (8, 10)])
+def test_tree_columns_that_share_values(nh, nkv, hd, n, kvb):
+    """Enough columns a sequence that groups of them share a tile of values, ragged at the last group."""
+    rng = np.random.default_rng(hd + n)
+    check_tree(rng, nh, nkv, hd, [90, 33], [bush(rng, n), bush(rng, n - 3)], kvb, pad=5)
+
+
+@pytest.mark.parametrize("kvb", [(0, 0), (8, 10)])
+def test_cache_offsets_beyond_32_bits(kvb):
+    """The last sequence of a cache whose element offsets (exact: byte offsets too) pass 32 bits."""
+    rng = np.random.default_rng(23)
+    kb, vb = kvb
+    nkv, hd, M, nh, n, ln = 2, 256, 32767, 4, 3, 200
+    S = (1 << (32 if kb else 31)) // (M * nkv * hd) + 2
+    make = lambda dt, *tail: torch.empty((S, M, nkv) + tail, dtype=dt, device="cuda")
+    t = (dict(kq=make(torch.uint8, hd), vq=make(torch.int16, hd), k_mag=make(torch.int64), v_mag=make(torch.int64))
+         if kb else dict(k=make(torch.int64, hd), v=make(torch.int64, hd)))
+    small, ts = new_cache(1, M, nkv, hd, kb, vb)
+    big = iq.KVCache(S, M, nkv, hd, k_bits=kb, v_bits=vb, **t)
+    rows = ln + n
+    k, v = dev(rnd(rng, rows, nkv * hd)), dev(rnd(rng, rows, nkv * hd))
+    slot = np.arange(rows)
+    slot[-1] = M - 1                                  # the last vector of the cache
+    iq.kv_write_dev(big, k, v, i32(slot), rows, seq=i32([S - 1] * rows))
+    iq.kv_write_dev(small, k, v, i32(slot), rows)
+    at = torch.from_numpy(slot).cuda()
+    for name in t:
+        assert (t[name][S - 1][at] == ts[name][0][at]).all()
+    got, want = [full(rows, nkv * hd) for _ in range(2)], [full(rows, nkv * hd) for _ in range(2)]
+    iq.kv_read_dev(*got, big, i32(slot), rows, seq=i32([S - 1] * rows))
+    iq.kv_read_dev(*want, small, i32(slot), rows)
+    assert all((a == b).all() for a, b in zip(got, want))
+    q = dev(rnd(rng, 2, nh * hd, scale=1.5))
+    args = (kvb, [ln], [0, 2], [-1, 0], nh)
+    assert (run_tree(q, t, *args, seqs=[S - 1]) == run_tree(q, ts, *args)).all()
+
+
+def test_strides_beyond_32_bits():
+    """Rows of queries, of a rotation and of logits more than 2^32 elements apart."""
+    rng = np.random.default_rng(24)
+    nh, hd, V, st = 4, 64, 500, (1 << 32) + 2
+    big = torch.empty(st + V, dtype=torch.int64, device="cuda")
+    x = rnd(rng, 2, V, scale=2)
+    for r in range(2):
+        big[r * st:r * st + V].copy_(dev(x[r]))
+    ids, tl, lp = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), full(2, 3), full(2)
+    ids1, tl1, lp1 = ids.clone(), tl.clone(), lp.clone()
+    iq.logprobs_dev(big, 2, V, i32([3, 499]), lp, None, 3, ids, tl, ld=st)
+    iq.logprobs_dev(dev(x), 2, V, i32([3, 499]), lp1, None, 3, ids1, tl1)
+    assert (ids == ids1).all() and (tl == tl1).all() and (lp == lp1).all()
+    _, t = new_cache(1, 40, 2, hd, 0, 0)
+    t["k"].copy_(dev(rnd(rng, 1, 40, 2, hd)))
+    t["v"].copy_(dev(rnd(rng, 1, 40, 2, hd)))
+    q = dev(np.ascontiguousarray(x[:, :nh * hd]))
+    args = (t, (0, 0), [30], [0, 2], [-1, 0], nh)
+    assert (run_tree(big, *args, q_stride=st, rows=2) == run_tree(q, *args)).all()
+    cos, sin = dev(rnd(rng, 5, hd // 2)), dev(rnd(rng, 5, hd // 2))
+    rope, want = iq.Rope(cos, sin, i32([4, 2]), 5, hd), full(2, nh * hd)
+    iq.rope_dev(want, q, rope, 2, nh, hd)
+    iq.rope_dev(big, big, rope, 2, nh, hd, x_stride=st, out_stride=st)
+    assert all((big[r * st:r * st + nh * hd] == want[r]).all() for r in range(2))
