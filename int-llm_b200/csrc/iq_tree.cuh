@@ -64,7 +64,7 @@ __device__ __forceinline__ bool tree_seq(const TreeArgs &a, int b, TreeSeq &s) {
     if (s.n == 0) return false;
     const bool ok = s.sq >= 0 && s.sq < a.c.seqs && s.row0 >= 0 && s.n > 0 && s.n <= a.max_nodes &&
                     s.row0 <= a.rows - s.n && s.len >= 0 && s.len <= a.max_len - s.n;
-    if (!ok && s.sq != -1) atomicExch(&g_iq_err, (int)IQ_ERR_RANGE);
+    if (!ok && s.sq >= 0) atomicExch(&g_iq_err, (int)IQ_ERR_RANGE);
     return ok;
 }
 

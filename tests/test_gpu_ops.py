@@ -798,3 +798,13 @@ def test_strides_beyond_32_bits():
     iq.rope_dev(want, q, rope, 2, nh, hd)
     iq.rope_dev(big, big, rope, 2, nh, hd, x_stride=st, out_stride=st)
     assert all((big[r * st:r * st + nh * hd] == want[r]).all() for r in range(2))
+
+
+@pytest.mark.parametrize("sq", [-1, -7, -(1 << 31)])
+def test_tree_negative_cache_sequence_is_padding(sq):
+    """Any negative sequence index leaves its rows as they were, silently, as the other operators' do."""
+    rng = np.random.default_rng(25)
+    t = dict(k=dev(rnd(rng, 1, 8, 1, 16)), v=dev(rnd(rng, 1, 8, 1, 16)))
+    q = dev(rnd(rng, 2, 32))
+    got = run_tree(q, t, (0, 0), [3, 4], [0, 1, 2], [-1, -1], 2, seqs=[0, sq])
+    assert (got[1] == KEEP).all() and (got[0] == run_tree(q[:1], t, (0, 0), [3], [0, 1], [-1], 2)[0]).all()
