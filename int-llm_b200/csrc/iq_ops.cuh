@@ -295,7 +295,7 @@ struct KVArgs {
 // NJ items of four elements: rotate, take the magnitude, write the codes. One item a
 // lane up to 128-wide heads (2048 rows of 32 heads of 128 written as codes: 82 us,
 // issue-bound at 68 %, two products a rotated element and an exact quotient; two items a
-// lane 103 us, the narrow form 123).
+// lane and a divided reciprocal 103 us, the narrow form 123).
 template <bool PACKED, int NJ>
 __global__ void __launch_bounds__(256)
 k_kv_write_wide(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restrict__ v, const int *__restrict__ seq,
