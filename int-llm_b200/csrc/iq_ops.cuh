@@ -144,9 +144,11 @@ __device__ __forceinline__ RopeItem rope_item(const RopeArgs &r, int q) {
     else { it.ea = 4 * q; it.eb = 4 * q + 2; }
     return it;
 }
-// fp_mul for |x| < 2^60 and |c| < 2^49: with both halves signed, x = xh 2^32 + xl and
+// fp_mul for |x| < 2^59 and |c| < 2^49: with both halves signed, x = xh 2^32 + xl and
 // c = ch 2^32 + cl, every product is one wide multiply-add:
-// floor(x c / 2^48) = 4 xh 2^14 ch + floor((xh cl + xl ch + floor(xl cl / 2^32)) / 2^16).
+// floor(x c / 2^48) = 8 xh 2^13 ch + floor((xh cl + xl ch + floor(xl cl / 2^32)) / 2^16).
+// A negative low half carries into the high one, so |xh| <= 2^27 and |ch| <= 2^17 with
+// both ends: 8 xh and 2^13 ch stay within 2^30.
 struct Half { int h, l; };
 __device__ __forceinline__ Half halves(int64_t x) {
     const int l = (int)(uint32_t)x;
@@ -157,7 +159,7 @@ __device__ __forceinline__ int64_t mul_small(const Half &x, const Half &c) {
     madw(t, x.h, c.l);
     madw(t, x.l, c.h);
     t >>= 16;
-    madw(t, x.h * 4, c.h * (1 << 14));
+    madw(t, x.h * 8, c.h * (1 << 13));
     return t;
 }
 __device__ __forceinline__ void turn_small(int64_t &a, int64_t &b, int64_t c, int64_t s) {
@@ -172,7 +174,7 @@ __device__ __forceinline__ uint32_t beyond(int64_t x, int k) { return ((uint32_t
 __device__ __forceinline__ void rope_turn4(const RopeArgs &r, longlong2 &a, longlong2 &b, const longlong2 &c, const longlong2 &s) {
     int64_t v[4] = {a.x, a.y, b.x, b.y};
     if (r.layout == IQ_ROPE_HALF) { v[1] = b.x; v[2] = a.y; }   // pairs (0, 1), (2, 3)
-    if ((beyond(a.x, 28) | beyond(a.y, 28) | beyond(b.x, 28) | beyond(b.y, 28) | beyond(c.x, 17) | beyond(c.y, 17) |
+    if ((beyond(a.x, 27) | beyond(a.y, 27) | beyond(b.x, 27) | beyond(b.y, 27) | beyond(c.x, 17) | beyond(c.y, 17) |
          beyond(s.x, 17) | beyond(s.y, 17)) == 0) {
         turn_small(v[0], v[1], c.x, s.x);
         turn_small(v[2], v[3], c.y, s.y);

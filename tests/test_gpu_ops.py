@@ -808,3 +808,59 @@ def test_tree_negative_cache_sequence_is_padding(sq):
     q = dev(rnd(rng, 2, 32))
     got = run_tree(q, t, (0, 0), [3, 4], [0, 1, 2], [-1, -1], 2, seqs=[0, sq])
     assert (got[1] == KEEP).all() and (got[0] == run_tree(q[:1], t, (0, 0), [3], [0, 1], [-1], 2)[0]).all()
+
+
+# table values up to 2.0, where the halves of the fast products are largest; -2.0 and beyond are the general form's
+NEAR_TWO = [2 * ONE - 1, 2 * ONE - (1 << 31), 2 * ONE - (1 << 31) - 1, 2 * ONE - (1 << 31) + 1, 2 * ONE - (1 << 32),
+            -2 * ONE + 1, -2 * ONE + (1 << 31), -2 * ONE + (1 << 31) - 1, -2 * ONE, 2 * ONE, ONE + 11, 0]
+NEAR_X = [1 << 59, (1 << 59) - 1, (1 << 59) - (1 << 31), -(1 << 59), -(1 << 59) - 1, -(1 << 59) + 1, (1 << 60) - 1,
+          -(1 << 60), 1 << 60, (1 << 31) - 1, -(1 << 31), 3 * ONE]
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("where", ["cos", "sin", "both"])
+def test_rotation_by_table_values_near_two(layout, where):
+    """Each value alone among ordinary ones, as either pair of its 16-byte piece, in the rotation and in written keys."""
+    rng = np.random.default_rng(26)
+    heads, hd, half = 2, 64, 32
+    rows = n = 2 * len(NEAR_TWO)
+    cos, sin = rnd(rng, n, half, scale=0.3), rnd(rng, n, half, scale=0.3)
+    for i, c in enumerate(NEAR_TWO * 2):                  # position i: value i, in the first or the second pair
+        at = slice(i // len(NEAR_TWO), None, 4)
+        if where != "sin":
+            cos[i, at] = c
+        if where != "cos":
+            sin[i, at] = c
+    x = rnd(rng, rows, heads, hd, scale=3)
+    x[:, 0, :12] = NEAR_X
+    x[:, 0, 32:44] = NEAR_X[::-1]
+    pos = rng.permutation(n)
+    r = iq.Rope(dev(cos), dev(sin), i32(pos), n, hd, layout)
+    want = ref.rotate(x, cos[pos], sin[pos], hd, layout)
+    out = full(rows, heads * hd)
+    iq.rope_dev(out, dev(x), r, rows, heads, hd)
+    assert (out.cpu().numpy().reshape(want.shape) == want).all()
+    for kb, vb in ((0, 0), (8, 10)):
+        c, t = new_cache(1, rows, heads, hd, kb, vb)
+        h = host_cache(t)
+        iq.kv_write_dev(c, dev(x), dev(x), i32(range(rows)), rows, rope=r)
+        write_ref(h, want, x, [0] * rows, range(rows), kb, vb)
+        got = host_cache(t)
+        for name in h:
+            assert (got[name] == h[name]).all(), name
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("mscale", [2 * ONE, 2 * ONE - 1, 1024 * ONE])
+def test_rotation_by_scaled_tables(mscale, layout):
+    """Tables with a large factor on cos and sin, then rows rotated by them."""
+    rng = np.random.default_rng(27)
+    n, heads, hd = 4096, 2, 64
+    cos, sin = full(n, hd // 2), full(n, hd // 2)
+    iq.rope_tables_dev(cos, sin, hd, n, 10000, dict(mscale=mscale))
+    pos = np.r_[0:24, rng.integers(0, n, 200)]
+    c, s = ref.tables(hd, pos.tolist(), 10000, mscale=mscale)
+    assert (cos[dev(pos)].cpu().numpy() == c).all() and (sin[dev(pos)].cpu().numpy() == s).all()
+    x, out = rnd(rng, len(pos), heads, hd, scale=3), full(len(pos), heads * hd)
+    iq.rope_dev(out, dev(x), iq.Rope(cos, sin, i32(pos), n, hd, layout), len(pos), heads, hd)
+    assert (out.cpu().numpy().reshape(x.shape) == ref.rotate(x, c, s, hd, layout)).all()

@@ -238,3 +238,27 @@ def test_score_from_shifted_bytes():
                 low = (low >> 8) + v   # floors of floors
             dot = (low >> 8) + sum(v << 8 * (s - 6) for s, v in enumerate(diag) if s >= 6) - ((sum(q) + sum(k)) << 15)
             assert dot % (1 << 64) == (sum(a * b for a, b in zip(q, k)) >> 48) % (1 << 64)
+
+
+def test_products_of_signed_halves():
+    """mul_small: floor(x c / 2^48) for |x| < 2^59 and |c| < 2^49 from 32-bit halves, no intermediate beyond its type."""
+    def fits(v, bits):
+        assert -(1 << bits - 1) <= v < 1 << bits - 1
+        return v
+
+    def halves(x):
+        low = (x & 0xffffffff) - ((x & 0x80000000) << 1)
+        return fits((x >> 32) + (low < 0), 32), low
+
+    rng = random.Random(13)
+    X, C = 1 << 59, 1 << 49
+    ends = lambda m: [m - 1, m - (1 << 31), m - (1 << 31) - 1, -m, -m + 1, -m + (1 << 31), 0, -1, 1 << 31]  # noqa: E731
+    xs = ends(X) + [rng.randrange(-X, X) for _ in range(400)]
+    cs = ends(C) + [ONE + 11, -ONE] + [rng.randrange(-C, C) for _ in range(100)]
+    for x in xs:
+        xh, xl = halves(x)
+        for c in cs:
+            ch, cl = halves(c)
+            t = fits((xl * cl >> 32) + xh * cl, 64)
+            t = fits(t + xl * ch, 64) >> 16
+            assert fits(t + fits(8 * xh, 32) * fits(ch << 13, 32), 64) == x * c >> 48
