@@ -256,7 +256,7 @@ __device__ __forceinline__ KVMag kv_mag(int64_t M, int bits) {
     m.top = (1 << bits) - 1;
     return m;
 }
-__device__ __forceinline__ int kv_code(int64_t x, const KVMag &m) {   // M < 2^61
+__device__ __forceinline__ int kv_code(int64_t x, const KVMag &m) {   // |x| <= M < 2^61
     const uint64_t u = (uint64_t)(x + m.M);   // u <= D
     // the floored quotient in the binade of 2^52
     const uint32_t q = (uint32_t)__double_as_longlong(__fma_rd(f64_u64(u), m.inv, 4503599627370496.0));
@@ -266,8 +266,9 @@ __device__ __forceinline__ int kv_code(int64_t x, const KVMag &m) {   // M < 2^6
     const uint32_t h = (uint32_t)(t >> 32) + q * (uint32_t)(m.D >> 32);
     return min((int)(q + (h >> 31)), m.top);
 }
-// the same for any M, as the reference's int64 wraps
+// the same for any x and M, as the reference's int64 wraps
 __device__ __noinline__ int kv_code_any(int64_t x, int64_t M, int bits) {
+    if (M == 0) return 0;
     const int64_t top = ((int64_t)1 << bits) - 1;
     const i128 num = (i128)(int64_t)((uint64_t)x + (uint64_t)M) * ((i128)1 << bits);
     i128 t = d_sdiv128_64(num, (int64_t)((uint64_t)M * 2));
@@ -275,6 +276,16 @@ __device__ __noinline__ int kv_code_any(int64_t x, int64_t M, int bits) {
     if (t > top) t = top;
     return (int)t;
 }
+
+// The magnitude of x as the reference takes it: |INT64_MIN| wraps to itself, below every
+// other, so that an element can lie below -M. `hi` gathers the high words, for kv_fits.
+__device__ __forceinline__ int64_t kv_abs(int64_t x, uint32_t &hi) {
+    const int64_t a = x < 0 ? (int64_t)(0 - (uint64_t)x) : x;
+    hi |= (uint32_t)(a >> 32);
+    return a;
+}
+// whether the elements of which kv_abs gathered hi, of a vector of magnitude M, may take kv_code
+__device__ __forceinline__ bool kv_fits(uint32_t hi, int64_t M) { return M < (1ll << 61) && (int)hi >= 0; }
 
 // ((2q + 1) M >> b) - M (kv_unpack_vector, llama_int.c:1226-1235) from 32-bit halves of M:
 // c M = c Mh 2^32 + c Ml with c < 2^17, and 2^32 is a multiple of 2^b.
@@ -333,22 +344,25 @@ k_kv_write_wide(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restri
         }
     }
     int64_t M = 0;
+    uint32_t hi = 0;
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
         const int q = lane + j * L;
         if (live && q < np && 4 * q < r.rot) rope_turn4(r, a[j], b[j], __ldg(cs + q), __ldg(sn + q));
-        if (PACKED) {   // |INT64_MIN| wraps to itself, below every magnitude, as in the reference
+        if (PACKED) {
             const int64_t w[4] = {a[j].x, a[j].y, b[j].x, b[j].y};
 #pragma unroll
-            for (int i = 0; i < 4; i++) M = max(M, w[i] < 0 ? (int64_t)(0 - (uint64_t)w[i]) : w[i]);
+            for (int i = 0; i < 4; i++) M = max(M, kv_abs(w[i], hi));
         }
     }
     const int bits = which ? c.vbits : c.kbits;
     KVMag km = {};
+    bool fits = true;
     if (PACKED) {
         for (int m = L >> 1; m >= 1; m >>= 1) M = max(M, (int64_t)__shfl_xor_sync(0xffffffffu, M, m));
         if (live && lane == 0) (which ? c.vmag : c.kmag)[vec] = M;
         km = kv_mag(M, bits);
+        fits = kv_fits(hi, M);
     }
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
@@ -357,7 +371,7 @@ k_kv_write_wide(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restri
         const RopeItem it = rope_item(r, q);
         if (PACKED) {
             int c0, c1, c2, c3;
-            if (M < (1ll << 61)) {
+            if (fits) {
                 c0 = kv_code(a[j].x, km);
                 c1 = kv_code(a[j].y, km);
                 c2 = kv_code(b[j].x, km);
@@ -408,6 +422,7 @@ k_kv_write(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restrict__ 
     const int64_t *cs = rr.rot ? r.cos + (size_t)pos * half : nullptr, *sn = rr.rot ? r.sin + (size_t)pos * half : nullptr;
     const size_t vec = ((size_t)sq * c.max_seq + t) * c.nkv + h, e0v = vec * c.hd;
     int64_t a[4], b[4], M = 0;
+    uint32_t hi = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const int p = lane + 32 * j;
@@ -418,18 +433,19 @@ k_kv_write(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restrict__ 
         a[j] = src[e0];
         if (e1 < c.hd) b[j] = src[e1];
         if (p < half) rope_turn(a[j], b[j], cs[p], sn[p]);
-        if (PACKED) {   // |INT64_MIN| wraps to itself, below every magnitude, as in the reference
-            const int64_t ma = a[j] < 0 ? (int64_t)(0 - (uint64_t)a[j]) : a[j];
-            const int64_t mb = b[j] < 0 ? (int64_t)(0 - (uint64_t)b[j]) : b[j];
-            M = max(M, max(ma, mb));
+        if (PACKED) {
+            M = max(M, kv_abs(a[j], hi));
+            M = max(M, kv_abs(b[j], hi));
         }
     }
     KVMag km = {};
+    bool fits = true;
     const int bits = which ? c.vbits : c.kbits;
     if (PACKED) {
         for (int m = 16; m >= 1; m >>= 1) M = max(M, (int64_t)__shfl_xor_sync(0xffffffffu, M, m));
         if (lane == 0) (which ? c.vmag : c.kmag)[vec] = M;
         km = kv_mag(M, bits);
+        fits = kv_fits(hi, M);
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -438,8 +454,8 @@ k_kv_write(KVArgs c, const int64_t *__restrict__ k, const int64_t *__restrict__ 
         int e0, e1;
         rope_pair(rr, p, e0, e1);
         if (PACKED) {
-            const int q0 = M < (1ll << 61) ? kv_code(a[j], km) : kv_code_any(a[j], M, bits);
-            const int q1 = M < (1ll << 61) ? kv_code(b[j], km) : kv_code_any(b[j], M, bits);
+            const int q0 = fits ? kv_code(a[j], km) : kv_code_any(a[j], M, bits);
+            const int q1 = fits ? kv_code(b[j], km) : kv_code_any(b[j], M, bits);
             if (which) {
                 c.vq[e0v + e0] = (uint16_t)q0;
                 if (e1 < c.hd) c.vq[e0v + e1] = (uint16_t)q1;

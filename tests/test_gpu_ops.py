@@ -864,3 +864,31 @@ def test_rotation_by_scaled_tables(mscale, layout):
     x, out = rnd(rng, len(pos), heads, hd, scale=3), full(len(pos), heads * hd)
     iq.rope_dev(out, dev(x), iq.Rope(cos, sin, i32(pos), n, hd, layout), len(pos), heads, hd)
     assert (out.cpu().numpy().reshape(x.shape) == ref.rotate(x, c, s, hd, layout)).all()
+
+
+@pytest.mark.parametrize("kb,vb", [(8, 10), (1, 1), (4, 16)])
+@pytest.mark.parametrize("hd", [64, 256, 33])
+def test_codes_of_the_lowest_value(hd, kb, vb):
+    """INT64_MIN wraps below every magnitude: code 0 beside small elements, zeros and large ones, as K and as V, in
+    16-byte pieces and element by element."""
+    rng = np.random.default_rng(hd + kb)
+    mags = [0, 1, 5, ONE, 3 * ONE, (1 << 61) - 1, 1 << 61, (1 << 62) - 1, ref.I64_MAX]
+    rows, nkv = 2 * len(mags), 2
+    x = np.zeros((rows, nkv, hd), np.int64)
+    for i, m in enumerate(mags):
+        x[2 * i:2 * i + 2] = rng.integers(-m, m, (2, nkv, hd), endpoint=True)
+        x[2 * i:2 * i + 2, :, 0] = m
+    for r in range(rows):                         # one in each lane's place in turn, and a few in one vector
+        x[r, 0, 1 + 7 * r % (hd - 1)] = ref.I64_MIN
+        x[r, 1, 1::5] = ref.I64_MIN
+    for skip in (0, 1):
+        buf = torch.empty(x.size + 1, dtype=torch.int64, device="cuda")
+        d = buf[skip:x.size + skip]               # 16-byte aligned, and 8-byte aligned only
+        d.copy_(dev(x).flatten())
+        c, t = new_cache(1, rows, nkv, hd, kb, vb)
+        h = host_cache(t)
+        iq.kv_write_dev(c, d, d, i32(range(rows)), rows)
+        write_ref(h, x, x, [0] * rows, range(rows), kb, vb)
+        got = host_cache(t)
+        for name in h:
+            assert (got[name] == h[name]).all(), name

@@ -262,3 +262,27 @@ def test_products_of_signed_halves():
             t = fits((xl * cl >> 32) + xh * cl, 64)
             t = fits(t + xl * ch, 64) >> 16
             assert fits(t + fits(8 * xh, 32) * fits(ch << 13, 32), 64) == x * c >> 48
+
+
+def test_code_from_a_lowered_quotient():
+    """kv_code: the estimate u inv rounded down, inv lowered by 2^-50, is q or q - 1 whichever way each rounding before
+    it goes, and the sign of (q + 1) D - u 2^b - 1 in 64 bits tells which; an element whose magnitude wraps
+    (INT64_MIN) is the one that x + M leaves negative, and its code is 0."""
+    rng = random.Random(14)
+    half = Fraction(1, 1 << 53)
+    for _ in range(1500):
+        M = rng.choice([rng.randrange(1, 1 << 61), rng.randrange(1, 1 << 20), (1 << 61) - 1, 1, 2, ONE])
+        x = rng.choice([rng.randint(-M, M), M, -M, 0, M - 1, 1 - M])
+        b = rng.choice([1, 4, 8, 16])
+        u, D = x + M, 2 * M
+        q = (u << b) // D
+        for e in (-1, 1):
+            # D as a double, its reciprocal, the scaled reciprocal and u as a double, each off by its bound
+            inv = Fraction(1, D) / (1 + e * half) * (1 + Fraction(e, 1 << 51)) * (1 << b) * (1 - Fraction(1, 1 << 50))
+            f = math.floor(u * (1 + e * half) * inv * (1 + e * half))
+            assert f in (q - 1, q) or (u == 0 and f == 0)
+            sign = ((f + 1) * D - (u << b) - 1) % (1 << 64) >> 63
+            assert f + sign == q
+    for M in (0, 1, ONE, (1 << 61) - 1):
+        assert ref.pack([M, ref.I64_MIN, -M], 8) == ([255 if M else 0, 0, 0], M)
+        assert ref.wrap(ref.I64_MIN + M) < 0 <= min(-M + M, M + M)
