@@ -126,8 +126,9 @@ static void tree_plan(TreeArgs *a) {
     const int64_t cols = (int64_t)std::min(a->max_nodes, a->rows) * grp;
     // the row stride keeps every row 16-byte aligned
     a->Tw = (a->max_len + 3) / 4 * 4;
-    // columns of all sequences, on average over them
-    const int64_t avg = std::max<int64_t>(1, (int64_t)a->rows * grp / a->n_seq);
+    // columns of all sequences, on average over them (rows outside the sequences may be many,
+    // a sequence has no more than cols)
+    const int64_t avg = std::min(cols, std::max<int64_t>(1, (int64_t)a->rows * grp / a->n_seq));
     // 8 columns a block for single tokens of up to 8 heads a kv head (64 of them at 2000
     // positions: 175 us, with half-empty blocks of 16: 190 us)
     const int nt = cols <= 8 ? 1 : 2, blocks = (int)((cols + 8 * nt - 1) / (8 * nt));

@@ -892,3 +892,25 @@ def test_codes_of_the_lowest_value(hd, kb, vb):
         got = host_cache(t)
         for name in h:
             assert (got[name] == h[name]).all(), name
+
+
+@pytest.mark.parametrize("kvb", [(0, 0), (8, 10)])
+@pytest.mark.parametrize("nh,nkv,hd,S,n,rows", [(32, 4, 64, 4, 1, 64), (32, 4, 64, 1, 1, 1000), (8, 1, 64, 2, 1, 25),
+                                                (4, 4, 64, 1, 2, 500), (32, 4, 32, 3, 1, 64), (32, 4, 128, 2, 1, 99),
+                                                (16, 2, 64, 2, 3, 400), (8, 1, 256, 1, 1, 300)])
+def test_tree_many_padding_rows(nh, nkv, hd, S, n, rows, kvb):
+    """Many more rows than the sequences' nodes: a batch padded to a fixed size."""
+    rng = np.random.default_rng(rows + hd)
+    kb, vb = kvb
+    lens, trees, M = [70 + 9 * i for i in range(S)], [bush(rng, n) for _ in range(S)], 120
+    starts, parents = list(range(0, S * n + 1, n)), [x for p in trees for x in p]
+    q, k, v = rnd(rng, rows, nh * hd), rnd(rng, S * M, nkv * hd), rnd(rng, S * M, nkv * hd)
+    c, t = new_cache(S, M, nkv, hd, kb, vb)
+    at = np.arange(S * M)
+    iq.kv_write_dev(c, dev(k), dev(v), i32(at % M), S * M, seq=i32(at // M))
+    kr, vr = full(S * M, nkv * hd), full(S * M, nkv * hd)
+    iq.kv_read_dev(kr, vr, c, i32(at % M), S * M, seq=i32(at // M))
+    got = run_tree(dev(q), t, kvb, lens, starts, parents + [-1] * (rows - S * n), nh)
+    kr, vr = (list(x.cpu().numpy().reshape(S, M, nkv, hd)) for x in (kr, vr))
+    want = ref.tree(q[:S * n].reshape(S * n, nh, hd), kr, vr, lens, starts, parents, nh)
+    assert (got[:S * n] == want.reshape(S * n, -1)).all() and (got[S * n:] == KEEP).all()
