@@ -22,6 +22,7 @@ static int g_last_cuda = 0;
 
 int cuda_fail(cudaError_t e) {
     g_last_cuda = (int)e;
+    cudaGetLastError();   // answered here: the next call's launch check must not find it again
     if (e == cudaErrorMemoryAllocation) return IQ_ERR_OOM;
     if (e == cudaErrorNoDevice || e == cudaErrorInsufficientDriver ||
         e == cudaErrorNoKernelImageForDevice || e == cudaErrorInvalidDevice)

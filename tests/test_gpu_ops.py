@@ -914,3 +914,16 @@ def test_tree_many_padding_rows(nh, nkv, hd, S, n, rows, kvb):
     kr, vr = (list(x.cpu().numpy().reshape(S, M, nkv, hd)) for x in (kr, vr))
     want = ref.tree(q[:S * n].reshape(S * n, nh, hd), kr, vr, lens, starts, parents, nh)
     assert (got[:S * n] == want.reshape(S * n, -1)).all() and (got[S * n:] == KEEP).all()
+
+
+def test_a_failed_call_is_not_reported_again():
+    """An allocation that the device refuses fails its own call; the next call is answered for itself."""
+    x = dev(np.zeros((1, 8), np.int64))
+    rng = np.zeros((8192, 2), np.uint64)
+    with pytest.raises(iq.IQError) as e:
+        iq.sample_dev(x, 8192, (1 << 31) - 1, ONE, 0, 0, rng)     # 140 TB of work space: nothing is launched
+    assert e.value.status == -3
+    iq.softmax_dev(x, 1, 8)
+    logp = full(1)
+    iq.logprobs_dev(x, 1, 8, i32([3]), logp)
+    assert int(logp[0]) == ref.logprobs([ONE // 8] * 8, 3, 0)[0]
