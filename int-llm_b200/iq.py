@@ -152,6 +152,14 @@ def _dp(t):
 _CUDA_STREAM_LEGACY = 0x1
 
 
+def _handle(stream):
+    """Handle of an explicit stream: a torch stream's, or a number (0: the library's own
+    stream). torch's default stream has handle 0, which the library would read as its
+    own: name the legacy default stream (cudaStreamLegacy) instead."""
+    h = getattr(stream, "cuda_stream", None)
+    return stream if h is None else h or _CUDA_STREAM_LEGACY
+
+
 def _sp(stream):
     """Stream argument: an explicit stream, else torch's current stream when torch
     has initialised CUDA (so device calls order with the tensors' producers),
@@ -160,12 +168,9 @@ def _sp(stream):
         import sys
         t = sys.modules.get("torch")
         if t is not None and t.cuda.is_initialized():
-            h = t.cuda.current_stream().cuda_stream
-            # torch's default stream has handle 0, which the library would read as
-            # "its own stream": name the legacy default stream (cudaStreamLegacy) instead
-            return ctypes.c_void_p(h if h else _CUDA_STREAM_LEGACY)
+            return ctypes.c_void_p(_handle(t.cuda.current_stream()))
         return None
-    return ctypes.c_void_p(getattr(stream, "cuda_stream", stream))
+    return ctypes.c_void_p(_handle(stream))
 
 
 # ---------------------------------------------------------------- host API
@@ -387,7 +392,7 @@ def _cur(stream):
         if _raw_device is None:
             _bind_torch()
         return _raw_stream(_raw_device()) or _CUDA_STREAM_LEGACY
-    return getattr(stream, "cuda_stream", stream)
+    return _handle(stream)
 
 
 def _ref(x):

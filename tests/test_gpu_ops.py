@@ -927,3 +927,23 @@ def test_a_failed_call_is_not_reported_again():
     logp = full(1)
     iq.logprobs_dev(x, 1, 8, i32([3]), logp)
     assert int(logp[0]) == ref.logprobs([ONE // 8] * 8, 3, 0)[0]
+
+
+def test_torch_default_stream_given_explicitly():
+    """Calls on torch.cuda.default_stream() follow what torch has queued there, and torch follows them."""
+    rng = np.random.default_rng(28)
+    x = dev(rnd(rng, 2000, 4096))
+    cos, sin, pos = dev(rnd(rng, 5, 32)), dev(rnd(rng, 5, 32)), i32([3] * 2000)
+    want, out, y = full(2000, 4096), full(2000, 4096), torch.zeros_like(x)
+    rope = iq.Rope(cos, sin, pos, 5, 64)
+    iq.rope_dev(want, x, rope, 2000, 64, 64)
+    torch.cuda.synchronize()
+    s = torch.cuda.default_stream()
+    for _ in range(20):
+        y.zero_()
+        for _ in range(8):
+            y.add_(x, alpha=3)
+        y.sub_(x, alpha=23)                 # 24 x - 23 x, last of ten passes over y
+        iq.rope_dev(out, y, rope, 2000, 64, 64, stream=s)
+        assert torch.equal(out, want)
+        out.fill_(KEEP)

@@ -286,3 +286,15 @@ def test_code_from_a_lowered_quotient():
     for M in (0, 1, ONE, (1 << 61) - 1):
         assert ref.pack([M, ref.I64_MIN, -M], 8) == ([255 if M else 0, 0, 0], M)
         assert ref.wrap(ref.I64_MIN + M) < 0 <= min(-M + M, M + M)
+
+
+def test_explicit_streams():
+    """torch's default stream (handle 0) is the legacy default stream, not the library's own; numbers go through."""
+    class Stream:
+        def __init__(self, handle):
+            self.cuda_stream = handle
+
+    assert iq._cur(Stream(0)) == 1 and iq._sp(Stream(0)).value == 1
+    assert iq._cur(Stream(0x70)) == 0x70 and iq._sp(Stream(0x70)).value == 0x70
+    for handle in (0, 1, 0x70):
+        assert iq._cur(handle) == handle and (iq._sp(handle).value or 0) == handle
