@@ -131,10 +131,9 @@ def lib():
 
 
 def _call(name, *args):
-    L = lib()
-    rc = getattr(L, name)(*args)
+    rc = getattr(_lib or lib(), name)(*args)
     if rc != 0:
-        raise IQError(name, rc, L)
+        raise IQError(name, rc, _lib)
     return rc
 
 
@@ -360,45 +359,80 @@ def softmax_dev(x, rows, n, stream=None):
 
 # ------------------------- drafted tokens: rotary, cache, tree attention, scores
 
-_raw_device = _raw_stream = None   # torch's current device and stream handle, bound at the first call
+_raw_device = _raw_stream = None     # torch's current device and stream handle, bound at the first call
+_i8 = _i16 = _i32 = _i64 = ()        # types of operands of 1, 2, 4 and 8 bytes
 
 
 def _bind_torch():
-    global _raw_device, _raw_stream
+    global _raw_device, _raw_stream, _i8, _i16, _i32, _i64
     import torch
-    _raw_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    _raw_device, _raw_stream = _raw_device or torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    _i8, _i16 = (torch.uint8, torch.int8), (torch.int16, torch.uint16)
+    _i32, _i64 = (torch.int32, torch.uint32), (torch.int64, torch.uint64)
 
 
-def _dev_ptr(t, itemsize, name):
-    """Device pointer of t (None: NULL) after checking its element size and that
-    it lies on the device that calls go to (torch's current one)."""
-    if t is None:
-        return None
-    if t.element_size() != itemsize:
-        raise ValueError(f"{name}: {itemsize}-byte elements expected, got {t.element_size()}")
-    dev = t.get_device()
-    if dev < 0:
-        raise ValueError(f"{name} must be in device memory, got {t.device}")
-    if _raw_device is None:
+def _device():
+    """The device that calls go to: torch's current one (None without a GPU)."""
+    if _raw_device is None or not _i8:
         _bind_torch()
-    if dev != _raw_device():
-        raise ValueError(f"{name} lies on {t.device}, calls go to device {_raw_device()}")
-    return t.data_ptr()
+    try:
+        return _raw_device()
+    except RuntimeError:
+        return None
 
 
-def _cur(stream):
-    """Stream argument as _sp's: an explicit one, else torch's current stream."""
-    if stream is None:
-        if _raw_device is None:
-            _bind_torch()
-        return _raw_stream(_raw_device()) or _CUDA_STREAM_LEGACY
-    return _handle(stream)
+def _dev_ptr(t, types, dev, name, n, width=0, rows=1, ld=0):
+    """Device pointer of t (None: NULL) after checking that it has one of the types, lies on the device `dev`
+    and holds what the call takes there: n elements side by side or, in a tensor that is not contiguous,
+    `rows` rows of `width` elements ld apart (n = (rows - 1) ld + width)."""
+    if t is not None:
+        if t.dtype in types and t.get_device() == dev and (
+                t.numel() >= n if t.is_contiguous() else _holds(t, width or n, rows, ld)):
+            return t.data_ptr()
+        raise ValueError(_refusal(t, types, dev, name, n, width or n, rows, ld))
 
 
-def _ref(x):
-    """x (a Rope or KVCache) by reference, after checking that its tensors lie where calls go to."""
-    if x.dev is not None and x.dev != _raw_device():
-        raise ValueError(f"{type(x).__name__} of device {x.dev}, calls go to device {_raw_device()}")
+def _refusal(t, types, dev, name, n, width, rows, ld):
+    if t.dtype not in types:
+        return f"{name}: one of {types} expected, got {t.dtype}"
+    if t.is_contiguous() and t.numel() < n:
+        return f"{name} holds {t.numel()} elements, {n} expected"
+    if not t.is_contiguous() and not _holds(t, width, rows, ld):
+        return (f"{name}: {rows} rows of {width} elements, {ld} apart, expected, got shape {tuple(t.shape)} with "
+                f"strides {t.stride()}")
+    return f"{name} must be in memory of the device {dev}, where calls go to, got {t.device}"
+
+
+def _holds(t, width, rows, ld):
+    """Whether the strided t holds `rows` rows of `width` elements side by side, ld elements apart: its
+    last dimensions as one row or several, the ones before as their number."""
+    shape, steps, n, r = t.shape, t.stride(), 1, 1
+    if len(steps) == 2 and steps[1] == 1 and (steps[0] == ld or rows <= 1):   # columns of a matrix, as of a fused q|k|v
+        return shape[0] >= rows and shape[1] >= width
+    for size, step in zip(reversed(shape), reversed(steps)):
+        if size == 1:
+            continue
+        if r == 1 and step == n:
+            n *= size
+        elif step == ld * r:
+            r *= size
+        else:
+            break
+    return rows < 1 or n >= (rows - 1) * ld + width or (n >= width and r >= rows)
+
+
+def _cur(stream, dev=None):
+    """Stream argument as _sp's: an explicit one, else torch's current stream on `dev`."""
+    return _raw_stream(dev) or _CUDA_STREAM_LEGACY if stream is None else _handle(stream)
+
+
+def _ref(x, dev, rows=0):
+    """x (a Rope or KVCache) by reference, after checking that its tensors lie where calls go to and
+    that a Rope has the positions of `rows` rows."""
+    if x.dev is not None and x.dev != dev:
+        raise ValueError(f"{type(x).__name__} of device {x.dev}, calls go to device {dev}")
+    if rows and rows > x.rows:
+        raise ValueError(f"Rope of {x.rows} positions, {rows} rows")
     return ctypes.byref(x)
 
 
@@ -412,13 +446,13 @@ class _RopeScaling(ctypes.Structure):
 
 def rope_tables_dev(cos, sin, rot_dim, n_pos, theta, scaling=None, stream=None):
     """Tables [n_pos][rot_dim / 2]; scaling: dict of kind, factor, orig_len, low, high, mscale (Q16.48 ints)."""
-    sc = None
+    sc, dev, n = None, _device(), n_pos * (rot_dim // 2)
     if scaling is not None:
         f = dict(scaling)
         f["kind"] = ROPE_SCALE[f.get("kind", "none")]
         sc = ctypes.byref(_RopeScaling(**f))
-    _call("iq_rope_tables_dev", _dev_ptr(cos, 8, "cos"), _dev_ptr(sin, 8, "sin"), rot_dim, n_pos, theta, sc,
-          _cur(stream))
+    _call("iq_rope_tables_dev", _dev_ptr(cos, _i64, dev, "cos", n), _dev_ptr(sin, _i64, dev, "sin", n), rot_dim, n_pos,
+          theta, sc, _cur(stream, dev))
 
 
 class Rope(ctypes.Structure):
@@ -426,16 +460,20 @@ class Rope(ctypes.Structure):
     _fields_ = [("d_cos", _P), ("d_sin", _P), ("d_pos", _P), ("n_pos", _I), ("rot_dim", _I), ("layout", _I)]
 
     def __init__(self, cos, sin, pos, n_pos, rot_dim, layout="half"):
-        super().__init__(_dev_ptr(cos, 8, "cos"), _dev_ptr(sin, 8, "sin"), _dev_ptr(pos, 4, "pos"), n_pos, rot_dim,
-                         ROPE_LAYOUT[layout])
+        dev, n, rows = _device(), n_pos * (rot_dim // 2), 0 if pos is None else pos.numel()
+        super().__init__(_dev_ptr(cos, _i64, dev, "cos", n), _dev_ptr(sin, _i64, dev, "sin", n),
+                         _dev_ptr(pos, _i32, dev, "pos", rows), n_pos, rot_dim, ROPE_LAYOUT[layout])
         self.keep = (cos, sin, pos)
-        self.dev = None if cos is None else cos.get_device()
+        self.dev = None if cos is None else dev
+        self.rows = rows
 
 
 def rope_dev(out, x, rope, rows, heads, head_dim, x_stride=None, out_stride=None, stream=None):
-    w = heads * head_dim
-    _call("iq_rope_dev", _dev_ptr(out, 8, "out"), _dev_ptr(x, 8, "x"), _ref(rope), rows, heads, head_dim,
-          w if x_stride is None else x_stride, w if out_stride is None else out_stride, _cur(stream))
+    dev, w = _device(), heads * head_dim
+    xs, outs = w if x_stride is None else x_stride, w if out_stride is None else out_stride
+    _call("iq_rope_dev", _dev_ptr(out, _i64, dev, "out", (rows - 1) * outs + w, w, rows, outs),
+          _dev_ptr(x, _i64, dev, "x", (rows - 1) * xs + w, w, rows, xs),
+          _ref(rope, dev, rows), rows, heads, head_dim, xs, outs, _cur(stream, dev))
 
 
 class KVCache(ctypes.Structure):
@@ -445,24 +483,29 @@ class KVCache(ctypes.Structure):
 
     def __init__(self, seqs, max_seq, kv_heads, head_dim, k=None, v=None, kq=None, vq=None, k_mag=None, v_mag=None,
                  k_bits=0, v_bits=0):
-        super().__init__(seqs, max_seq, kv_heads, head_dim, k_bits, v_bits, _dev_ptr(k, 8, "k"), _dev_ptr(v, 8, "v"),
-                         _dev_ptr(kq, 1, "kq"), _dev_ptr(vq, 2, "vq"), _dev_ptr(k_mag, 8, "k_mag"),
-                         _dev_ptr(v_mag, 8, "v_mag"))
+        dev, m = _device(), seqs * max_seq * kv_heads
+        n = m * head_dim
+        super().__init__(seqs, max_seq, kv_heads, head_dim, k_bits, v_bits, _dev_ptr(k, _i64, dev, "k", n),
+                         _dev_ptr(v, _i64, dev, "v", n), _dev_ptr(kq, _i8, dev, "kq", n),
+                         _dev_ptr(vq, _i16, dev, "vq", n), _dev_ptr(k_mag, _i64, dev, "k_mag", m),
+                         _dev_ptr(v_mag, _i64, dev, "v_mag", m))
         self.keep = (k, v, kq, vq, k_mag, v_mag)
-        t = kq if k is None else k
-        self.dev = None if t is None else t.get_device()
+        self.dev = None if k is None and kq is None else dev
 
 
 def kv_write_dev(cache, k, v, slot, rows, seq=None, rope=None, k_stride=None, v_stride=None, stream=None):
-    w = cache.kv_heads * cache.head_dim
-    _call("iq_kv_write_dev", _ref(cache), _dev_ptr(k, 8, "k"), _dev_ptr(v, 8, "v"), _dev_ptr(seq, 4, "seq"),
-          _dev_ptr(slot, 4, "slot"), rows, w if k_stride is None else k_stride, w if v_stride is None else v_stride,
-          None if rope is None else _ref(rope), _cur(stream))
+    dev, w = _device(), cache.kv_heads * cache.head_dim
+    ks, vs = w if k_stride is None else k_stride, w if v_stride is None else v_stride
+    _call("iq_kv_write_dev", _ref(cache, dev), _dev_ptr(k, _i64, dev, "k", (rows - 1) * ks + w, w, rows, ks),
+          _dev_ptr(v, _i64, dev, "v", (rows - 1) * vs + w, w, rows, vs), _dev_ptr(seq, _i32, dev, "seq", rows),
+          _dev_ptr(slot, _i32, dev, "slot", rows), rows, ks, vs, None if rope is None else _ref(rope, dev, rows),
+          _cur(stream, dev))
 
 
 def kv_read_dev(k, v, cache, slot, rows, seq=None, stream=None):
-    _call("iq_kv_read_dev", _dev_ptr(k, 8, "k"), _dev_ptr(v, 8, "v"), _ref(cache), _dev_ptr(seq, 4, "seq"),
-          _dev_ptr(slot, 4, "slot"), rows, _cur(stream))
+    dev, n = _device(), rows * cache.kv_heads * cache.head_dim
+    _call("iq_kv_read_dev", _dev_ptr(k, _i64, dev, "k", n), _dev_ptr(v, _i64, dev, "v", n), _ref(cache, dev),
+          _dev_ptr(seq, _i32, dev, "seq", rows), _dev_ptr(slot, _i32, dev, "slot", rows), rows, _cur(stream, dev))
 
 
 def attn_tree_work(cache, num_heads, n_seq, rows, max_nodes, max_len):
@@ -474,20 +517,28 @@ def attn_tree_work(cache, num_heads, n_seq, rows, max_nodes, max_len):
 
 def attn_tree_dev(out, q, cache, num_heads, lens, starts, parents, n_seq, rows, max_nodes, max_len, work=None,
                   seqs=None, q_stride=None, stream=None):
-    """Tree attention; work: a device tensor of at least attn_tree_work(...) bytes."""
-    nbytes = 0 if work is None else work.numel() * work.element_size()
-    _call("iq_attn_tree_dev", _dev_ptr(out, 8, "out"), _dev_ptr(q, 8, "q"), _ref(cache), num_heads,
-          _dev_ptr(seqs, 4, "seqs"), _dev_ptr(lens, 4, "lens"), _dev_ptr(starts, 4, "starts"),
-          _dev_ptr(parents, 4, "parents"), n_seq, rows, max_nodes, max_len,
-          num_heads * cache.head_dim if q_stride is None else q_stride,
-          None if work is None else _dev_ptr(work, work.element_size(), "work"), nbytes, _cur(stream))
+    """Tree attention; work: a contiguous device tensor of at least attn_tree_work(...) bytes."""
+    dev, w = _device(), num_heads * cache.head_dim
+    qs = w if q_stride is None else q_stride
+    n = nbytes = 0
+    if work is not None:
+        n = work.numel()
+        nbytes = n * work.element_size()
+    _call("iq_attn_tree_dev", _dev_ptr(out, _i64, dev, "out", rows * w),
+          _dev_ptr(q, _i64, dev, "q", (rows - 1) * qs + w, w, rows, qs), _ref(cache, dev), num_heads,
+          _dev_ptr(seqs, _i32, dev, "seqs", n_seq), _dev_ptr(lens, _i32, dev, "lens", n_seq),
+          _dev_ptr(starts, _i32, dev, "starts", n_seq + 1), _dev_ptr(parents, _i32, dev, "parents", rows), n_seq, rows,
+          max_nodes, max_len, qs, None if work is None else _dev_ptr(work, (work.dtype,), dev, "work", n), nbytes,
+          _cur(stream, dev))
 
 
 def logprobs_dev(logits, rows, vocab, tokens=None, logp=None, entropy=None, top=0, top_ids=None, top_logp=None,
                  ld=None, stream=None):
-    _call("iq_logprobs_dev", _dev_ptr(logits, 8, "logits"), vocab if ld is None else ld, rows, vocab,
-          _dev_ptr(tokens, 4, "tokens"), _dev_ptr(logp, 8, "logp"), _dev_ptr(entropy, 8, "entropy"), top,
-          _dev_ptr(top_ids, 4, "top_ids"), _dev_ptr(top_logp, 8, "top_logp"), _cur(stream))
+    dev, ld = _device(), vocab if ld is None else ld
+    _call("iq_logprobs_dev", _dev_ptr(logits, _i64, dev, "logits", (rows - 1) * ld + vocab, vocab, rows, ld), ld, rows,
+          vocab, _dev_ptr(tokens, _i32, dev, "tokens", rows), _dev_ptr(logp, _i64, dev, "logp", rows),
+          _dev_ptr(entropy, _i64, dev, "entropy", rows), top, _dev_ptr(top_ids, _i32, dev, "top_ids", rows * top),
+          _dev_ptr(top_logp, _i64, dev, "top_logp", rows * top), _cur(stream, dev))
 
 
 # --------------------------------------------------------- synthetic inputs

@@ -298,3 +298,117 @@ def test_explicit_streams():
     assert iq._cur(Stream(0x70)) == 0x70 and iq._sp(Stream(0x70)).value == 0x70
     for handle in (0, 1, 0x70):
         assert iq._cur(handle) == handle and (iq._sp(handle).value or 0) == handle
+
+
+class _Binding:
+    """The binding with host memory as its device and its calls recorded, not made."""
+
+    def __init__(self, monkeypatch):
+        import torch
+        self.t, self.calls = torch, []
+        monkeypatch.setattr(iq, "_raw_device", lambda: -1)      # a host tensor's device number
+        monkeypatch.setattr(iq, "_call", lambda *a: self.calls.append(a))
+
+    def q(self, *shape):
+        return self.t.zeros(*shape, dtype=self.t.int64)
+
+    def i(self, n):
+        return self.t.zeros(n, dtype=self.t.int32)
+
+
+OPERANDS = [(op, name) for op, names in dict(
+    tables="cos sin", rope_of="cos sin pos", rope="out x", cache="k v", packed="kq vq k_mag v_mag",
+    write="k v seq slot", read="k v seq slot", tree="out q seqs lens starts parents",
+    logprobs="logits tokens logp entropy top_ids top_logp").items() for name in names.split()]
+
+
+def _make(b, op):
+    """(operands of a call by name, the call)"""
+    q, i, t = b.q, b.i, b.t
+    if op == "tables":
+        return dict(cos=q(6, 4), sin=q(6, 4)), lambda a: iq.rope_tables_dev(a["cos"], a["sin"], 8, 6, 10000, stream=1)
+    if op == "rope_of":
+        return dict(cos=q(6, 4), sin=q(6, 4), pos=i(3)), lambda a: iq.rope_dev(
+            q(3, 16), q(3, 16), iq.Rope(a["cos"], a["sin"], a["pos"], 6, 8), 3, 2, 8, stream=1)
+    if op == "rope":
+        r = iq.Rope(q(6, 4), q(6, 4), i(3), 6, 8)
+        return dict(out=q(3, 16), x=q(3, 16)), lambda a: iq.rope_dev(a["out"], a["x"], r, 3, 2, 8, stream=1)
+    if op == "cache":
+        return dict(k=q(2, 5, 2, 8), v=q(2, 5, 2, 8)), lambda a: iq.KVCache(2, 5, 2, 8, **a)
+    if op == "packed":
+        n = (2, 5, 2, 8)
+        return dict(kq=t.zeros(n, dtype=t.uint8), vq=t.zeros(n, dtype=t.int16), k_mag=q(2, 5, 2), v_mag=q(2, 5, 2)), \
+            lambda a: iq.KVCache(2, 5, 2, 8, k_bits=8, v_bits=10, **a)
+    c = iq.KVCache(2, 5, 2, 8, q(2, 5, 2, 8), q(2, 5, 2, 8))
+    if op == "write":
+        return dict(k=q(3, 16), v=q(3, 16), slot=i(3), seq=i(3)), \
+            lambda a: iq.kv_write_dev(c, a["k"], a["v"], a["slot"], 3, seq=a["seq"], stream=1)
+    if op == "read":
+        return dict(k=q(3, 16), v=q(3, 16), slot=i(3), seq=i(3)), \
+            lambda a: iq.kv_read_dev(a["k"], a["v"], c, a["slot"], 3, seq=a["seq"], stream=1)
+    if op == "tree":
+        return dict(out=q(3, 32), q=q(3, 32), lens=i(2), starts=i(3), parents=i(3), seqs=i(2)), \
+            lambda a: iq.attn_tree_dev(cache=c, num_heads=4, n_seq=2, rows=3, max_nodes=2, max_len=5, work=q(100),
+                                       stream=1, **a)
+    return dict(logits=q(3, 50), tokens=i(3), logp=q(3), entropy=q(3), top_ids=i(12), top_logp=q(3, 4)), \
+        lambda a: iq.logprobs_dev(a["logits"], 3, 50, a["tokens"], a["logp"], a["entropy"], 4, a["top_ids"],
+                                  a["top_logp"], stream=1)
+
+
+@pytest.mark.parametrize("op,name", OPERANDS)
+def test_binding_refuses_wrong_operands(op, name, monkeypatch):
+    """An operand that is one element short, of real numbers, scattered in memory, repeated or elsewhere is refused
+    before the library sees its address; the right one passes."""
+    b = _Binding(monkeypatch)
+    args, call = _make(b, op)
+    call(args)
+    x, n = args[name], len(b.calls)
+    real = {1: b.t.float8_e4m3fn, 2: b.t.bfloat16, 4: b.t.float32, 8: b.t.float64}[x.element_size()]
+    twice = b.t.zeros(2 * x.numel(), dtype=x.dtype)
+    for bad, why in ((x.flatten()[1:], "expected|3 rows"), (x.to(real), "one of"), (twice[::2], "strides"),
+                     (x.flatten()[:1].expand(x.numel()), "strides")):
+        with pytest.raises(ValueError, match=f"{name}.*{why}" if why != "expected|3 rows" else why):
+            call(dict(args, **{name: bad}))
+    assert len(b.calls) == n
+    monkeypatch.setattr(iq, "_raw_device", lambda: 0)
+    with pytest.raises(ValueError, match="memory of the device 0|of device"):
+        call(args)
+    monkeypatch.setattr(iq, "_raw_device", lambda: -1)
+    call(dict(args, **{name: twice[1:x.numel() + 1]}))       # a longer or flat one in one piece is right
+
+
+def test_binding_row_layouts(monkeypatch):
+    """Row operands: contiguous by length, views by their strides; a Rope by its rows; a work space in one piece."""
+    b = _Binding(monkeypatch)
+    q = b.q
+    rope = iq.Rope(q(6, 4), q(6, 4), b.i(6), 6, 8)
+    out = q(6, 16)
+
+    def x(t, ld, rows=6):
+        iq.rope_dev(out, t, rope, rows, 2, 8, x_stride=ld, stream=1)
+        assert b.calls.pop()[2] == t.data_ptr()
+
+    x(q(6, 40)[:, 8:24], 40)
+    x(q(6, 40)[:, 8:], 40)
+    x(q(6, 5, 8)[:, 1:3], 40)                       # heads of a fused row
+    x(q(2, 3, 40)[:, :, :16], 40)                   # rows in two dimensions
+    x(q(12, 16)[::2], 32)
+    x(q(2, 200)[:, :96].view(2, 6, 16), 16)         # rows side by side in the last dimensions
+    x(q(5 * 40 + 16), 40)                           # ends with the last row
+    x(q(1, 40)[:, 3:19], 16, rows=1)
+    x(q(4, 40)[:, :16], 99, rows=1)                 # one row: no distance
+    x(q(4, 40)[:, :16], 40, rows=0)
+    for t, ld, rows in ((q(5 * 40 + 15), 40, 6), (q(5, 40)[:, :16], 40, 6), (q(6, 40)[:, :15], 40, 6),
+                        (q(6, 40)[:, :16], 16, 6), (q(16, 6).t(), 16, 6), (q(16, 16).t(), 16, 6),
+                        (q(2, 4, 40)[:, :3, :16], 40, 6), (q(2, 200)[:, :80].view(2, 5, 16), 16, 6),
+                        (q(1, 16).expand(6, 16), 16, 6), (q(6, 8, 5)[:, :, :2], 40, 6), (q(32)[::2], 16, 1),
+                        (q(7, 16), 16, 7)):
+        with pytest.raises(ValueError):
+            iq.rope_dev(q(7, 16), t, rope, rows, 2, 8, x_stride=ld, stream=1)
+    c = iq.KVCache(1, 5, 2, 8, q(1, 5, 2, 8), q(1, 5, 2, 8))
+    call = lambda w: iq.attn_tree_dev(q(32), q(32), c, 4, b.i(1), b.i(2), b.i(1), 1, 1, 1, 5, w, stream=1)  # noqa: E731
+    call(q(10))
+    assert b.calls.pop()[14:16][-1] == 80
+    for w in (q(20)[::2], q(1).expand(100)):
+        with pytest.raises(ValueError, match="work"):
+            call(w)
