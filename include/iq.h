@@ -312,16 +312,17 @@ IQ_API int iq_attn_tree_dev(int64_t *d_out, const int64_t *d_q, const iq_kv_cach
                             void *stream);
 
 /* Log probabilities of rows of logits (d_logits row r at r * ld; vocab <=
- * 2^20) in Q16.48 nats. With m = max l, d = m - l, E(d) = e^-d rounded down to
- * Q16.48 (within 2^-44 relative above 2^-48, no cut-off at 10 as in
- * fp_safe_exp) and S = sum E(d):
+ * 2^20) in Q16.48 nats. With m = max l, d = m - l, E(d) = e^-d in Q16.48
+ * ((1 - 2^-44) e^-d - 2^-48 <= E(d) <= (1 + 2^-44) e^-d, E(0) = 1, 0 from d = 34
+ * on; no cut-off at 10 as in fp_safe_exp) and S = sum E(d):
  *   d_logp[r] = -d_token - ln S for the row's given token (d_tokens NULL: none),
  *   d_entropy[r] = ln S + (sum fp_mul(E(d), d)) / S (may be NULL),
  *   d_top_ids, d_top_logp [rows][top]: the `top` (0..32) largest logits in
  *   falling order, equal ones by rising index, and their log probabilities.
  * A log probability below INT64_MIN is INT64_MIN. Every step is a whole-number
  * operation, so results are the same on every run and machine. A token outside
- * the vocabulary leaves d_logp[r] as it was. */
+ * the vocabulary leaves d_logp[r] as it was (the row's entropy and alternatives
+ * do not depend on it and are written). */
 IQ_API int iq_logprobs_dev(const int64_t *d_logits, int64_t ld, int rows, int vocab, const int *d_tokens,
                            int64_t *d_logp, int64_t *d_entropy, int top, int *d_top_ids, int64_t *d_top_logp,
                            void *stream);

@@ -84,8 +84,9 @@ __device__ __forceinline__ void cordic(const RopeTab &t, int64_t &x, int64_t &y,
 // product (p < 2^24, th <= 2^48): a double estimate of the quotient is within
 // one of it, and the wrapped remainder is exact, so it equals fp_sincos's
 // repeated subtraction at the positions where that has no overflow.
-// Issue-bound on the 48 CORDIC steps, not on the 16 bytes an entry writes: 65536
-// positions of 64 pairs 154 us (67 MB would take 10), with 64-bit steps throughout 199.
+// Bound by the 48 CORDIC steps, each waiting for the one before, not by the 16 bytes an
+// entry writes: 65536 positions of 64 pairs 154 us (67 MB would take 10; 109 M warp
+// instructions, 62 % of the issue slots), with 64-bit steps throughout 199.
 __global__ void __launch_bounds__(256) k_rope_tables(int64_t *__restrict__ cs, int64_t *__restrict__ sn,
                                                      const __grid_constant__ RopeTab t) {
     __shared__ int64_t th[128];

@@ -118,8 +118,9 @@ struct LpArgs {
 // of the slice's n-th largest logit; the few logits not below it are ranked by
 // counting. Where more than LP_CAND reach it (many equal logits) the slice is searched
 // n times instead. CTA 0 ranks the slices' lists the same way. Measured: one row of
-// 32000 15 us, the latency of its steps in turn; 512 rows 89 us, about 80 instructions a logit
-// in chains of doubles (issue 47 %), 256 MB read in two passes (39 us).
+// 32000 15 us, the latency of its steps in turn; 512 rows 89 us: 40 M warp
+// instructions (35 us at full issue) in chains of doubles and 256 MB read in two passes (39 us), which hardly
+// overlap, since all rows are on the GPU at once and read and compute in step.
 #define LP_T 256
 #define LP_CAND 512
 

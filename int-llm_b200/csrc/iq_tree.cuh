@@ -238,7 +238,7 @@ __host__ __device__ constexpr size_t tree_scores_smem(int NT, int hd) { return 1
 // Two CTAs an SM (three with 8 columns; four would spill: 92 us for 88 with
 // 64 single tokens) overlap one another's loads, products and epilogues; TMEM holds
 // 128 NT columns a CTA. Measured: 64 single tokens at 2000 positions (32 heads over 4 of
-// 64) 88 us, 260 MB of keys at 3.0 TB/s; 8 drafts of 16-48 nodes 140 us, of which the
+// 64) 88 us, 260 MB of keys at 3.0 TB/s; 8 drafts of 16-48 nodes 143 us, of which the
 // tensor cores need 25: issue (47 %) of the byte planes and the epilogue bounds it; from
 // the packed cache 69 us (2 drafts, 32 heads of 128).
 template <int NT, bool PK, bool W>
@@ -520,8 +520,8 @@ __device__ __noinline__ void tree_wrapped(const TreeArgs &a, const TreeSeq &s, i
 // score 11 below the maximum, whose exponential is 0, so that one loop serves
 // all. A row whose score differences wrap (the reference's int64 then gives other
 // numbers, reproduced here) is finished here term by term and leaves zeros to
-// k_tree_pv. Measured: 105 us for the 12.7 M (row, head, position) of 8 drafts of 16-48
-// nodes, issue 64 %: about 165 instructions each, most of them 12 squarings of two fused
+// k_tree_pv. Measured: 102 us for the 13.6 M (row, head, position) of 8 drafts of 16-48
+// nodes, issue 66 %: about 160 instructions each, most of them 12 squarings of two fused
 // multiply-adds, 2 in 32-bit pieces and 2 quotients.
 #define TREE_SM_T 128
 #define TREE_SM_MAX 2560   // positions whose scores are kept in shared memory
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(TREE_SM_T, 10) k_tree_softmax(const __grid_con
 // from a multiple of 128, which puts the four positions (or columns) of a
 // quarter-warp on different banks. Else the lanes read global memory themselves (scores
 // and values so: 263 us for 175 with 64 single tokens, 427 for 339 with 8 drafts).
-// Measured: 64 single tokens 54 us (292 MB, 5.5 TB/s); 8 drafts 111 us, 43 % of the FP64
+// Measured: 64 single tokens 54 us (292 MB, 5.5 TB/s); 8 drafts 115 us, 42 % of the FP64
 // rate of 64 terms a clock and SM; the rest is conversions and waiting for tiles (issue 42 %).
 struct TreeTile { int vrow, vpitch, ppitch, bytes; };   // bytes of a stage
 template <bool PK>
