@@ -222,7 +222,8 @@ IQ_API int iq_softmax_dev(int64_t *d_x, int rows, int n, void *stream);
  * library up). Index arrays are read on the device: a row whose index lies
  * outside its range is left out and its outputs stay as they were. A negative
  * index is the mark of a padding row; any other bad index is also recorded as
- * IQ_ERR_RANGE in the device status (iq_device_status). */
+ * IQ_ERR_RANGE in the device status (iq_device_status). Without rows there is
+ * nothing to do, and the rows' pointers may be NULL. */
 
 /* Rotary tables scaled for contexts beyond the trained one. The frequency of
  * pair i is th_i = fp_exp(fp_mul(-fp_div(2i, rot_dim), ln theta))

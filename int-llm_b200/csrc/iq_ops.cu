@@ -294,14 +294,14 @@ IQ_API int iq_rope_tables_dev(int64_t *d_cos, int64_t *d_sin, int rot_dim, int n
 IQ_API int iq_rope_dev(int64_t *d_out, const int64_t *d_x, const iq_rope *rope, int rows, int heads, int head_dim,
                        int64_t x_stride, int64_t out_stride, void *stream) {
     RopeArgs r;
-    if (!d_out || !d_x || misaligned(d_out, 8) || misaligned(d_x, 8) || rows < 0 || heads < 1 || heads > 65536 ||
-        head_dim < 1 || head_dim > 256)
-        return IQ_ERR_ARG;
+    if (rows < 0 || heads < 1 || heads > 65536 || head_dim < 1 || head_dim > 256) return IQ_ERR_ARG;
     const int64_t w = (int64_t)heads * head_dim;
-    if (x_stride < w || out_stride < w || (d_out == d_x && x_stride != out_stride)) return IQ_ERR_ARG;
+    if (x_stride < w || out_stride < w) return IQ_ERR_ARG;
+    if (rows == 0) return IQ_OK;   // (an empty tensor's pointer may be NULL)
+    if (!d_out || !d_x || misaligned(d_out, 8) || misaligned(d_x, 8) || (d_out == d_x && x_stride != out_stride))
+        return IQ_ERR_ARG;
     int dev, rc;
     if ((rc = rope_check(rope, head_dim, &r))) return rc;
-    if (rows == 0) return IQ_OK;
     if ((rc = cur_device(&dev))) return rc;
     const bool wide = rope_wide(r, head_dim) && !misaligned(d_x, 16) && !misaligned(d_out, 16) && x_stride % 2 == 0 &&
                       out_stride % 2 == 0;
@@ -323,11 +323,12 @@ IQ_API int iq_kv_write_dev(const iq_kv_cache *cache, const int64_t *d_k, const i
     int dev, rc;
     if ((rc = cache_check(cache, &c))) return rc;
     const int64_t w = (int64_t)c.nkv * c.hd;
+    if (rows < 0 || k_stride < w || v_stride < w || (int64_t)rows * c.nkv > INT_MAX / 2) return IQ_ERR_ARG;
+    if (rows == 0) return IQ_OK;
     if (!d_k || !d_v || !d_slot || misaligned(d_k, 8) || misaligned(d_v, 8) || misaligned(d_slot, 4) ||
-        misaligned(d_seq, 4) || rows < 0 || k_stride < w || v_stride < w || (int64_t)rows * c.nkv > INT_MAX / 2)
+        misaligned(d_seq, 4))
         return IQ_ERR_ARG;
     if (rope && (rc = rope_check(rope, c.hd, &r))) return rc;
-    if (rows == 0) return IQ_OK;
     if ((rc = cur_device(&dev))) return rc;
     const int64_t vecs = (int64_t)rows * c.nkv * 2;
     cudaStream_t st = pick(stream);
@@ -356,10 +357,11 @@ IQ_API int iq_kv_read_dev(int64_t *d_k, int64_t *d_v, const iq_kv_cache *cache, 
     KVArgs c;
     int dev, rc;
     if ((rc = cache_check(cache, &c))) return rc;
-    if (!d_k || !d_v || !d_slot || misaligned(d_k, 8) || misaligned(d_v, 8) || misaligned(d_slot, 4) ||
-        misaligned(d_seq, 4) || rows < 0 || (int64_t)rows * c.nkv > INT_MAX / 2)
-        return IQ_ERR_ARG;
+    if (rows < 0 || (int64_t)rows * c.nkv > INT_MAX / 2) return IQ_ERR_ARG;
     if (rows == 0) return IQ_OK;
+    if (!d_k || !d_v || !d_slot || misaligned(d_k, 8) || misaligned(d_v, 8) || misaligned(d_slot, 4) ||
+        misaligned(d_seq, 4))
+        return IQ_ERR_ARG;
     if ((rc = cur_device(&dev))) return rc;
     const bool wide = c.hd % 4 == 0 && !misaligned(d_k, 16) && !misaligned(d_v, 16) &&
                       (c.kbits ? !misaligned(c.kq, 4) && !misaligned(c.vq, 8) : !misaligned(c.k, 16) && !misaligned(c.v, 16));
@@ -415,12 +417,13 @@ IQ_API int iq_attn_tree_dev(int64_t *d_out, const int64_t *d_q, const iq_kv_cach
 IQ_API int iq_logprobs_dev(const int64_t *d_logits, int64_t ld, int rows, int vocab, const int *d_tokens,
                            int64_t *d_logp, int64_t *d_entropy, int top, int *d_top_ids, int64_t *d_top_logp,
                            void *stream) {
-    if (!d_logits || rows < 0 || vocab < 1 || ld < vocab || !d_tokens != !d_logp || top < 0 || top > vocab ||
-        (top && (!d_top_ids || !d_top_logp)) || misaligned(d_logits, 8) || misaligned(d_tokens, 4) ||
-        misaligned(d_logp, 8) || misaligned(d_entropy, 8) || misaligned(d_top_ids, 4) || misaligned(d_top_logp, 8))
-        return IQ_ERR_ARG;
+    if (rows < 0 || vocab < 1 || ld < vocab || top < 0 || top > vocab) return IQ_ERR_ARG;
     if (vocab > (1 << 20) || top > IQ_LP_MAX_TOP || rows > INT_MAX / 8) return IQ_ERR_RANGE;
     if (rows == 0) return IQ_OK;
+    if (!d_logits || !d_tokens != !d_logp || (top && (!d_top_ids || !d_top_logp)) || misaligned(d_logits, 8) ||
+        misaligned(d_tokens, 4) || misaligned(d_logp, 8) || misaligned(d_entropy, 8) || misaligned(d_top_ids, 4) ||
+        misaligned(d_top_logp, 8))
+        return IQ_ERR_ARG;
     int dev, rc;
     if ((rc = cur_device(&dev))) return rc;
     LpArgs a = {d_logits, ld, rows, vocab, top, d_tokens, d_logp, d_entropy, d_top_ids, d_top_logp, 1};

@@ -412,3 +412,28 @@ def test_binding_row_layouts(monkeypatch):
     for w in (q(20)[::2], q(1).expand(100)):
         with pytest.raises(ValueError, match="work"):
             call(w)
+
+
+def test_calls_without_rows():
+    """No rows: nothing to do, whatever the rows' pointers (an empty tensor's is NULL); sizes are checked all the same."""
+    c, r = cache(), rope(d_pos=None)
+    assert status("iq_rope_dev", None, None, r, 0, 2, 16, 32, 32, None) == 0
+    assert status("iq_kv_write_dev", c, None, None, None, None, 0, 32, 32, r, None) == 0
+    assert status("iq_kv_read_dev", None, None, c, None, None, 0, None) == 0
+    assert status("iq_logprobs_dev", None, 100, 0, 100, None, None, None, 3, None, None, None) == 0
+    assert status("iq_rope_dev", None, None, r, 0, 0, 16, 32, 32, None) == ARG
+    assert status("iq_kv_write_dev", c, None, None, None, None, 0, 31, 32, r, None) == ARG
+    assert status("iq_kv_read_dev", None, None, cache(seqs=0), None, None, 0, None) == ARG
+    assert status("iq_logprobs_dev", None, 99, 0, 100, None, None, None, 3, None, None, None) == ARG
+
+
+def test_binding_calls_without_rows(monkeypatch):
+    b = _Binding(monkeypatch)
+    q, i = b.q, b.i
+    r, c = iq.Rope(q(6, 4), q(6, 4), i(0), 6, 8), iq.KVCache(2, 5, 2, 8, q(2, 5, 2, 8), q(2, 5, 2, 8))
+    monkeypatch.undo()
+    monkeypatch.setattr(iq, "_raw_device", lambda: -1)
+    iq.rope_dev(q(0, 16), q(0, 16), r, 0, 2, 8, stream=1)
+    iq.kv_write_dev(c, q(0, 16), q(0, 16), i(0), 0, seq=i(0), rope=r, stream=1)
+    iq.kv_read_dev(q(0, 16), q(0, 16), c, i(0), 0, stream=1)
+    iq.logprobs_dev(q(0, 50), 0, 50, i(0), q(0), q(0), 3, i(0), q(0, 3), stream=1)
